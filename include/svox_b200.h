@@ -35,7 +35,8 @@ typedef enum {
     SVOXB_ERR_CUDA = 5,        /* a CUDA runtime call failed                 */
     SVOXB_ERR_TREE = 6,        /* device status: descent left the node array */
     SVOXB_ERR_MARCH = 7,       /* device status: a ray hit the step cap      */
-    SVOXB_ERR_TOO_LARGE = 8    /* size beyond a documented maximum           */
+    SVOXB_ERR_TOO_LARGE = 8,   /* size beyond a documented maximum           */
+    SVOXB_ERR_INDEX = 9        /* device status: an offset or id out of range */
 } svoxb_status;
 
 /* Data formats (svox/csrc/include/data_spec.hpp:44-49). */
@@ -386,6 +387,104 @@ int svoxb_volume_render_noalloc(const svoxb_tree* tree, const svoxb_rays* rays,
 int svoxb_march_stats(const svoxb_tree* tree, const svoxb_rays* rays,
                       const svoxb_render_options* opt, int32_t* visits, int32_t* contrib_fwd,
                       int32_t* contrib_bwd, void* stream);
+
+/* Element types of the recurrence's arrays and of what a record cache is read and written in. */
+enum { SVOXB_TYPE_F32 = 0, SVOXB_TYPE_BF16 = 1, SVOXB_TYPE_F16 = 2 };
+
+/* A gated linear recurrence over the steps of B rows (no counterpart in the
+ * reference; along a ray it is the emission and absorption that trace_ray
+ * accumulates, svox/csrc/rt_kernel.cu:261-316):
+ *     h[t] = a[t] h[t-1] + (1 - a[t]) x[t],   a = exp(-thickness)
+ * (`weighted`: + x[t]).  `values` holds C channels a step, `thickness` H of
+ * them (C a multiple of H): C / H neighbouring channels share one.  The state
+ * is kept in 32 bits whatever the types.  A step whose weight 1 - a is 0 adds
+ * nothing whatever its value, and nothing from before a step with a = 0 gets
+ * past it.
+ *   offsets == null: every row has T steps, step t of row b lies at
+ *     b * values_row + t * values_step (elements; the channels are neighbours).
+ *   else rows are packed: row b has the steps [offsets[b], offsets[b+1]) of T
+ *     (device memory, B + 1 ascending numbers; an offset out of order or
+ *     range is cut to it and recorded as SVOXB_ERR_INDEX in the device
+ *     status).  *_row is not used.
+ * `reverse`: from the last step of a row to its first.  `thickness` has the
+ * type of `values` or is float. */
+typedef struct {
+    const void* values;
+    const void* thickness;
+    const float* initial;    /* (B, C) state before the row, rows initial_row apart; null: zeros */
+    const int64_t* offsets;
+    int64_t B;
+    int64_t T;
+    int64_t values_row;
+    int64_t values_step;
+    int64_t thickness_row;
+    int64_t thickness_step;
+    int64_t initial_row;     /* 0: one state for all rows */
+    int32_t C;
+    int32_t H;
+    int32_t values_type;
+    int32_t thickness_type;
+    int32_t reverse;
+    int32_t weighted;
+} svoxb_scan;
+
+/* Floats that `kept` needs, bytes that `workspace` needs (-1: bad arguments). */
+int64_t svoxb_gated_scan_kept(const svoxb_scan* scan);
+int64_t svoxb_gated_scan_workspace(const svoxb_scan* scan, int backward);
+
+/* states: all states, contiguous like `values` without strides and in its type, or null; last:
+ * (B, C) the state after each row; kept: null, or what the backward pass needs.  Steps of a packed
+ * call that no row covers get zeros. */
+int svoxb_gated_scan(const svoxb_scan* scan, void* states, float* last, float* kept,
+                     void* workspace, void* stream);
+
+/* The gradients of sum(d_states * states) + sum(d_last * last): d_states (contiguous) and d_last may
+ * be null, and so may each output.  `kept`: from the forward call with the same arguments. */
+int svoxb_gated_scan_backward(const svoxb_scan* scan, const float* kept, const void* d_states,
+                              const float* d_last, void* d_values, void* d_thickness,
+                              float* d_initial, void* workspace, void* stream);
+
+/* Leaf records held in 8 bits (no counterpart in the reference, whose files
+ * hold fp16): of K floats the first K - 1 in groups of `group` neighbouring
+ * ones, as codes and one exponent each (value = code * 2^(exponent - 127), the
+ * smallest power of two that leaves the group's largest magnitude at most 127
+ * after rounding, or at most 448 for e4m3), the last one (the density) as
+ * fp16.  A group with a value that is not finite reads as NaN.
+ * `records` holds M N^3 records of svoxb_record_bytes each, 16-byte aligned:
+ * K - 1 codes, the exponents, and in the last two bytes the density; zeros
+ * read as zeros.  `owner`, only for writes: one zero per record, zero again
+ * after each call.  child, offset and scaling: as in svoxb_tree, only for calls
+ * that give points. */
+enum { SVOXB_CODE_INT8 = 0, SVOXB_CODE_E4M3 = 1 };
+#define SVOXB_RECORDS_MAX_K 1024
+typedef struct {
+    void* records;
+    uint32_t* owner;
+    const int32_t* child;
+    const float* offset;
+    const float* scaling;
+    int64_t M;
+    int32_t N;
+    int32_t K;
+    int32_t group;
+    int32_t code_type;
+} svoxb_records;
+
+/* Bytes of a record (-1: bad sizes). */
+int svoxb_record_bytes(int32_t K, int32_t group);
+
+/* out (Q, K) in out_type: the records of the leaves that hold the points
+ * (Q, 3), or those of the packed ids (Q), or with both null the first Q
+ * records.  An id out of range gives a row of NaN and SVOXB_ERR_INDEX in the device status. */
+int svoxb_records_read(const svoxb_records* records, const float* points, const int64_t* ids,
+                       int64_t Q, void* out, int32_t out_type, void* stream);
+
+/* Quantises row q of values (Q, K) into the record of the leaf of point q, or of
+ * ids[q], or with both null into record q.  Of several rows for one leaf the last
+ * one is written.  found: Q int64 of workspace (not used with both null).  Two calls on the same records have to be ordered by the caller. */
+int svoxb_records_write(const svoxb_records* records, const float* points, const int64_t* ids,
+                        int64_t Q, const void* values, int32_t values_type, int64_t* found,
+                        void* stream);
 
 /* Device-side anomaly report.  The kernels bound every loop (the
  * reference's descent and march are unbounded, svox/csrc/include/

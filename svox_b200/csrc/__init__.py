@@ -457,6 +457,22 @@ def refuse_tangent(data):
         raise NotImplementedError("svox_b200 has no forward-mode derivatives")
 
 
+def refuse_tangents(*tensors):
+    """``refuse_tangent`` of each tensor that is not None."""
+    if _fwd._current_level >= 0:
+        for t in tensors:
+            if t is not None:
+                refuse_tangent(t)
+
+
+def record_bytes(K, group):
+    """Bytes of a quantised record of ``K`` floats with a scale for every ``group`` of them."""
+    n = int(library().svoxb_record_bytes(C.c_int32(int(K)), C.c_int32(int(group))))
+    if n < 0:
+        raise RuntimeError("a quantised record has 2 to 1024 values in groups of one or more")
+    return n
+
+
 def log_words(capacity):
     """int32 words of a log of ``capacity`` chunks."""
     fn = library().svoxb_item_log_words

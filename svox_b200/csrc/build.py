@@ -11,17 +11,23 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = os.path.join(HERE, "svox_b200.cu")
 LIB = os.path.join(HERE, "libsvox_b200.so")
-DEPS = ["svox_b200.cu", "common.cuh", "arith.cuh", "host.cuh", "binned.cuh", "tiles.cuh", "query.cuh", "render.cuh", "render_index.cuh",
-        "render_queue.cuh", "render_back.cuh", "render_replay.cuh", "noalloc.cuh", "collective.cuh", "open_groups.h",
-        os.path.join("..", "..", "include", "svox_b200.h")]
+_HEADER = os.path.join("..", "..", "include", "svox_b200.h")
+# the translation units, each with what it includes
+UNITS = {
+    "svox_b200.cu": ["common.cuh", "arith.cuh", "host.cuh", "binned.cuh", "tiles.cuh", "query.cuh",
+                     "render.cuh", "render_index.cuh", "render_queue.cuh", "render_back.cuh",
+                     "render_replay.cuh", "noalloc.cuh", "collective.cuh", "open_groups.h",
+                     "status.h", _HEADER],
+    "recurrence.cu": ["recurrence.cuh", "common.cuh", "arith.cuh", "status.h", _HEADER],
+    "records.cu": ["records.cuh", "common.cuh", "arith.cuh", "status.h", _HEADER],
+}
 
 
 # the host side of the hot calls, a Python extension (host.cpp)
 HOST_SRC = os.path.join(HERE, "host.cpp")
 HOST_LIB = os.path.join(HERE, "_host.so")
-HOST_DEPS = ["host.cpp", os.path.join("..", "..", "include", "svox_b200.h")]
+HOST_DEPS = ["host.cpp", _HEADER]
 
 
 def _stale(lib, deps):
@@ -54,15 +60,26 @@ def _build_host():
 def build(force=False, verbose=False):
     if force or _stale(HOST_LIB, HOST_DEPS):
         _build_host()
-    if not force and not _stale(LIB, DEPS):
-        return LIB
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-    cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3",
-           "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-o", LIB, SRC]
-    if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
-    subprocess.run(cmd, check=True)
+    arch = ["-gencode", "arch=compute_100a,code=sm_100a"]
+    objects, running = [], []
+    for unit, deps in UNITS.items():
+        obj = os.path.join(HERE, unit[:-3] + ".o")
+        objects.append(obj)
+        if not force and not _stale(obj, [unit, *deps]):
+            continue
+        # (to a name of its own first: a build that is interrupted leaves no half of an object)
+        part = obj + ".part"
+        cmd = [nvcc, *arch, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
+               *(["-Xptxas", "-v"] if verbose else []), "-c", "-o", part, os.path.join(HERE, unit)]
+        running.append((subprocess.Popen(cmd), cmd, part, obj))
+    for process, cmd, part, obj in running:
+        if process.wait() != 0:
+            raise subprocess.CalledProcessError(process.returncode, cmd)
+        os.replace(part, obj)
+    if running or not os.path.exists(LIB) or \
+            any(os.path.getmtime(o) > os.path.getmtime(LIB) for o in objects):
+        subprocess.run([nvcc, *arch, "-shared", "-o", LIB, *objects], check=True)
     return LIB
 
 

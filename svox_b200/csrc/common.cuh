@@ -16,8 +16,8 @@
 
 namespace svoxb {
 
-// Per-device anomaly word (see svoxb_device_status).
-__device__ int g_status = 0;  // the library is a single translation unit
+// Per-device anomaly word (see svoxb_device_status), one in each translation unit.
+static __device__ int g_status = 0;
 
 __device__ __forceinline__ void report(int code) { atomicMax(&g_status, code); }
 

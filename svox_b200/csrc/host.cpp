@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <dlfcn.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <array>
@@ -36,6 +37,8 @@ struct Library {
     X(se_grad_replay) X(se_grad_image_replay) X(item_log_words) X(item_log_watch)               \
     X(item_log_used)                                                                            \
     X(volume_render_logged_clear) X(volume_render_image_logged_clear) X(log_is_sorted)          \
+    X(gated_scan) X(gated_scan_backward) X(gated_scan_kept) X(gated_scan_workspace)             \
+    X(records_read) X(records_write)                                                            \
     X(strerror) X(last_cuda_error)
 #define SVOXB_MEMBER(name) decltype(&svoxb_##name) name = nullptr;
     SVOXB_FUNCTIONS(SVOXB_MEMBER)
@@ -628,6 +631,248 @@ class QueryNode : public torch::autograd::Function<QueryNode> {
 };
 
 // ---------------------------------------------------------------------------
+// The gated recurrence
+
+int32_t element_type(at::ScalarType t) {
+    switch (t) {
+        case at::kFloat: return SVOXB_TYPE_F32;
+        case at::kBFloat16: return SVOXB_TYPE_BF16;
+        case at::kHalf: return SVOXB_TYPE_F16;
+        default: return -1;
+    }
+}
+
+// `t` with its last dimension dense (a copy if it is not).
+Tensor dense_rows(const Tensor& t) {
+    const int64_t last = t.dim() - 1;
+    return t.size(last) <= 1 || t.stride(last) == 1 ? t : t.contiguous();
+}
+
+// What a call of the recurrence works on; the tensors lie as the kernels read them.
+struct Scan {
+    Tensor values, thickness, initial, offsets;
+    bool reverse = false, weighted = false, states = true;
+    svoxb_scan c{};
+    void bind();
+    std::vector<int64_t> last_shape() const { return {c.B, c.C}; }
+    Tensor workspace(bool backward) const {
+        const int64_t bytes = lib.gated_scan_workspace(&c, backward);
+        return bytes > 0 ? at::empty({bytes}, values.options().dtype(at::kByte)) : Tensor();
+    }
+};
+
+void* pointer_of(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
+
+void Scan::bind() {
+    const bool packed = offsets.defined();
+    const int64_t lead = packed ? 1 : 2;
+    c = svoxb_scan{};
+    c.B = packed ? offsets.numel() - 1 : values.size(0);
+    c.T = values.size(lead - 1);
+    c.C = (int32_t)values.size(lead);
+    c.H = thickness.dim() == lead ? 1 : (int32_t)thickness.size(lead);
+    // (a dimension of one step: any stride will do)
+    auto stride = [](const Tensor& t, int64_t dim, int64_t dense) {
+        return t.size(dim) <= 1 ? dense : t.stride(dim);
+    };
+    c.values_step = stride(values, lead - 1, c.C);
+    c.thickness_step = stride(thickness, lead - 1, c.H);
+    if (!packed) {
+        c.values_row = stride(values, 0, c.T * c.values_step);
+        c.thickness_row = stride(thickness, 0, c.T * c.thickness_step);
+    } else {
+        c.offsets = offsets.data_ptr<int64_t>();
+    }
+    c.values = pointer_of(values);
+    c.thickness = pointer_of(thickness);
+    if (initial.defined()) {
+        c.initial = static_cast<const float*>(pointer_of(initial));
+        c.initial_row = stride(initial, 0, c.C);
+    }
+    c.values_type = element_type(values.scalar_type());
+    c.thickness_type = element_type(thickness.scalar_type());
+    c.reverse = reverse;
+    c.weighted = weighted;
+}
+
+Scan read_scan(const Tensor& values, const Tensor& thickness, const optional<Tensor>& initial,
+               const optional<Tensor>& offsets, const char* state_name) {
+    const bool packed = offsets.has_value();
+    const int64_t lead = packed ? 1 : 2;
+    if (element_type(values.scalar_type()) < 0)
+        fail("values must be float32, bfloat16 or float16");
+    if (values.dim() != lead + 1)
+        fail(packed ? "values must be (N, C) where offsets are given" : "values must be (B, T, C)");
+    if (values.size(lead) < 1) fail("values must have a channel");
+    if (thickness.device() != values.device())
+        fail("thickness must be on the same device as values");
+    if (thickness.scalar_type() != at::kFloat && thickness.scalar_type() != values.scalar_type())
+        fail("thickness must be float32 or of the type of values");
+    if (thickness.dim() != lead && thickness.dim() != lead + 1)
+        fail(packed ? "thickness must be (N,) or (N, H)" : "thickness must be (B, T) or (B, T, H)");
+    for (int64_t d = 0; d < lead; ++d)
+        if (thickness.size(d) != values.size(d)) fail("thickness must have the steps of values");
+    if (thickness.dim() == lead + 1 &&
+        (thickness.size(lead) < 1 || values.size(lead) % thickness.size(lead) != 0))
+        fail("the channels of values must be a multiple of those of thickness");
+    const int64_t B = packed ? offsets->numel() - 1 : values.size(0), C = values.size(lead);
+    if (packed) {
+        if (offsets->device() != values.device())
+            fail("offsets must be on the same device as values");
+        if (offsets->scalar_type() != at::kLong || offsets->dim() != 1 || offsets->numel() < 1)
+            fail("offsets must be (B + 1,) int64");
+    }
+    if (initial) {
+        const std::string name = state_name;
+        if (initial->device() != values.device())
+            fail(name + " must be on the same device as values");
+        if (!at::isFloatingType(initial->scalar_type())) fail(name + " must be of a floating type");
+        const int64_t n = initial->dim();
+        if (n > 2 || (n > 0 && initial->size(-1) != C && initial->size(-1) != 1) ||
+            (n == 2 && initial->size(0) != B && initial->size(0) != 1))
+            fail(name + " must be (B, C) or broadcast to it");
+    }
+    if (!values.is_cuda()) fail("values must be a CUDA tensor");
+    Scan s;
+    s.values = dense_rows(values);
+    s.thickness = thickness.dim() == lead + 1 ? dense_rows(thickness) : thickness;
+    if (packed) s.offsets = offsets->contiguous();
+    if (initial) s.initial = dense_rows(initial->to(at::kFloat).expand({B, C}));
+    return s;
+}
+
+// -> (states or undefined, last state, what the backward needs or undefined)
+std::array<Tensor, 3> run_scan(const Scan& s, bool train) {
+    const c10::cuda::CUDAGuard guard(s.values.device());
+    Tensor states, kept;
+    if (s.states) states = at::empty(s.values.sizes(), s.values.options());
+    const auto floats = s.values.options().dtype(at::kFloat);
+    Tensor last = at::empty(s.last_shape(), floats);
+    if (train) kept = at::empty({std::max<int64_t>(lib.gated_scan_kept(&s.c), 0)}, floats);
+    const Tensor space = s.workspace(false);
+    check(lib.gated_scan(&s.c, pointer_of(states), static_cast<float*>(pointer_of(last)),
+                         static_cast<float*>(pointer_of(kept)), pointer_of(space),
+                         stream_of(s.values)),
+          "gated_scan");
+    return {states, last, kept};
+}
+
+class ScanNode : public torch::autograd::Function<ScanNode> {
+  public:
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                  const Tensor& values, const Tensor& thickness,
+                                                  const optional<Tensor>& initial,
+                                                  std::shared_ptr<Scan> call) {
+        ctx->set_materialize_grads(false);
+        auto [states, last, kept] = run_scan(*call, true);
+        ctx->save_for_backward(
+            {values, thickness, initial ? *initial : Tensor(), call->offsets, kept});
+        torch::autograd::variable_list out;
+        if (states.defined()) out.push_back(states);
+        out.push_back(last);
+        // (the tensors are those that are saved: no second reference, which would hide an edit)
+        call->values = call->thickness = call->initial = call->offsets = Tensor();
+        keep(ctx, std::move(call));
+        return out;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        Scan s = *kept<std::shared_ptr<Scan>>(ctx);
+        s.values = saved[0], s.thickness = saved[1], s.initial = saved[2], s.offsets = saved[3];
+        const Tensor& kept = saved[4];
+        s.bind();
+        const c10::cuda::CUDAGuard guard(s.values.device());
+        Tensor d_states, d_last;
+        if (s.states && grads[0].defined()) d_states = grads[0].contiguous();
+        if (grads.back().defined()) d_last = grads.back().contiguous();
+        Tensor dx, dg, d0;
+        if (ctx->needs_input_grad(0)) dx = at::empty(s.values.sizes(), s.values.options());
+        if (ctx->needs_input_grad(1)) dg = at::empty(s.thickness.sizes(), s.thickness.options());
+        if (s.initial.defined() && ctx->needs_input_grad(2))
+            d0 = at::empty(s.last_shape(), s.initial.options());
+        const Tensor space = s.workspace(true);
+        check(lib.gated_scan_backward(&s.c, static_cast<const float*>(pointer_of(kept)),
+                                      pointer_of(d_states),
+                                      static_cast<const float*>(pointer_of(d_last)),
+                                      pointer_of(dx), pointer_of(dg),
+                                      static_cast<float*>(pointer_of(d0)), pointer_of(space),
+                                      stream_of(s.values)),
+              "gated_scan_backward");
+        torch::autograd::variable_list out{dx, dg, d0};
+        if (at::GradMode::is_enabled()) {       // create_graph: there is no second derivative
+            auto refuse = std::make_shared<torch::autograd::DelayedError>(
+                "svox_b200.gated_scan has no second derivative", 3);
+            for (Tensor& t : out)               // (it marks only what asks for a gradient)
+                if (t.defined()) t.set_requires_grad(true);
+            out = (*refuse)(std::move(out));
+        }
+        out.emplace_back();
+        return out;
+    }
+};
+
+// ---------------------------------------------------------------------------
+// Quantised records
+
+svoxb_records read_records(const Tensor& records, const optional<Tensor>& owner,
+                           const Tensor& child, const Tensor& offset, const Tensor& scaling,
+                           int64_t K, int64_t group, int64_t code) {
+    const auto dev = records.device();
+    if (!records.is_cuda()) fail("the records must be on a CUDA device");
+    check_input(child, "child", at::kInt);
+    check_input(offset, "offset");
+    check_input(scaling, "scaling");
+    svoxb_records r{};
+    if (child.device() != dev || offset.device() != dev || scaling.device() != dev ||
+        (owner && owner->device() != dev))
+        fail("the parts of a record cache must be on one device");
+    if (records.scalar_type() != at::kByte || records.dim() != 2 || !records.is_contiguous() ||
+        child.dim() != 4 || records.size(0) != child.numel())
+        fail("records must be (M * N^3, bytes) uint8");
+    if (owner && (owner->scalar_type() != at::kInt || !owner->is_contiguous() ||
+                  owner->numel() != child.numel()))
+        fail("owner must hold one int32 for every record");
+    r.records = records.data_ptr();
+    r.owner = owner ? reinterpret_cast<uint32_t*>(owner->data_ptr<int32_t>()) : nullptr;
+    r.child = child.data_ptr<int32_t>();
+    r.offset = offset.data_ptr<float>();
+    r.scaling = scaling.data_ptr<float>();
+    r.M = child.size(0);
+    r.N = (int32_t)child.size(1);
+    r.K = (int32_t)K;
+    r.group = (int32_t)group;
+    r.code_type = (int32_t)code;
+    return r;
+}
+
+// Where rows go: points, ids, or (neither) each row to the record of its number.
+struct Places {
+    const float* points = nullptr;
+    const int64_t* ids = nullptr;
+    int64_t Q = 0;
+};
+Places read_places(const optional<Tensor>& where, bool points, const Tensor& records) {
+    Places p;
+    if (!where) {
+        p.Q = records.size(0);
+        return p;
+    }
+    if (where->device() != records.device())
+        fail(std::string(points ? "points" : "ids") + " must be on the device of the records");
+    p.Q = where->numel() / (points ? 3 : 1);
+    if (points) {
+        check_points(*where);
+        p.points = where->data_ptr<float>();
+    } else {
+        if (where->scalar_type() != at::kLong || where->dim() != 1 || !where->is_contiguous())
+            fail("ids must be (Q,) int64, contiguous");
+        p.ids = where->data_ptr<int64_t>();
+    }
+    return p;
+}
+
+// ---------------------------------------------------------------------------
 // The functions Python sees: arguments are read with the interpreter lock held, the calls run
 // without it.
 
@@ -753,6 +998,71 @@ PYBIND11_MODULE(_host, m) {
                 check(lib.item_log_used(words, &used, side.stream()), "item_log_used");
             }
             return std::make_tuple(out, grad, hess, used);
+        });
+    });
+
+    // -> (states, last), or (last,) without `states`
+    m.def("gated_scan", [](const Tensor& values, const Tensor& thickness,
+                           const optional<Tensor>& initial, const optional<Tensor>& offsets,
+                           bool reverse, bool weighted, bool states, const char* state_name) {
+        return unlocked([&]() -> torch::autograd::variable_list {
+            auto call = std::make_shared<Scan>(
+                read_scan(values, thickness, initial, offsets, state_name));
+            call->reverse = reverse;
+            call->weighted = weighted;
+            call->states = states;
+            call->bind();
+            const bool train = at::GradMode::is_enabled() &&
+                               (call->values.requires_grad() || call->thickness.requires_grad() ||
+                                (call->initial.defined() && call->initial.requires_grad()));
+            if (train)
+                return ScanNode::apply(
+                    Tensor(call->values), Tensor(call->thickness),
+                    call->initial.defined() ? optional<Tensor>(call->initial) : std::nullopt, call);
+            auto [all, last, kept] = run_scan(*call, false);
+            if (states) return {all, last};
+            return {last};
+        });
+    });
+
+    m.def("records_read", [](const Tensor& records, const Tensor& child, const Tensor& offset,
+                             const Tensor& scaling, int64_t K, int64_t group, int64_t code,
+                             const optional<Tensor>& where, bool points, at::ScalarType type) {
+        const svoxb_records r =
+            read_records(records, {}, child, offset, scaling, K, group, code);
+        const Places at = read_places(where, points, records);
+        if (element_type(type) < 0) fail("records are read as float32, bfloat16 or float16");
+        return unlocked([&] {
+            const c10::cuda::CUDAGuard guard(records.device());
+            Tensor out = at::empty({at.Q, K}, records.options().dtype(type));
+            check(lib.records_read(&r, at.points, at.ids, at.Q, out.data_ptr(), element_type(type),
+                                   stream_of(records)),
+                  "records_read");
+            return out;
+        });
+    });
+    m.def("records_write", [](const Tensor& records, const Tensor& owner, const Tensor& child,
+                              const Tensor& offset, const Tensor& scaling, int64_t K, int64_t group,
+                              int64_t code, const optional<Tensor>& where, bool points,
+                              const Tensor& values) {
+        const svoxb_records r =
+            read_records(records, owner, child, offset, scaling, K, group, code);
+        const Places at = read_places(where, points, records);
+        if (values.device() != records.device())
+            fail("values must be on the device of the records");
+        if (values.dim() != 2 || values.size(0) != at.Q || values.size(1) != K ||
+            !values.is_contiguous())
+            fail("values must be (Q, K), contiguous");
+        if (element_type(values.scalar_type()) < 0)
+            fail("values must be float32, bfloat16 or float16");
+        unlocked([&] {
+            const c10::cuda::CUDAGuard guard(records.device());
+            Tensor found;
+            if (where) found = at::empty({at.Q}, records.options().dtype(at::kLong));
+            check(lib.records_write(&r, at.points, at.ids, at.Q, values.data_ptr(),
+                                    element_type(values.scalar_type()),
+                                    static_cast<int64_t*>(pointer_of(found)), stream_of(records)),
+                  "records_write");
         });
     });
 

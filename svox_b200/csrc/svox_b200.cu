@@ -1,6 +1,6 @@
 // C-ABI entry points of libsvox_b200 (see include/svox_b200.h) and the
 // dispatch from run-time record layouts to the templated sm_100a kernels.
-// The library is this single translation unit.
+// (The recurrence and the quantised records are translation units of their own.)
 #include "common.cuh"
 #include "host.cuh"
 #include "query.cuh"
@@ -9,6 +9,7 @@
 #include "render_back.cuh"
 #include "render_replay.cuh"
 #include "collective.cuh"
+#include "status.h"
 #include <initializer_list>
 #include <new>
 
@@ -1154,6 +1155,12 @@ int svoxb_device_status(int clear, void* stream) {
         const int zero = 0;
         SVOXB_CUDA(cudaMemcpyToSymbol(g_status, &zero, sizeof(int)));
     }
+    for (auto more : {status_of_recurrence, status_of_records}) {
+        int other = 0;
+        const int st = more(clear, &other);
+        if (st) return st;
+        if (other > word) word = other;
+    }
     return word;
 }
 
@@ -1168,6 +1175,7 @@ const char* svoxb_strerror(int status) {
         case SVOXB_ERR_TREE: return "corrupt tree: a descent left the node array";
         case SVOXB_ERR_MARCH: return "a ray exceeded the marching step cap";
         case SVOXB_ERR_TOO_LARGE: return "size beyond the supported maximum";
+        case SVOXB_ERR_INDEX: return "an offset or leaf id is out of range";
     }
     return "unknown status";
 }

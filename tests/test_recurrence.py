@@ -1,0 +1,561 @@
+"""The gated recurrence and compositing against a plain loop in 64 bits.
+
+Tolerances come with the reference: it carries a bound of the rounding errors along.  With u =
+2^-24, a step of the kernel multiplies by a = exp(-g) (expf: 2 ulp, 4 u) and by w = 1 - a (below 14 u + u
+where it is a difference, g >= 0.25; below 2 u as a series) and adds, in whatever association the
+stretches are joined; every factor and sum enters the error once, so with the sums of magnitudes
+    H[t] = a H[t-1] + w |x|,   e[t] = a e[t-1] + (a H[t-1] + w |x|)
+the state is off by at most 20 u e[t], and likewise the adjoint.  Outputs of 16 bits are rounded once
+more, by half a step."""
+import pytest
+import torch
+
+import svox_b200 as svox
+from svox_b200 import csrc
+
+U = 2.0 ** -24
+HALF_STEP = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.bfloat16, torch.float16)}
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def rows_of(values, offsets):
+    if offsets is None:
+        n, T = values.shape[:2]
+        return [(b * T, b * T + T) for b in range(n)]
+    o = offsets.tolist()
+    return list(zip(o[:-1], o[1:]))
+
+
+def reference(values, thickness, initial, offsets, reverse, weighted, d_states=None, d_last=None):
+    """Plain loops in 64 bits -> {name: (value, tolerance before the output's rounding)}."""
+    C = values.shape[-1]
+    x = values.detach().cpu().double().reshape(-1, C)
+    g = thickness.detach().cpu().double()
+    g = g.reshape(x.shape[0], -1)
+    H = g.shape[1]
+    D = C // H
+    g = g.repeat_interleave(D, 1)
+    rows = rows_of(values, None if offsets is None else offsets.cpu())
+    B = len(rows)
+    h0 = torch.zeros(B, C, dtype=torch.float64) if initial is None else \
+        initial.detach().cpu().double().expand(B, C)
+    ds = torch.zeros_like(x) if d_states is None else d_states.cpu().double().reshape(-1, C)
+    dl = torch.zeros(B, C, dtype=torch.float64) if d_last is None else d_last.cpu().double()
+    a = torch.exp(-g)
+    w = torch.ones_like(a) if weighted else -torch.expm1(-g)
+    take = torch.where(w == 0, torch.zeros_like(x), w * x)
+    out = {n: torch.zeros_like(x) for n in ("states", "e_states", "dx", "e_dx", "dgc", "e_dgc")}
+    last, e_last, d0, e_d0 = (torch.zeros(B, C, dtype=torch.float64) for _ in range(4))
+    for b, (lo, hi) in enumerate(rows):
+        steps = list(range(lo, hi))
+        if reverse:
+            steps.reverse()
+        h, Habs, e = h0[b].clone(), h0[b].abs(), torch.zeros(C, dtype=torch.float64)
+        before = {}
+        for t in steps:
+            before[t] = (h, Habs, e)
+            gone = a[t] == 0
+            z = torch.zeros_like(h)
+            ah, aH, ae = (torch.where(gone, z, a[t] * q) for q in (h, Habs, e))
+            e = ae + aH + take[t].abs()
+            h, Habs = ah + take[t], aH + take[t].abs()
+            out["states"][t], out["e_states"][t] = h, e
+        last[b], e_last[b] = h, e
+        G, Gabs, eG = dl[b].clone(), dl[b].abs(), torch.zeros(C, dtype=torch.float64)
+        for t in reversed(steps):
+            G, Gabs = G + ds[t], Gabs + ds[t].abs()
+            eG = eG + Gabs
+            out["dx"][t], out["e_dx"][t] = w[t] * G, w[t] * (eG + Gabs)
+            hp, Hp, ep = before[t]
+            xt = torch.where((w[t] == 0) & ~x[t].isfinite(), hp, x[t])
+            gone = a[t] == 0
+            z = torch.zeros_like(h)
+            q = torch.where(gone, z, a[t] * (-hp if weighted else xt - hp))
+            qa = torch.where(gone, z, a[t] * (Hp if weighted else xt.abs() + Hp))
+            qe = torch.where(gone, z, a[t] * ep)
+            out["dgc"][t] = q * G
+            out["e_dgc"][t] = qa * (eG + Gabs) + qe * Gabs + D * qa * Gabs / 20
+            G, Gabs, eG = (torch.where(gone, z, a[t] * v) for v in (G, Gabs, eG + Gabs))
+        d0[b], e_d0[b] = G, eG
+
+    def grouped(v):
+        return v.reshape(-1, H, D).sum(2).reshape(thickness.shape)
+
+    shape = values.shape
+    tol = 20 * U
+    return {"states": (out["states"].reshape(shape), tol * out["e_states"].reshape(shape)),
+            "last": (last, tol * e_last), "d_initial": (d0, tol * e_d0),
+            "d_values": (out["dx"].reshape(shape), tol * out["e_dx"].reshape(shape)),
+            "d_thickness": (grouped(out["dgc"]), tol * grouped(out["e_dgc"]))}
+
+
+def close(name, got, want):
+    value, tol = want
+    assert got.shape == value.shape, name
+    g = got.detach().cpu().double()
+    # (what is below 2^-149 in 32 bits is 0: an error of at most that much in each of the fewer than
+    # 2^20 products that an output here consists of, times other factors below 2^20)
+    tol = tol + HALF_STEP[got.dtype] * (value.abs() + tol) + 2.0 ** -109
+    if got.dtype == F16:
+        tol = tol + 2.0 ** -25          # half of its smallest step
+    off = (g - value).abs()
+    bad = ~(off <= tol)
+    assert not bad.any(), (name, int(bad.sum()), off[bad].max().item(),
+                           bad.nonzero()[0].tolist())
+
+
+def inputs(gen, lead, C, H, dtype, gates, dev):
+    x = torch.randn(*lead, C, generator=gen).to(dev, dtype)
+    g = torch.exp(1.5 * torch.randn(*lead, *([H] if H > 1 else []), generator=gen) - 2)
+    g[torch.rand(g.shape, generator=gen) < 0.2] = 0.0
+    g[torch.rand(g.shape, generator=gen) < 0.05] = 12.0
+    return x, g.to(dev, gates)
+
+
+def check_call(dev, x, g, initial, offsets, reverse, weighted, gen, with_states=True,
+               with_last=True):
+    for t in (x, g, initial):
+        if t is not None:
+            t.requires_grad_(True)
+    states, last = svox.gated_scan(x, g, initial, offsets, reverse, weighted)
+    assert states.dtype == x.dtype and last.dtype == F32
+    ds = torch.randn(states.shape, generator=gen).to(dev, states.dtype) if with_states else None
+    dl = torch.randn(last.shape, generator=gen).to(dev) if with_last else None
+    want = reference(x, g, initial, offsets, reverse, weighted, ds, dl)
+    close("states", states, want["states"])
+    close("last", last, want["last"])
+    outs = [o for o, d in ((states, ds), (last, dl)) if d is not None]
+    leaves = [t for t in (x, g, initial) if t is not None]
+    grads = torch.autograd.grad(outs, leaves, [d for d in (ds, dl) if d is not None])
+    close("d_values", grads[0], want["d_values"])
+    close("d_thickness", grads[1], want["d_thickness"])
+    if initial is not None and initial.shape == last.shape:
+        close("d_initial", grads[2], want["d_initial"])
+    with torch.no_grad():       # the call that keeps nothing
+        again = svox.gated_scan(x, g, initial, offsets, reverse, weighted)
+    assert torch.equal(again[0], states) and torch.equal(again[1], last)
+    return states, last, grads
+
+
+# (B, T, C, H): one step to several stretches and splits, odd sizes, gates of all kinds
+SHAPES = [(1, 1, 1, 1), (3, 1, 5, 5), (2, 2, 3, 1), (2, 63, 33, 33), (1, 64, 64, 64), (3, 65, 66, 66),
+          (2, 130, 7, 7), (1, 257, 48, 3), (2, 71, 96, 4), (1, 40, 200, 1), (2, 33, 130, 2),
+          (5, 19, 34, 17), (1, 1500, 3, 1), (1, 1029, 70, 70), (40, 9, 16, 16), (2, 700, 1, 1),
+          (3, 100, 12, 4)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("dtype,gates", [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16),
+                                         (F16, F32)])
+def test_scan(cuda_device, shape, dtype, gates):
+    B, T, C, H = shape
+    gen = torch.Generator().manual_seed(B + T + C)
+    for k, (reverse, weighted) in enumerate([(False, False), (True, True)]):
+        x, g = inputs(gen, (B, T), C, H, dtype, gates, cuda_device)
+        initial = torch.randn(B, C, generator=gen).to(cuda_device) if k == 0 or T > 50 else None
+        check_call(cuda_device, x, g, initial, None, reverse, weighted, gen)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("C,H,dtype", [(3, 1, F32), (1, 1, F32), (4, 4, F16), (40, 8, BF16),
+                                       (66, 66, BF16), (33, 1, F32), (3, 1, BF16), (16, 1, F32),
+                                       (6, 2, F32), (130, 1, F32)])
+def test_packed(cuda_device, C, H, dtype, reverse):
+    """Rows of any length, empty ones among them, and steps that no row covers."""
+    gen = torch.Generator().manual_seed(C)
+    n = torch.tensor([0, 1, 5, 0, 0, 130, 64, 65, 2, 300, 0, 31, 32, 33, 0])
+    offsets = (7 + torch.cat([torch.zeros(1, dtype=torch.int64), n.cumsum(0)])).to(cuda_device)
+    N = int(offsets[-1]) + 11
+    x, g = inputs(gen, (N,), C, H, dtype, F32, cuda_device)
+    initial = torch.randn(n.numel(), C, generator=gen).to(cuda_device)
+    # the outputs' memory is not clean
+    junk = [torch.full((N * max(C, 64),), float("nan"), device=cuda_device) for _ in range(4)]
+    del junk
+    states, last, grads = check_call(cuda_device, x, g, initial, offsets, reverse, False, gen)
+    for t in (states, grads[0], grads[1]):
+        assert (t[:7] == 0).all() and (t[-11:] == 0).all()
+    empty = (n == 0).to(cuda_device)
+    assert torch.equal(last[empty], initial[empty])
+    assert csrc.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,dtype", [(1, F32), (2, F32), (3, F32), (3, BF16), (4, F32), (7, F16),
+                                     (8, BF16), (32, BF16), (35, F32), (64, F16)])
+@pytest.mark.parametrize("packed", [True, False])
+def test_composite(cuda_device, C, dtype, packed):
+    gen = torch.Generator().manual_seed(C)
+    if packed:
+        n = torch.cat([torch.randint(0, 70, (60,), generator=gen), torch.tensor([0, 0, 900, 1, 0])])
+        offsets = torch.cat([torch.zeros(1, dtype=torch.int64), n.cumsum(0)]).to(cuda_device)
+        lead, B = (int(offsets[-1]),), n.numel()
+    else:
+        offsets, lead, B = None, (37, 45), 37
+    x, g = inputs(gen, lead, C, 1, dtype, F32, cuda_device)
+    bg = torch.rand(B, C, generator=gen).to(cuda_device)
+    for t in (x, g, bg):
+        t.requires_grad_(True)
+    out = svox.composite(x, g, bg, offsets)
+    d = torch.randn(out.shape, generator=gen).to(cuda_device)
+    want = reference(x, g, bg, offsets, True, False, None, d)
+    close("last", out, want["last"])
+    for name, got in zip(("d_values", "d_thickness", "d_initial"),
+                         torch.autograd.grad([out], [x, g, bg], [d])):
+        close(name, got, want[name])
+    assert torch.equal(out, svox.gated_scan(x, g, bg, offsets, reverse=True)[1])
+    with torch.no_grad():
+        assert torch.equal(out, svox.composite(x, g, bg, offsets))
+
+
+@pytest.mark.gpu
+def test_composite_is_emission_and_absorption(cuda_device):
+    """The sum of what each sample emits, weighted by what reaches it."""
+    gen = torch.Generator().manual_seed(0)
+    x, g = inputs(gen, (50, 90), 3, 1, F32, F32, cuda_device)
+    bg = torch.rand(3, generator=gen).to(cuda_device)
+    through = torch.exp(-(g.double().cumsum(1) - g.double()))
+    w = through * -torch.expm1(-g.double())
+    want = (w[..., None] * x).sum(1) + torch.exp(-g.double().sum(1))[:, None] * bg
+    tol = reference(x, g, bg, None, True, False)["last"][1]
+    close("last", svox.composite(x, g, bg), (want.cpu(), tol))
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences(cuda_device):
+    """Central differences of the kernel's own output.  Their truncation error is the reference's,
+    found in 64 bits; the kernel's rounding is divided by the step."""
+    gen = torch.Generator().manual_seed(3)
+    x, g = inputs(gen, (4, 40), 3, 1, F32, F32, cuda_device)
+    bg = torch.rand(4, 3, generator=gen).to(cuda_device)
+    g = g.clamp(min=0.05)
+    d = torch.randn(4, 3, generator=gen).to(cuda_device)
+    step = 2.0 ** -6
+    leaves = [t.clone().requires_grad_(True) for t in (x, g, bg)]
+    grads = torch.autograd.grad([svox.composite(*leaves)], leaves, [d])
+
+    def plain(x, g, bg):
+        want = reference(x, g, bg, None, True, False)["last"]
+        return (want[0] * d.cpu()).sum().item(), (want[1] * d.cpu().abs()).sum().item()
+
+    for k in range(3):
+        way = torch.randn(leaves[k].shape, generator=gen).to(cuda_device)
+        way = (way * 16).round() / 16
+        ends = []
+        for sign in (1, -1):
+            args = [x, g, bg]
+            args[k] = args[k] + sign * step * way
+            ends.append(([(svox.composite(*args).double() * d).sum().item()], plain(*args)))
+        slope = (ends[0][0][0] - ends[1][0][0]) / (2 * step)
+        exact = (ends[0][1][0] - ends[1][1][0]) / (2 * step)
+        want = reference(x, g, bg, None, True, False, None, d)
+        name = ("d_values", "d_thickness", "d_initial")[k]
+        along = (want[name][0] * way.cpu()).sum().item()
+        mine = (grads[k].double() * way).sum().item()
+        rounding = (ends[0][1][1] + ends[1][1][1]) / (2 * step) + \
+            (want[name][1] * way.cpu().abs()).sum().item()
+        assert abs(mine - slope) <= abs(exact - along) + rounding
+
+
+@pytest.mark.gpu
+def test_strides_and_broadcasts(cuda_device):
+    """Slices of a wider projection, broken alignment, transposed and expanded inputs, a state for
+    all rows: the same results as their copies, and gradients of the right shape."""
+    gen = torch.Generator().manual_seed(1)
+    wide = torch.randn(3, 70, 150, generator=gen).to(cuda_device)
+    gate = torch.rand(3, 70, 150, generator=gen).to(cuda_device)
+    flat = torch.randn(3 * 70 * 64 + 1, generator=gen).to(cuda_device, BF16)
+    cases = [(wide[:, :, 5:69], gate[:, :, 3:67]), (wide[:, :, 4:68], gate[:, :, 2:66]),
+             (wide[:, ::2, 4:68], gate[:, ::2, 2:66]), (wide[1:, :, 1:4], gate[1:, :, 7]),
+             (wide.transpose(1, 2)[:, 3:40, :], gate.transpose(1, 2)[:, 3:40, :]),
+             (wide[:, :1, 4:68].expand(3, 70, 64), gate[:1, :, 0].expand(3, 70)),
+             (flat[1:].view(3, 70, 64), gate[:, :, 9:73].to(BF16)),
+             (wide[:, :, 4:5], gate[:, :, 4:5])]
+    for x, g in cases:
+        state = torch.randn(x.shape[-1], generator=gen).to(cuda_device)
+        a = [x.detach().clone(memory_format=torch.contiguous_format).requires_grad_(True),
+             g.detach().clone(memory_format=torch.contiguous_format).requires_grad_(True),
+             state.clone().requires_grad_(True)]
+        b = [x.detach().requires_grad_(True), g.detach().requires_grad_(True),
+             state.clone().requires_grad_(True)]
+        outs = [svox.gated_scan(*v[:2], initial=v[2]) for v in (a, b)]
+        d = [torch.randn(o.shape, generator=gen).to(cuda_device, o.dtype) for o in outs[0]]
+        for p, q in zip(outs[0], outs[1]):
+            assert torch.equal(p, q)
+        for p, q in zip(torch.autograd.grad(outs[0], a, d), torch.autograd.grad(outs[1], b, d)):
+            assert p.shape == q.shape and torch.equal(p, q)
+        want = reference(x, g, state, None, False, False, d[0], d[1])
+        close("states", outs[1][0], want["states"])
+    # an unaligned gradient
+    x = torch.randn(2, 30, 64, generator=gen).to(cuda_device, BF16).requires_grad_(True)
+    g = torch.rand(2, 30, 64, generator=gen).to(cuda_device, BF16)
+    states, last = svox.gated_scan(x, g)
+    d = torch.randn(2 * 30 * 64 + 1, generator=gen).to(cuda_device, BF16)[1:].view(2, 30, 64)
+    assert d.data_ptr() % 4 == 2
+    close("d_values", torch.autograd.grad(states, x, d)[0],
+          reference(x, g, None, None, False, False, d)["d_values"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [3, 64])
+def test_masked_places(cuda_device, C):
+    """Samples of no thickness may hold anything; nothing from behind an opaque sample shows."""
+    gen = torch.Generator().manual_seed(2)
+    x, g = inputs(gen, (6, 150), C, 1, F32, F32, cuda_device)
+    bg = torch.rand(6, C, generator=gen).to(cuda_device)
+    masked = torch.rand(6, 150, generator=gen).to(cuda_device) < 0.3
+    masked[5] = True                                   # a row whose mask leaves nothing
+    g = torch.where(masked, torch.zeros_like(g), g)
+    dirty = torch.where(masked[..., None], torch.full_like(x, float("nan")), x)
+    dirty[0][masked[0]] = float("inf")
+    dirty[1][masked[1]] = torch.finfo(F32).min
+    clean = torch.where(masked[..., None], torch.zeros_like(x), x)
+    d = torch.randn(6, C, generator=gen).to(cuda_device)
+    got = []
+    for v in (clean, dirty):
+        leaves = [v.clone().requires_grad_(True), g.clone().requires_grad_(True),
+                  bg.clone().requires_grad_(True)]
+        out = svox.composite(*leaves)
+        got.append([out, *torch.autograd.grad(out, leaves, d)])
+    assert torch.equal(got[0][0], got[1][0])
+    assert torch.equal(got[0][0][5], bg[5])
+    assert torch.equal(got[0][1], got[1][1]) and torch.equal(got[0][3], got[1][3])
+    assert torch.equal(got[0][2][~masked], got[1][2][~masked])
+    # (row 1 holds the lowest float where it is masked: with no thickness the gradient is its true sum
+    # over the channels, up to 64 times 3.4e38 times the adjoint, which is beyond the largest float)
+    rest = [0, 2, 3, 4, 5]
+    assert got[1][2][rest].isfinite().all()
+    # opaque: thickness inf, and what is behind it is not a number
+    g[:, 40] = float("inf")
+    dirty = clean.clone()
+    dirty[:, 41:] = float("nan")
+    bg[:] = float("nan")
+    g[:, 41:] = g[:, 41:].clamp(min=0.1)
+    leaves = [dirty.requires_grad_(True), g.requires_grad_(True), bg.requires_grad_(True)]
+    out = svox.composite(*leaves)
+    want = reference(clean[:, :41], g[:, :41], None, None, True, False, None, d)
+    close("last", out, want["last"])
+    grads = torch.autograd.grad(out, leaves, d)
+    close("d_values", grads[0][:, :41], want["d_values"])
+    assert (grads[0][:, 41:] == 0).all() and (grads[2] == 0).all()
+    assert grads[1][:, :41].isfinite().all()
+
+
+@pytest.mark.gpu
+def test_partial_gradients(cuda_device):
+    """Only some outputs used, only some inputs asked for."""
+    gen = torch.Generator().manual_seed(4)
+    for C, H in ((66, 66), (3, 1), (96, 2)):
+        x, g = inputs(gen, (2, 90), C, H, F32, F32, cuda_device)
+        s0 = torch.randn(2, C, generator=gen).to(cuda_device)
+        check_call(cuda_device, x, g, s0, None, False, False, gen, with_last=False)
+        check_call(cuda_device, x.detach(), g.detach(), s0.detach(), None, True, False, gen,
+                   with_states=False)
+        d = torch.randn(2, C, generator=gen).to(cuda_device)
+        args = [x.detach(), g.detach(), s0.detach()]
+        for k in range(3):
+            v = [t.clone() for t in args]
+            v[k].requires_grad_(True)
+            want = reference(*args, None, True, False, None, d)
+            got, = torch.autograd.grad(svox.composite(*v), [v[k]], d)
+            close(k, got, want[("d_values", "d_thickness", "d_initial")[k]])
+
+
+@pytest.mark.gpu
+def test_steps_carry_on(cuda_device):
+    """A sequence run in pieces, the last of single steps."""
+    gen = torch.Generator().manual_seed(5)
+    x, g = inputs(gen, (3, 100), 70, 70, F32, F32, cuda_device)
+    want = reference(x, g, None, None, False, False)
+    states, state = [], None
+    for lo, hi in [(0, 40), (40, 80)] + [(t, t + 1) for t in range(80, 100)]:
+        s, state = svox.gated_scan(x[:, lo:hi], g[:, lo:hi], state)
+        states.append(s)
+    close("states", torch.cat(states, 1), want["states"])
+    close("last", state, want["last"])
+
+
+@pytest.mark.gpu
+def test_empty(cuda_device):
+    z = torch.zeros
+    for lead in ((0, 5), (4, 0), (0, 0)):
+        x = z(*lead, 3, device=cuda_device, requires_grad=True)
+        g = z(*lead, device=cuda_device, requires_grad=True)
+        s0 = torch.rand(lead[0], 3, device=cuda_device).requires_grad_(True)
+        states, last = svox.gated_scan(x, g, s0)
+        assert states.shape == x.shape and torch.equal(last, s0)
+        (states.sum() + last.sum()).backward()
+        assert x.grad.shape == x.shape and g.grad.shape == g.shape
+        assert torch.equal(s0.grad, torch.ones_like(s0))
+    none = z(1, dtype=torch.int64, device=cuda_device)
+    x = torch.rand(4, 3, device=cuda_device).requires_grad_(True)
+    g = torch.rand(4, device=cuda_device).requires_grad_(True)
+    states, last = svox.gated_scan(x, g, offsets=none)
+    assert last.shape == (0, 3) and (states == 0).all()
+    states.sum().backward()
+    assert (x.grad == 0).all() and (g.grad == 0).all()
+    rays = z(6, dtype=torch.int64, device=cuda_device)
+    x, g = z(0, 3, device=cuda_device), z(0, device=cuda_device)
+    bg = torch.rand(3, device=cuda_device)
+    assert torch.equal(svox.composite(x, g, bg, rays), bg.expand(5, 3))
+    csrc.check_device_status()
+
+
+@pytest.mark.gpu
+def test_repeatable_streams_and_graphs(cuda_device):
+    gen = torch.Generator().manual_seed(6)
+    for lead, C, H, offsets in (((2, 900), 96, 1, None), ((1, 5000), 40, 40, None),
+                                ((2000,), 3, 1, torch.tensor([0, 700, 700, 2000]))):
+        x, g = inputs(gen, lead, C, H, F32, F32, cuda_device)
+        offsets = None if offsets is None else offsets.to(cuda_device)
+        x.requires_grad_(True)
+        g.requires_grad_(True)
+
+        def step():
+            # (no graph of the leaves outlives a step: their accumulation nodes would tie the
+            # capture to the stream that they were made on)
+            states, last = svox.gated_scan(x, g, offsets=offsets)
+            grads = torch.autograd.grad([states.sum() + last.sum()], [x, g])
+            return [states.detach(), last.detach(), *grads]
+
+        want = step()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(3):
+                got = step()
+        torch.cuda.current_stream().wait_stream(side)
+        for p, q in zip(want, got):
+            assert torch.equal(p, q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step()
+        with torch.no_grad():
+            x += 0.25
+            for t in held:
+                t.fill_(float("nan"))
+        for _ in range(2):
+            graph.replay()
+        for p, q in zip(step(), held):
+            assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
+def test_long_axis_past_32_bits(cuda_device):
+    """More than 2^31 elements: the last steps, behind one that forgets all before it."""
+    T, C = (1 << 21) + 5, 1030
+    x = torch.ones(1, T, C, dtype=BF16, device=cuda_device)
+    g = torch.full((1, T), 0.5, device=cuda_device)
+    assert x.numel() > 1 << 31
+    gen = torch.Generator().manual_seed(7)
+    tail = torch.randn(1, 20, C, generator=gen).to(cuda_device, BF16)
+    x[:, -20:] = tail
+    g[:, -20] = float("inf")
+    states, last = svox.gated_scan(x, g)
+    want = reference(tail, g[:, -20:], None, None, False, False)
+    close("states", states[:, -20:], want["states"])
+    close("last", last, want["last"])
+    del states
+    out = svox.composite(x[:, -20:], g[:, -20:])
+    g[:, -20] = 0.5
+    g[:, 3] = float("inf")
+    head = reference(x[:, :4], g[:, :4], None, None, True, False)
+    close("last", svox.composite(x, g), head["last"])
+    assert out.shape == last.shape
+
+
+@pytest.mark.gpu
+def test_bad_offsets_are_noticed(cuda_device):
+    x = torch.rand(50, 3, device=cuda_device).requires_grad_(True)
+    g = torch.rand(50, device=cuda_device).requires_grad_(True)
+    for bad in ([0, 30, 20, 50], [0, 10, 60], [-5, 10, 50], [0, 1 << 40, 50], [70, 80, 90]):
+        csrc.device_status()
+        o = torch.tensor(bad, device=cuda_device)
+        states, last = svox.gated_scan(x, g, offsets=o)
+        (states.sum() + last.sum()).backward()
+        svox.composite(x, g, offsets=o).sum().backward()
+        assert csrc.device_status() == 9
+        assert csrc.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_no_second_derivative_and_edits(cuda_device):
+    x = torch.rand(2, 30, 3, device=cuda_device, requires_grad=True)
+    g = torch.rand(2, 30, device=cuda_device, requires_grad=True)
+    grads = torch.autograd.grad(svox.composite(x, g).sum(), [x, g], create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        grads[0].sum().backward()
+    out = svox.composite(x, g)
+    with torch.no_grad():
+        x += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    import torch.autograd.forward_ad as fwad
+    with fwad.dual_level():
+        dual = fwad.make_dual(x.detach(), torch.ones_like(x))
+        with pytest.raises(NotImplementedError):
+            svox.composite(dual, g.detach())
+
+
+def test_refusals():
+    x, g = torch.rand(2, 5, 6), torch.rand(2, 5)
+    o = torch.tensor([0, 3, 5])
+    bad = [((x.double(), g), {}, "float32, bfloat16 or float16"),
+           ((x[0], g), {}, r"\(B, T, C\)"), ((x, g), {"offsets": o}, r"\(N, C\)"),
+           ((x[..., :0], g), {}, "must have a channel"),
+           ((x, g[:, :4]), {}, "the steps of values"), ((x, g[0]), {}, "thickness must be"),
+           ((x, g.bfloat16()), {}, "float32 or of the type"),
+           ((x.bfloat16(), g.half()), {}, "float32 or of the type"),
+           ((x, torch.rand(2, 5, 4)), {}, "multiple"), ((x, torch.rand(2, 5, 0)), {}, "multiple"),
+           ((x[0], g[0]), {"offsets": o.int()}, "int64"),
+           ((x[0], g[0]), {"offsets": o[None]}, "int64"),
+           ((x[0], g[0]), {"offsets": o[:0]}, "int64"),
+           ((x, g), {"initial": torch.rand(3, 6)}, "initial must be"),
+           ((x, g), {"initial": torch.rand(2, 4)}, "initial must be"),
+           ((x, g), {"initial": torch.rand(1, 2, 6)}, "initial must be"),
+           ((x, g), {"initial": torch.ones(2, 6, dtype=torch.int64)}, "floating"),
+           ((x, g), {}, "CUDA tensor"), ((x[0], g[0]), {"offsets": o}, "CUDA tensor")]
+    for args, more, text in bad:
+        with pytest.raises(RuntimeError, match=text):
+            svox.gated_scan(*args, **more)
+    with pytest.raises(RuntimeError, match="background must be"):
+        svox.composite(x, g, torch.rand(3, 6))
+
+
+def test_abi_refusals():
+    import ctypes as C
+
+    class Scan(C.Structure):
+        _fields_ = [("values", C.c_void_p), ("thickness", C.c_void_p), ("initial", C.c_void_p),
+                    ("offsets", C.c_void_p), ("B", C.c_int64), ("T", C.c_int64),
+                    ("values_row", C.c_int64), ("values_step", C.c_int64),
+                    ("thickness_row", C.c_int64), ("thickness_step", C.c_int64),
+                    ("initial_row", C.c_int64), ("C", C.c_int32), ("H", C.c_int32),
+                    ("values_type", C.c_int32), ("thickness_type", C.c_int32),
+                    ("reverse", C.c_int32), ("weighted", C.c_int32)]
+
+    lib = csrc.library()
+    lib.svoxb_gated_scan_kept.restype = lib.svoxb_gated_scan_workspace.restype = C.c_int64
+
+    def call(**k):
+        s = Scan(16, 16, None, None, 2, 3, 12, 4, 3, 1, 0, 4, 1, 0, 0, 0, 0)
+        for name, v in k.items():
+            setattr(s, name, v)
+        return lib.svoxb_gated_scan(C.byref(s), None, None, None, None, None), s
+
+    assert call()[0] == 1                                   # no `last`
+    assert call(values=None)[0] == 1 and call(thickness=None)[0] == 1
+    assert call(B=-1)[0] == 2 and call(T=-1)[0] == 2 and call(C=0)[0] == 2 and call(H=3)[0] == 2
+    assert call(values_type=3)[0] == 3 and call(thickness_type=1)[0] == 3
+    assert call(T=1 << 41)[0] == 8
+    assert call(B=0)[0] == 0                                # nothing to do
+    assert lib.svoxb_gated_scan(None, None, None, None, None, None) == 1
+    s = call(H=3)[1]
+    assert lib.svoxb_gated_scan_kept(C.byref(s)) == -1
+    assert lib.svoxb_gated_scan_workspace(C.byref(s), 1) == -1
+    assert lib.svoxb_gated_scan_backward(C.byref(s), None, None, None, None, None, None, None,
+                                         None) == 2
+    s = call()[1]
+    assert lib.svoxb_gated_scan_backward(C.byref(s), None, None, None, None, None, None, None,
+                                         None) == 1         # no kept states
