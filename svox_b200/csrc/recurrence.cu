@@ -2,6 +2,9 @@
 // kernels.
 #include "recurrence.cuh"
 
+#include <initializer_list>
+#include <type_traits>
+
 #include "status.h"
 
 namespace svoxb {
@@ -16,8 +19,6 @@ int status_of_recurrence(int clear, int* word) {
 }
 
 namespace {
-
-constexpr int kSteps = 8;           // steps of a thread's stretch
 
 size_t type_size(int type) { return type == SVOXB_TYPE_F32 ? 4 : 2; }
 
@@ -38,21 +39,32 @@ int validate(const svoxb_scan* s) {
 
 struct Plan {
     ScanArgs p{};
-    int wide = 1;               // channels of a thread
-    int64_t steps = 0;          // of all rows
+    bool channel_gates = false;     // a gate for each channel, or spread to one
+    int chunk = 1;                  // steps of a tile
+    int64_t steps = 0;              // of all rows
     int64_t blocks = 0;
-    int chunk() const { return p.segs * kSteps; }
-    int64_t kept() const {      // states kept for the backward pass
+    int64_t kept() const {          // states kept for the backward pass
         if (p.B == 0) return 0;
-        return (p.offsets ? p.T / chunk() + p.B : p.B * ((p.T + chunk() - 1) / chunk())) * p.C;
+        return (p.offsets ? p.T / chunk + p.B : p.B * ((p.T + chunk - 1) / chunk)) * p.C;
     }
     int64_t pair_bytes() const { return p.splits > 1 ? p.B * p.splits * p.C * 8 : 0; }
     int64_t part_bytes() const { return p.parts > 1 ? (int64_t)p.parts * steps * p.H * 4 : 0; }
 };
 
-// What decides the layout of the kept states comes from the sizes alone: the forward and the
-// backward pass have to agree on it.  `pairs`: whether a thread may take two channels.
-Plan make_plan(const svoxb_scan* s, bool pairs = true) {
+// The largest of 16, 4 and `size` bytes that the address, the strides and the width of a tile's rows
+// (`counts`, in elements) are multiples of.
+int copied_at_once(const void* ptr, size_t size, std::initializer_list<int64_t> counts) {
+    for (const size_t n : {(size_t)16, (size_t)4}) {
+        bool fits = reinterpret_cast<uintptr_t>(ptr) % n == 0;
+        for (const int64_t c : counts) fits = fits && c * (int64_t)size % (int64_t)n == 0;
+        if (fits) return (int)n;
+    }
+    return (int)size;
+}
+
+// The tiles of a call.  Nothing that decides the layout of the kept states (tile, chunk) looks at
+// more than the sizes: the forward and the backward pass have to agree on it.
+Plan make_plan(const svoxb_scan* s) {
     Plan plan;
     ScanArgs& p = plan.p;
     p.x = s->values; p.g = s->thickness; p.h0 = s->initial; p.offsets = s->offsets;
@@ -61,55 +73,93 @@ Plan make_plan(const svoxb_scan* s, bool pairs = true) {
     p.hb = s->initial_row;
     p.reverse = s->reverse; p.weighted = s->weighted;
     plan.steps = p.offsets ? p.T : p.B * p.T;
-    // two channels to a thread where every row of them lies on a boundary of two
-    auto even = [](const void* ptr, int64_t row, int64_t step, size_t size) {
-        return reinterpret_cast<uintptr_t>(ptr) % (2 * size) == 0 && row % 2 == 0 && step % 2 == 0;
-    };
     const size_t vs = type_size(s->values_type), gs = type_size(s->thickness_type);
-    if (pairs && p.C % 2 == 0 && (p.D == 1 || p.D % 2 == 0) && even(p.x, p.xb, p.xs, vs) &&
-        (p.D > 1 || even(p.g, p.gb, p.gs, gs)) && p.C > 32)
-        plan.wide = 2;
-    const int W = 32 * plan.wide;
+    const int V = vs == 2 ? 2 : 1, L = 16 / V, W = 32 * V;
+    // (a lane's two channels share a gate, or have one each)
+    plan.channel_gates = p.D == 1 || p.D % V != 0;
     p.parts = 1;
-    if (p.D == 1) {
-        p.tile = W;
-        p.tiles = (p.C + W - 1) / W;
-    } else if (p.D <= W) {
-        p.tile = W / p.D * p.D;
-        p.tiles = (p.C + p.tile - 1) / p.tile;
-    } else {
-        p.parts = (p.D + W - 1) / W;
-        p.tile = W;
-        p.tiles = p.H * p.parts;
-    }
+    int width;                      // of the widest tile
+    if (p.D == 1) width = p.C < W ? p.C : W;
+    else if (p.D <= W) width = p.C < W ? p.C : W / p.D * p.D;
+    else { p.parts = (p.D + W - 1) / W; width = W; }
+    p.lanes = 8;
+    while (p.lanes * V < width) p.lanes *= 2;
+    p.tile = width;
+    p.tiles = p.parts > 1 ? p.H * p.parts : (p.C + width - 1) / width;
     p.units = p.B * p.tiles;
     // (rows of a packed call: as long as twice the average)
     const int64_t len = p.offsets ? (p.B > 0 ? (2 * p.T + p.B - 1) / p.B : 0) : p.T;
-    p.segs = 1;
-    while (p.segs < kScanWarps && p.segs * kSteps < len) p.segs *= 2;
-    const int per = kScanWarps / p.segs;
+    p.warps = 1;
+    while (p.warps < kScanWarps && p.warps * (32 / p.lanes) * L < len) p.warps *= 2;
+    plan.chunk = p.warps * (32 / p.lanes) * L;
+    const int per = kScanWarps / p.warps;
     plan.blocks = (p.units + per - 1) / per;
     p.splits = 1;
-    const int64_t chunks = (len + plan.chunk() - 1) / plan.chunk(), want = 4 * (int64_t)sm_count();
-    if (plan.blocks > 0 && plan.blocks * 2 < want && chunks >= 8) {
+    const int64_t chunks = (len + plan.chunk - 1) / plan.chunk, want = 2 * (int64_t)sm_count();
+    if (plan.blocks > 0 && plan.blocks * 2 <= want && chunks >= 8) {
         int64_t n = want / plan.blocks;
         if (n > chunks / 4) n = chunks / 4;
         if (n > 256) n = 256;
         p.splits = (int)n;
     }
+    const int64_t tiles_of = (chunks + p.splits - 1) / p.splits;
+    p.stages = tiles_of < 1 ? 1 : tiles_of < kScanStages ? (int)tiles_of : kScanStages;
+    const int64_t last = p.parts > 1 ? p.D % p.tile : p.C % p.tile;
+    const int64_t start = p.parts > 1 ? p.D : p.tile;       // distances of the tiles' starts
+    p.x_bytes = copied_at_once(p.x, vs, {p.xb, p.xs, p.tile, last, start});
+    p.d_bytes = (int)vs;
+    p.g_bytes = copied_at_once(p.g, gs, {p.gb, p.gs, p.tile, last, start});
     return plan;
 }
 
-template <class VT, class GT, int V, bool PC>
+// Rows of C elements of `ptr` lie on boundaries of two, tile by tile.
+bool in_twos(const Plan& plan, const void* ptr, int type) {
+    const ScanArgs& p = plan.p;
+    return reinterpret_cast<uintptr_t>(ptr) % (2 * type_size(type)) == 0 && p.C % 2 == 0 &&
+           p.tile % 2 == 0 && (p.parts == 1 || p.D % 2 == 0);
+}
+
+template <class Kernel>
+int ready(Kernel kernel, size_t smem) {
+    int per_sm = 0;
+    return blocks_per_sm(reinterpret_cast<const void*>(kernel), kScanBlock, smem, &per_sm);
+}
+
+template <class VT, class GT, bool PC, int MODE>
+int launch_scan(const Plan& plan, const void* x, float2* pairs, void* states, float* last,
+                float* kept, cudaStream_t stream) {
+    using S = ScanShape<VT, GT, PC>;
+    const size_t smem = (size_t)kScanWarps * plan.p.stages * (S::kX + S::kG);
+    auto kernel = scan_kernel<VT, GT, PC, MODE>;
+    const int st = ready(kernel, smem);
+    if (st) return st;
+    kernel<<<dim3((unsigned)plan.blocks, plan.p.splits), kScanBlock, smem, stream>>>(
+        plan.p, static_cast<const VT*>(x), pairs, static_cast<VT*>(states), last, kept);
+    SVOXB_CUDA(cudaGetLastError());
+    return SVOXB_OK;
+}
+
+template <class VT, class GT, bool PC>
 int run_forward(const Plan& plan, void* states, float* last, float* kept, void* workspace,
                 cudaStream_t stream) {
     const ScanArgs& p = plan.p;
-    const dim3 grid((unsigned)plan.blocks, p.splits);
     float2* pairs = static_cast<float2*>(workspace);
-    if (p.splits > 1) {
-        scan_pairs_kernel<VT, GT, V, PC, kSteps, false><<<grid, kScanBlock, 0, stream>>>(
-            p, nullptr, pairs);
+    if (p.offsets == nullptr && p.T <= kFewSteps && p.B * p.C < (1LL << 37)) {
+        auto few = [&](auto w) {
+            constexpr int W = decltype(w)::value;
+            const int64_t n = p.B * (p.C / W);
+            scan_few_kernel<VT, GT, W><<<(unsigned)((n + 127) / 128), 128, 0, stream>>>(
+                p, static_cast<VT*>(states), last, kept);
+        };
+        if (p.paired && p.x_bytes >= 2 * (int)sizeof(VT)) few(std::integral_constant<int, 2>{});
+        else few(std::integral_constant<int, 1>{});
         SVOXB_CUDA(cudaGetLastError());
+        return SVOXB_OK;
+    }
+    if (p.splits > 1) {
+        const int st = launch_scan<VT, GT, PC, 1>(plan, p.x, pairs, nullptr, nullptr, nullptr,
+                                                  stream);
+        if (st) return st;
         if (states == nullptr && kept == nullptr) {
             scan_last_kernel<<<(unsigned)((p.B * p.C + 255) / 256), 256, 0, stream>>>(p, pairs,
                                                                                     last);
@@ -117,27 +167,36 @@ int run_forward(const Plan& plan, void* states, float* last, float* kept, void* 
             return SVOXB_OK;
         }
     }
-    scan_kernel<VT, GT, V, PC, kSteps><<<grid, kScanBlock, 0, stream>>>(
-        p, pairs, static_cast<VT*>(states), last, kept);
-    SVOXB_CUDA(cudaGetLastError());
-    return SVOXB_OK;
+    return launch_scan<VT, GT, PC, 0>(plan, p.x, pairs, states, last, kept, stream);
 }
 
-template <class VT, class GT, int V, bool PC>
+template <class VT, class GT, bool PC>
 int run_backward(const Plan& plan, const float* kept, const void* d, const float* d_last,
                  void* dx, void* dg, float* dh0, void* workspace, cudaStream_t stream) {
+    using S = ScanShape<VT, GT, PC>;
     const ScanArgs& p = plan.p;
-    const dim3 grid((unsigned)plan.blocks, p.splits);
     float2* pairs = static_cast<float2*>(workspace);
     float* parted = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.pair_bytes());
-    const VT* dv = static_cast<const VT*>(d);
     if (p.splits > 1) {
-        scan_pairs_kernel<VT, GT, V, PC, kSteps, true><<<grid, kScanBlock, 0, stream>>>(p, dv,
-                                                                                      pairs);
-        SVOXB_CUDA(cudaGetLastError());
+        // the gradients of the states in the values' place
+        Plan back = plan;
+        back.p.xb = 0;
+        back.p.xs = p.C;
+        back.p.x_bytes = p.d_bytes;
+        if (!p.offsets) back.p.xb = p.T * p.C;
+        const int st = launch_scan<VT, GT, PC, 2>(back, d, pairs, nullptr, nullptr, nullptr, stream);
+        if (st) return st;
     }
-    scan_back_kernel<VT, GT, V, PC, kSteps><<<grid, kScanBlock, 0, stream>>>(
-        p, pairs, kept, dv, d_last, static_cast<VT*>(dx), static_cast<GT*>(dg), parted, dh0);
+    Plan two = plan;                    // three arrays: two tiles of each are as much as fits twice
+    if (two.p.stages > 2) two.p.stages = 2;
+    const size_t smem = (size_t)kScanWarps * (two.p.stages * (2 * S::kX + S::kG) +
+                                              (p.D > 1 ? S::kSum : 0));
+    auto kernel = scan_back_kernel<VT, GT, PC>;
+    const int st = ready(kernel, smem);
+    if (st) return st;
+    kernel<<<dim3((unsigned)plan.blocks, p.splits), kScanBlock, smem, stream>>>(
+        two.p, static_cast<const VT*>(p.x), pairs, kept, static_cast<const VT*>(d), d_last,
+        static_cast<VT*>(dx), static_cast<GT*>(dg), parted, dh0);
     SVOXB_CUDA(cudaGetLastError());
     if (p.parts > 1 && dg != nullptr) {
         scan_parts_kernel<GT><<<(unsigned)((plan.steps * p.H + 255) / 256), 256, 0, stream>>>(
@@ -147,20 +206,16 @@ int run_backward(const Plan& plan, const float* kept, const void* d, const float
     return SVOXB_OK;
 }
 
-// Calls f with the values' and the gates' type, the channels of a thread, and whether each channel
-// has a gate of its own.
+// Calls f with the values' and the gates' type, and whether each channel has a gate of its own.
 template <class VT, class GT> struct Types { using V = VT; using G = GT; };
-template <int N> struct Int { static constexpr int value = N; };
-template <bool B> struct Bool { static constexpr bool value = B; };
 template <class F>
 int with_kernel(const svoxb_scan* s, const Plan& plan, F f) {
     auto types = [&](auto t) {
-        const bool pc = plan.p.D == 1;
-        if (plan.wide == 2) return pc ? f(t, Int<2>{}, Bool<true>{}) : f(t, Int<2>{}, Bool<false>{});
-        return pc ? f(t, Int<1>{}, Bool<true>{}) : f(t, Int<1>{}, Bool<false>{});
+        return plan.channel_gates ? f(t, std::true_type{}) : f(t, std::false_type{});
     };
     const bool same = s->thickness_type == s->values_type;
     switch (s->values_type) {
+        // (a lane has one channel: gates that are shared stay shared)
         case SVOXB_TYPE_F32: return types(Types<float, float>{});
         case SVOXB_TYPE_BF16:
             return same ? types(Types<__nv_bfloat16, __nv_bfloat16>{})
@@ -168,10 +223,6 @@ int with_kernel(const svoxb_scan* s, const Plan& plan, F f) {
         default:
             return same ? types(Types<__half, __half>{}) : types(Types<__half, float>{});
     }
-}
-
-bool on_pairs(const void* ptr, int type) {
-    return reinterpret_cast<uintptr_t>(ptr) % (2 * type_size(type)) == 0;
 }
 
 int too_many(const Plan& plan) {
@@ -193,13 +244,8 @@ int64_t svoxb_gated_scan_kept(const svoxb_scan* s) {
 
 int64_t svoxb_gated_scan_workspace(const svoxb_scan* s, int backward) {
     if (validate(s) != SVOXB_OK) return -1;
-    int64_t most = 0;
-    for (const bool pairs : {false, true}) {
-        const Plan plan = make_plan(s, pairs);
-        const int64_t bytes = plan.pair_bytes() + (backward ? plan.part_bytes() : 0);
-        if (bytes > most) most = bytes;
-    }
-    return most;
+    const Plan plan = make_plan(s);
+    return plan.pair_bytes() + (backward ? plan.part_bytes() : 0);
 }
 
 int svoxb_gated_scan(const svoxb_scan* s, void* states, float* last, float* kept, void* workspace,
@@ -212,12 +258,13 @@ int svoxb_gated_scan(const svoxb_scan* s, void* states, float* last, float* kept
             SVOXB_CUDA(cudaMemsetAsync(states, 0, s->T * s->C * type_size(s->values_type), str));
         return SVOXB_OK;
     }
-    const Plan plan = make_plan(s, on_pairs(states, s->values_type));
+    Plan plan = make_plan(s);
+    plan.p.paired = in_twos(plan, states, s->values_type);
     if (!last || (plan.pair_bytes() > 0 && !workspace)) return SVOXB_ERR_NULL;
     if (too_many(plan)) return SVOXB_ERR_TOO_LARGE;
-    return with_kernel(s, plan, [&](auto t, auto v, auto pc) {
+    return with_kernel(s, plan, [&](auto t, auto pc) {
         using K = decltype(t);
-        return run_forward<typename K::V, typename K::G, decltype(v)::value, decltype(pc)::value>(
+        return run_forward<typename K::V, typename K::G, decltype(pc)::value>(
             plan, states, last, kept, workspace, str);
     });
 }
@@ -238,15 +285,19 @@ int svoxb_gated_scan_backward(const svoxb_scan* s, const float* kept, const void
         }
         return SVOXB_OK;
     }
-    const Plan plan = make_plan(s, on_pairs(d_states, s->values_type) &&
-                                       on_pairs(d_values, s->values_type) &&
-                                       (s->H != s->C || on_pairs(d_thickness, s->thickness_type)));
+    Plan plan = make_plan(s);
+    plan.p.paired = in_twos(plan, d_values, s->values_type) &&
+                    (s->H != s->C || in_twos(plan, d_thickness, s->thickness_type));
+    plan.p.d_bytes = copied_at_once(d_states, type_size(s->values_type),
+                                    {s->C, plan.p.tile, plan.p.C % plan.p.tile,
+                                     plan.p.parts > 1 ? plan.p.D : 0,
+                                     plan.p.parts > 1 ? plan.p.D % plan.p.tile : 0});
     if ((plan.kept() > 0 && !kept) || (plan.pair_bytes() + plan.part_bytes() > 0 && !workspace))
         return SVOXB_ERR_NULL;
     if (too_many(plan)) return SVOXB_ERR_TOO_LARGE;
-    return with_kernel(s, plan, [&](auto t, auto v, auto pc) {
+    return with_kernel(s, plan, [&](auto t, auto pc) {
         using K = decltype(t);
-        return run_backward<typename K::V, typename K::G, decltype(v)::value, decltype(pc)::value>(
+        return run_backward<typename K::V, typename K::G, decltype(pc)::value>(
             plan, kept, d_states, d_last, d_values, d_thickness, d_initial, workspace, str);
     });
 }

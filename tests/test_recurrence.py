@@ -1,9 +1,12 @@
 """The gated recurrence and compositing against a plain loop in 64 bits.
 
 Tolerances come with the reference: it carries a bound of the rounding errors along.  With u =
-2^-24, a step of the kernel multiplies by a = exp(-g) (expf: 2 ulp, 4 u) and by w = 1 - a (below 14 u + u
-where it is a difference, g >= 0.25; below 2 u as a series) and adds, in whatever association the
-stretches are joined; every factor and sum enters the error once, so with the sums of magnitudes
+2^-24, a step of the kernel multiplies by a = exp(-g) (off by 4 u, the hardware's power of two, and
+1.5 g u, its argument) and by w = 1 - a (below 14 u + u where it is a difference, g >= 0.25; below 3 u
+as a series) and adds, in whatever association the stretches are joined; every factor and sum enters
+the error once (where g > 8, a is below 2^-11 of the w |x| beside it, unless x is 0: such states are
+compared through the half step of their last rounding and 2^-24 of the state before), so with the
+sums of magnitudes
     H[t] = a H[t-1] + w |x|,   e[t] = a e[t-1] + (a H[t-1] + w |x|)
 the state is off by at most 20 u e[t], and likewise the adjoint.  Outputs of 16 bits are rounded once
 more, by half a step."""
