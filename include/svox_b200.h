@@ -426,20 +426,23 @@ typedef struct {
     int32_t thickness_type;
     int32_t reverse;
     int32_t weighted;
+    int32_t last_only;       /* no states are wanted, now or for the backward pass */
+    int32_t reserved_;
 } svoxb_scan;
 
 /* Floats that `kept` needs, bytes that `workspace` needs (-1: bad arguments). */
 int64_t svoxb_gated_scan_kept(const svoxb_scan* scan);
 int64_t svoxb_gated_scan_workspace(const svoxb_scan* scan, int backward);
 
-/* states: all states, contiguous like `values` without strides and in its type, or null; last:
+/* states: all states, contiguous like `values` without strides and in its type (null, and only
+ * then, if last_only); last:
  * (B, C) the state after each row; kept: null, or what the backward pass needs.  Steps of a packed
  * call that no row covers get zeros. */
 int svoxb_gated_scan(const svoxb_scan* scan, void* states, float* last, float* kept,
                      void* workspace, void* stream);
 
-/* The gradients of sum(d_states * states) + sum(d_last * last): d_states (contiguous) and d_last may
- * be null, and so may each output.  `kept`: from the forward call with the same arguments. */
+/* The gradients of sum(d_states * states) + sum(d_last * last): d_states (contiguous; null if
+ * last_only) and d_last may be null, and so may each output.  `kept`: from the forward call with the same arguments. */
 int svoxb_gated_scan_backward(const svoxb_scan* scan, const float* kept, const void* d_states,
                               const float* d_last, void* d_values, void* d_thickness,
                               float* d_initial, void* workspace, void* stream);

@@ -19,7 +19,9 @@ UNITS = {
                      "render.cuh", "render_index.cuh", "render_queue.cuh", "render_back.cuh",
                      "render_replay.cuh", "noalloc.cuh", "collective.cuh", "open_groups.h",
                      "status.h", _HEADER],
-    "recurrence.cu": ["recurrence.cuh", "common.cuh", "arith.cuh", "status.h", _HEADER],
+    "recurrence.cu": ["recurrence.cuh", "rays.h", "common.cuh", "arith.cuh", "status.h", _HEADER],
+    "rays.cu": ["rays.cuh", "rays.h", "recurrence.cuh", "common.cuh", "arith.cuh", "status.h",
+                _HEADER],
     "records.cu": ["records.cuh", "common.cuh", "arith.cuh", "status.h", _HEADER],
 }
 

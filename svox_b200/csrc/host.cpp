@@ -693,6 +693,7 @@ void Scan::bind() {
     c.thickness_type = element_type(thickness.scalar_type());
     c.reverse = reverse;
     c.weighted = weighted;
+    c.last_only = !states;
 }
 
 Scan read_scan(const Tensor& values, const Tensor& thickness, const optional<Tensor>& initial,

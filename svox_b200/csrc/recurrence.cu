@@ -5,6 +5,7 @@
 #include <initializer_list>
 #include <type_traits>
 
+#include "rays.h"
 #include "status.h"
 
 namespace svoxb {
@@ -239,11 +240,13 @@ extern "C" {
 
 int64_t svoxb_gated_scan_kept(const svoxb_scan* s) {
     if (validate(s) != SVOXB_OK) return -1;
+    if (const int group = ray_group(s)) return ray_kept(s, group);
     return make_plan(s).kept();
 }
 
 int64_t svoxb_gated_scan_workspace(const svoxb_scan* s, int backward) {
     if (validate(s) != SVOXB_OK) return -1;
+    if (ray_group(s)) return 0;
     const Plan plan = make_plan(s);
     return plan.pair_bytes() + (backward ? plan.part_bytes() : 0);
 }
@@ -258,9 +261,12 @@ int svoxb_gated_scan(const svoxb_scan* s, void* states, float* last, float* kept
             SVOXB_CUDA(cudaMemsetAsync(states, 0, s->T * s->C * type_size(s->values_type), str));
         return SVOXB_OK;
     }
+    const bool any_states = s->offsets ? s->T > 0 : s->B * s->T > 0;
+    if (!last || (any_states && (states == nullptr) != (s->last_only != 0))) return SVOXB_ERR_NULL;
+    if (const int group = ray_group(s)) return ray_forward(s, group, last, kept, str);
     Plan plan = make_plan(s);
     plan.p.paired = in_twos(plan, states, s->values_type);
-    if (!last || (plan.pair_bytes() > 0 && !workspace)) return SVOXB_ERR_NULL;
+    if (plan.pair_bytes() > 0 && !workspace) return SVOXB_ERR_NULL;
     if (too_many(plan)) return SVOXB_ERR_TOO_LARGE;
     return with_kernel(s, plan, [&](auto t, auto pc) {
         using K = decltype(t);
@@ -284,6 +290,11 @@ int svoxb_gated_scan_backward(const svoxb_scan* s, const float* kept, const void
                                            str));
         }
         return SVOXB_OK;
+    }
+    if (s->last_only && d_states) return SVOXB_ERR_OPTION;
+    if (const int group = ray_group(s)) {
+        if (ray_kept(s, group) > 0 && !kept) return SVOXB_ERR_NULL;
+        return ray_backward(s, group, kept, d_last, d_values, d_thickness, d_initial, str);
     }
     Plan plan = make_plan(s);
     plan.p.paired = in_twos(plan, d_values, s->values_type) &&

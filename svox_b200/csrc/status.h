@@ -4,5 +4,6 @@
 
 namespace svoxb {
 int status_of_recurrence(int clear, int* word);
+int status_of_rays(int clear, int* word);
 int status_of_records(int clear, int* word);
 }  // namespace svoxb

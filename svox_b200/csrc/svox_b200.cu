@@ -1155,7 +1155,7 @@ int svoxb_device_status(int clear, void* stream) {
         const int zero = 0;
         SVOXB_CUDA(cudaMemcpyToSymbol(g_status, &zero, sizeof(int)));
     }
-    for (auto more : {status_of_recurrence, status_of_records}) {
+    for (auto more : {status_of_recurrence, status_of_rays, status_of_records}) {
         int other = 0;
         const int st = more(clear, &other);
         if (st) return st;

@@ -4,11 +4,10 @@ Tolerances come with the reference: it carries a bound of the rounding errors al
 2^-24, a step of the kernel multiplies by a = exp(-g) (off by 4 u, the hardware's power of two, and
 1.5 g u, its argument) and by w = 1 - a (below 14 u + u where it is a difference, g >= 0.25; below 3 u
 as a series) and adds, in whatever association the stretches are joined; every factor and sum enters
-the error once (where g > 8, a is below 2^-11 of the w |x| beside it, unless x is 0: such states are
-compared through the half step of their last rounding and 2^-24 of the state before), so with the
-sums of magnitudes
-    H[t] = a H[t-1] + w |x|,   e[t] = a e[t-1] + (a H[t-1] + w |x|)
-the state is off by at most 20 u e[t], and likewise the adjoint.  Outputs of 16 bits are rounded once
+the error once, so with the sums of magnitudes
+    H[t] = a H[t-1] + w |x|,   e[t] = a e[t-1] + ((1 + g / 10) a H[t-1] + w |x|)
+the state is off by at most 20 u e[t], and likewise the adjoint.  (Where the transmittance of several
+steps is exp of their summed thickness, the sum's roundings are g u a step as well.)  Outputs of 16 bits are rounded once
 more, by half a step."""
 import pytest
 import torch
@@ -46,6 +45,7 @@ def reference(values, thickness, initial, offsets, reverse, weighted, d_states=N
     dl = torch.zeros(B, C, dtype=torch.float64) if d_last is None else d_last.cpu().double()
     a = torch.exp(-g)
     w = torch.ones_like(a) if weighted else -torch.expm1(-g)
+    f = torch.where(a == 0, torch.ones_like(a), 1 + 0.1 * g)
     take = torch.where(w == 0, torch.zeros_like(x), w * x)
     out = {n: torch.zeros_like(x) for n in ("states", "e_states", "dx", "e_dx", "dgc", "e_dgc")}
     last, e_last, d0, e_d0 = (torch.zeros(B, C, dtype=torch.float64) for _ in range(4))
@@ -60,7 +60,7 @@ def reference(values, thickness, initial, offsets, reverse, weighted, d_states=N
             gone = a[t] == 0
             z = torch.zeros_like(h)
             ah, aH, ae = (torch.where(gone, z, a[t] * q) for q in (h, Habs, e))
-            e = ae + aH + take[t].abs()
+            e = ae + f[t] * aH + take[t].abs()
             h, Habs = ah + take[t], aH + take[t].abs()
             out["states"][t], out["e_states"][t] = h, e
         last[b], e_last[b] = h, e
@@ -77,8 +77,8 @@ def reference(values, thickness, initial, offsets, reverse, weighted, d_states=N
             qa = torch.where(gone, z, a[t] * (Hp if weighted else xt.abs() + Hp))
             qe = torch.where(gone, z, a[t] * ep)
             out["dgc"][t] = q * G
-            out["e_dgc"][t] = qa * (eG + Gabs) + qe * Gabs + D * qa * Gabs / 20
-            G, Gabs, eG = (torch.where(gone, z, a[t] * v) for v in (G, Gabs, eG + Gabs))
+            out["e_dgc"][t] = qa * (eG + f[t] * Gabs) + qe * Gabs + D * qa * Gabs / 20
+            G, Gabs, eG = (torch.where(gone, z, a[t] * v) for v in (G, Gabs, eG + f[t] * Gabs))
         d0[b], e_d0[b] = G, eG
 
     def grouped(v):
@@ -207,7 +207,7 @@ def test_composite(cuda_device, C, dtype, packed):
     for name, got in zip(("d_values", "d_thickness", "d_initial"),
                          torch.autograd.grad([out], [x, g, bg], [d])):
         close(name, got, want[name])
-    assert torch.equal(out, svox.gated_scan(x, g, bg, offsets, reverse=True)[1])
+    close("last", svox.gated_scan(x, g, bg, offsets, reverse=True)[1], want["last"])
     with torch.no_grad():
         assert torch.equal(out, svox.composite(x, g, bg, offsets))
 
@@ -536,13 +536,14 @@ def test_abi_refusals():
                     ("thickness_row", C.c_int64), ("thickness_step", C.c_int64),
                     ("initial_row", C.c_int64), ("C", C.c_int32), ("H", C.c_int32),
                     ("values_type", C.c_int32), ("thickness_type", C.c_int32),
-                    ("reverse", C.c_int32), ("weighted", C.c_int32)]
+                    ("reverse", C.c_int32), ("weighted", C.c_int32),
+                    ("last_only", C.c_int32), ("reserved_", C.c_int32)]
 
     lib = csrc.library()
     lib.svoxb_gated_scan_kept.restype = lib.svoxb_gated_scan_workspace.restype = C.c_int64
 
     def call(**k):
-        s = Scan(16, 16, None, None, 2, 3, 12, 4, 3, 1, 0, 4, 1, 0, 0, 0, 0)
+        s = Scan(16, 16, None, None, 2, 3, 12, 4, 3, 1, 0, 4, 1, 0, 0, 0, 0, 1, 0)
         for name, v in k.items():
             setattr(s, name, v)
         return lib.svoxb_gated_scan(C.byref(s), None, None, None, None, None), s
@@ -552,6 +553,7 @@ def test_abi_refusals():
     assert call(B=-1)[0] == 2 and call(T=-1)[0] == 2 and call(C=0)[0] == 2 and call(H=3)[0] == 2
     assert call(values_type=3)[0] == 3 and call(thickness_type=1)[0] == 3
     assert call(T=1 << 41)[0] == 8
+    assert call(last_only=0)[0] == 1                        # no states
     assert call(B=0)[0] == 0                                # nothing to do
     assert lib.svoxb_gated_scan(None, None, None, None, None, None) == 1
     s = call(H=3)[1]
