@@ -20,7 +20,8 @@ int status_of_rays(int clear, int* word) {
 int ray_group(const svoxb_scan* s) {
     if (!s->last_only || !s->reverse || s->H != 1 || s->C > kRayChannels) return 0;
     const int64_t mean = s->offsets ? (s->B > 0 ? s->T / s->B : 0) : s->T;
-    if (mean > kRayLongest || s->B > (1LL << 33)) return 0;
+    // (their lengths are counted in 32 bits)
+    if (mean > kRayLongest || (s->offsets && s->T > 0x7fffffff)) return 0;
     return mean <= kRayShort ? 8 : 32;
 }
 
