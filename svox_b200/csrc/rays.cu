@@ -8,6 +8,12 @@
 
 namespace svoxb {
 
+// Rays of at most this many samples on average: beyond, a ray is split among blocks instead.
+constexpr int64_t kRayLongest = 4096;
+// Up to this many a ray gets 8 lanes instead of 32 (a sample each); by quads 4, up to the next 8.
+constexpr int64_t kRayShort = 12;
+constexpr int64_t kQuadsFew = 10, kQuadsMany = 160;
+
 int status_of_rays(int clear, int* word) {
     SVOXB_CUDA(cudaMemcpyFromSymbol(word, g_status, sizeof(int)));
     if (clear && *word != 0) {
@@ -17,16 +23,31 @@ int status_of_rays(int clear, int* word) {
     return SVOXB_OK;
 }
 
-int ray_group(const svoxb_scan* s) {
-    if (!s->last_only || !s->reverse || s->H != 1 || s->C > kRayChannels) return 0;
+RayPlan ray_plan(const svoxb_scan* s) {
+    RayPlan plan;
+    if (!s->last_only || !s->reverse || s->H != 1 || s->C > kRayChannels) return plan;
     const int64_t mean = s->offsets ? (s->B > 0 ? s->T / s->B : 0) : s->T;
     // (their lengths are counted in 32 bits)
-    if (mean > kRayLongest || (s->offsets && s->T > 0x7fffffff)) return 0;
-    return mean <= kRayShort ? 8 : 32;
+    if (mean > kRayLongest || (s->offsets && s->T > 0x7fffffff - 256)) return plan;
+    const bool dense = s->values_step == s->C && s->thickness_step == 1 &&
+                       (s->offsets || ((s->values_row == s->T * s->C || s->B == 1) &&
+                                       (s->thickness_row == s->T || s->B == 1)));
+    const auto on = [](const void* ptr, int type) {
+        return reinterpret_cast<uintptr_t>(ptr) % (type == SVOXB_TYPE_F32 ? 16 : 8) == 0;
+    };
+    plan.quads = dense && on(s->values, s->values_type) && on(s->thickness, s->thickness_type);
+    if (plan.quads) plan.lanes = mean <= kQuadsFew ? 4 : mean <= kQuadsMany ? 8 : 32;
+    else plan.lanes = mean <= kRayShort ? 8 : 32;
+    return plan;
 }
 
-int64_t ray_kept(const svoxb_scan* s, int group) {
-    return s->offsets ? s->T / group + s->B : s->B * ((s->T + group - 1) / group);
+// Floats that the forward keeps: the thickness in front of every chunk.  The chunks of quads begin
+// with the ray's first quad, up to three samples in front of it, so that a ray may have one more:
+// two rays never share an entry where ray b begins at first / chunk + 2 b.
+int64_t ray_kept(const svoxb_scan* s, RayPlan plan) {
+    const int chunk = plan.lanes * (plan.quads ? 4 : 1), more = plan.quads ? 1 : 0;
+    return s->offsets ? s->T / chunk + s->B * (1 + more)
+                      : s->B * ((s->T + chunk - 1) / chunk + more);
 }
 
 namespace {
@@ -46,10 +67,13 @@ ScanArgs ray_args(const svoxb_scan* s) {
 template <class VT, class GT> struct Types { using V = VT; using G = GT; };
 template <int N> using Int = std::integral_constant<int, N>;
 template <class F>
-void with_kernel(const svoxb_scan* s, int group, F f) {
+void with_kernel(const svoxb_scan* s, RayPlan plan, F f) {
     auto lanes = [&](auto t, auto c) {
-        if (group == 8) f(t, c, Int<8>{});
-        else f(t, c, Int<32>{});
+        if (plan.quads && plan.lanes == 4) f(t, c, Int<4>{}, std::true_type{});
+        else if (plan.quads && plan.lanes == 8) f(t, c, Int<8>{}, std::true_type{});
+        else if (plan.quads) f(t, c, Int<32>{}, std::true_type{});
+        else if (plan.lanes == 8) f(t, c, Int<8>{}, std::false_type{});
+        else f(t, c, Int<32>{}, std::false_type{});
     };
     auto types = [&](auto t) {
         switch (s->C) {
@@ -67,32 +91,44 @@ void with_kernel(const svoxb_scan* s, int group, F f) {
     else types(Types<__half, float>{});
 }
 
-unsigned blocks_of(const svoxb_scan* s, int group) {
-    return (unsigned)((s->B * group + kRayBlock - 1) / kRayBlock);
+unsigned blocks_of(const svoxb_scan* s, RayPlan plan) {
+    return (unsigned)((s->B * plan.lanes + kRayBlock - 1) / kRayBlock);
 }
 
 }  // namespace
 
-int ray_forward(const svoxb_scan* s, int group, float* last, float* kept, cudaStream_t stream) {
-    with_kernel(s, group, [&](auto t, auto c, auto g) {
-        using K = decltype(t);
-        ray_kernel<typename K::V, typename K::G, decltype(c)::value, decltype(g)::value>
-            <<<blocks_of(s, group), kRayBlock, 0, stream>>>(ray_args(s), last, kept);
+int ray_forward(const svoxb_scan* s, RayPlan plan, float* last, float* kept, cudaStream_t stream) {
+    const ScanArgs p = ray_args(s);
+    with_kernel(s, plan, [&](auto t, auto c, auto g, auto quads) {
+        using VT = typename decltype(t)::V;
+        using GT = typename decltype(t)::G;
+        constexpr int C = decltype(c)::value, G = decltype(g)::value;
+        if constexpr (decltype(quads)::value)
+            quad_kernel<VT, GT, C, G><<<blocks_of(s, plan), kRayBlock, 0, stream>>>(p, last, kept);
+        else
+            ray_kernel<VT, GT, C, G><<<blocks_of(s, plan), kRayBlock, 0, stream>>>(p, last, kept);
     });
     SVOXB_CUDA(cudaGetLastError());
     return SVOXB_OK;
 }
 
-int ray_backward(const svoxb_scan* s, int group, const float* kept, const float* d_last, void* dx,
+int ray_backward(const svoxb_scan* s, RayPlan plan, const float* kept, const float* d_last, void* dx,
                  void* dg, float* dh0, cudaStream_t stream) {
-    with_kernel(s, group, [&](auto t, auto c, auto g) {
-        using K = decltype(t);
-        using VT = typename K::V;
-        using GT = typename K::G;
-        ray_back_kernel<VT, GT, decltype(c)::value, decltype(g)::value>
-            <<<blocks_of(s, group), kRayBlock, 0, stream>>>(ray_args(s), kept, d_last,
-                                                            static_cast<VT*>(dx),
-                                                            static_cast<GT*>(dg), dh0);
+    ScanArgs p = ray_args(s);
+    with_kernel(s, plan, [&](auto t, auto c, auto g, auto quads) {
+        using VT = typename decltype(t)::V;
+        using GT = typename decltype(t)::G;
+        constexpr int C = decltype(c)::value, G = decltype(g)::value;
+        VT* x = static_cast<VT*>(dx);
+        GT* gates = static_cast<GT*>(dg);
+        p.paired = reinterpret_cast<uintptr_t>(x) % (4 * sizeof(VT)) == 0 &&
+                   reinterpret_cast<uintptr_t>(gates) % (4 * sizeof(GT)) == 0;
+        if constexpr (decltype(quads)::value)
+            quad_back_kernel<VT, GT, C, G><<<blocks_of(s, plan), kRayBlock, 0, stream>>>(
+                p, kept, d_last, x, gates, dh0);
+        else
+            ray_back_kernel<VT, GT, C, G><<<blocks_of(s, plan), kRayBlock, 0, stream>>>(
+                p, kept, d_last, x, gates, dh0);
     });
     SVOXB_CUDA(cudaGetLastError());
     return SVOXB_OK;

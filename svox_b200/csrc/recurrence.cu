@@ -240,13 +240,13 @@ extern "C" {
 
 int64_t svoxb_gated_scan_kept(const svoxb_scan* s) {
     if (validate(s) != SVOXB_OK) return -1;
-    if (const int group = ray_group(s)) return ray_kept(s, group);
+    if (const RayPlan rays = ray_plan(s); rays.lanes) return ray_kept(s, rays);
     return make_plan(s).kept();
 }
 
 int64_t svoxb_gated_scan_workspace(const svoxb_scan* s, int backward) {
     if (validate(s) != SVOXB_OK) return -1;
-    if (ray_group(s)) return 0;
+    if (ray_plan(s).lanes) return 0;
     const Plan plan = make_plan(s);
     return plan.pair_bytes() + (backward ? plan.part_bytes() : 0);
 }
@@ -263,7 +263,8 @@ int svoxb_gated_scan(const svoxb_scan* s, void* states, float* last, float* kept
     }
     const bool any_states = s->offsets ? s->T > 0 : s->B * s->T > 0;
     if (!last || (any_states && (states == nullptr) != (s->last_only != 0))) return SVOXB_ERR_NULL;
-    if (const int group = ray_group(s)) return ray_forward(s, group, last, kept, str);
+    if (const RayPlan rays = ray_plan(s); rays.lanes)
+        return ray_forward(s, rays, last, kept, str);
     Plan plan = make_plan(s);
     plan.p.paired = in_twos(plan, states, s->values_type);
     if (plan.pair_bytes() > 0 && !workspace) return SVOXB_ERR_NULL;
@@ -292,9 +293,9 @@ int svoxb_gated_scan_backward(const svoxb_scan* s, const float* kept, const void
         return SVOXB_OK;
     }
     if (s->last_only && d_states) return SVOXB_ERR_OPTION;
-    if (const int group = ray_group(s)) {
-        if (ray_kept(s, group) > 0 && !kept) return SVOXB_ERR_NULL;
-        return ray_backward(s, group, kept, d_last, d_values, d_thickness, d_initial, str);
+    if (const RayPlan rays = ray_plan(s); rays.lanes) {
+        if (ray_kept(s, rays) > 0 && !kept) return SVOXB_ERR_NULL;
+        return ray_backward(s, rays, kept, d_last, d_values, d_thickness, d_initial, str);
     }
     Plan plan = make_plan(s);
     plan.p.paired = in_twos(plan, d_values, s->values_type) &&

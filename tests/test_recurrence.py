@@ -301,6 +301,51 @@ def test_strides_and_broadcasts(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C", [1, 2, 3, 4])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+def test_composite_wherever_it_lies(cuda_device, C, dtype):
+    """Rays of every length at every place of a quad, in an array that ends anywhere; values and
+    gradients off their boundaries, and with strides."""
+    gen = torch.Generator().manual_seed(C)
+    for lengths in (list(range(1, 40)) + [0, 0, 127, 128, 129, 3, 1], [5], [4], [1, 1, 1], [0, 2, 0],
+                    [600] * 5, [2500, 3, 0, 2499]):
+        n = torch.tensor(lengths)
+        offsets = torch.cat([torch.zeros(1, dtype=torch.int64), n.cumsum(0)]).to(cuda_device)
+        N = int(n.sum())
+        x, g = inputs(gen, (N,), C, 1, dtype, F32 if C % 2 else dtype, cuda_device)
+        bg = torch.rand(n.numel(), C, generator=gen).to(cuda_device)
+        d = torch.randn(n.numel(), C, generator=gen).to(cuda_device)
+        want = reference(x, g, bg, offsets, True, False, None, d)
+        flat = torch.zeros(N * C + 1, device=cuda_device, dtype=dtype)
+        flat[1:] = x.flatten()
+        wide = torch.zeros(N, C + 2, device=cuda_device, dtype=dtype)
+        wide[:, 1:-1] = x
+        gates = torch.zeros(N, 2, device=cuda_device, dtype=g.dtype)
+        gates[:, 1] = g
+        for xv, gv in ((x, g), (flat[1:].view(N, C), g), (wide[:, 1:-1], g), (x, gates[:, 1])):
+            leaves = [xv.detach().requires_grad_(True), gv.detach().requires_grad_(True),
+                      bg.clone().requires_grad_(True)]
+            out = svox.composite(*leaves, offsets)
+            close("last", out, want["last"])
+            for name, got in zip(("d_values", "d_thickness", "d_initial"),
+                                 torch.autograd.grad(out, leaves, d)):
+                close(name, got, want[name])
+            with torch.no_grad():
+                assert torch.equal(svox.composite(xv, gv, bg, offsets), out)
+    for premultiplied in (False, True):
+        x, g = inputs(gen, (3, 37), C, 1, dtype, F32, cuda_device)
+        x.requires_grad_(True)
+        g.requires_grad_(True)
+        out = svox.composite(x, g, premultiplied=premultiplied)
+        d = torch.randn(3, C, generator=gen).to(cuda_device)
+        want = reference(x, g, None, None, True, premultiplied, None, d)
+        close("last", out, want["last"])
+        grads = torch.autograd.grad(out, [x, g], d)
+        close("d_values", grads[0], want["d_values"])
+        close("d_thickness", grads[1], want["d_thickness"])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("C", [3, 64])
 def test_masked_places(cuda_device, C):
     """Samples of no thickness may hold anything; nothing from behind an opaque sample shows."""
