@@ -10,9 +10,15 @@ namespace svoxb {
 
 // Rays of at most this many samples on average: beyond, a ray is split among blocks instead.
 constexpr int64_t kRayLongest = 4096;
-// Up to this many a ray gets 8 lanes instead of 32 (a sample each); by quads 4, up to the next 8.
+// Up to this many a ray gets 8 lanes instead of 32, a sample each.
 constexpr int64_t kRayShort = 12;
-constexpr int64_t kQuadsFew = 10, kQuadsMany = 160;
+// By quads a ray gets 4 lanes, and twice as many beyond each of these averages.  Rays of 3 channels of
+// exponentially distributed lengths, forward and backward, us with 4 / 8 / 16 / 32 lanes:
+//   2^20 rays of 4: 177 / 298 / 557 / 1058, of 20: 422 / 459 / 631 / 1130, of 42: 744 / 712 / 809 / 1225;
+//   2^16 of 84: 172 / 124 / 101 / 111; 2^17 of 160: 585 / 400 / 300 / 285; 2^15 of 600: 859 / 533 / 357 / 268
+constexpr int64_t kQuadsMean[] = {28, 60, 130};
+// Lanes that all rays together can have at once; 4096 rays of 21, forward: 9.1 / 6.0 / 4.3 / 4.0 us.
+constexpr int64_t kQuadsFew = 1 << 17;
 
 int status_of_rays(int clear, int* word) {
     SVOXB_CUDA(cudaMemcpyFromSymbol(word, g_status, sizeof(int)));
@@ -36,8 +42,15 @@ RayPlan ray_plan(const svoxb_scan* s) {
         return reinterpret_cast<uintptr_t>(ptr) % (type == SVOXB_TYPE_F32 ? 16 : 8) == 0;
     };
     plan.quads = dense && on(s->values, s->values_type) && on(s->thickness, s->thickness_type);
-    if (plan.quads) plan.lanes = mean <= kQuadsFew ? 4 : mean <= kQuadsMany ? 8 : 32;
-    else plan.lanes = mean <= kRayShort ? 8 : 32;
+    if (!plan.quads) {
+        plan.lanes = mean <= kRayShort ? 8 : 32;
+        return plan;
+    }
+    plan.lanes = 4;
+    for (const int64_t upto : kQuadsMean)
+        if (mean > upto) plan.lanes *= 2;
+    // few rays: as many lanes as leave none of them without a place
+    while (plan.lanes < 32 && s->B * plan.lanes * 2 <= kQuadsFew) plan.lanes *= 2;
     return plan;
 }
 
@@ -71,6 +84,7 @@ void with_kernel(const svoxb_scan* s, RayPlan plan, F f) {
     auto lanes = [&](auto t, auto c) {
         if (plan.quads && plan.lanes == 4) f(t, c, Int<4>{}, std::true_type{});
         else if (plan.quads && plan.lanes == 8) f(t, c, Int<8>{}, std::true_type{});
+        else if (plan.quads && plan.lanes == 16) f(t, c, Int<16>{}, std::true_type{});
         else if (plan.quads) f(t, c, Int<32>{}, std::true_type{});
         else if (plan.lanes == 8) f(t, c, Int<8>{}, std::false_type{});
         else f(t, c, Int<32>{}, std::false_type{});

@@ -266,7 +266,7 @@ struct RayQuads {
 };
 
 template <class VT, class GT, int C, int G>
-__global__ void __launch_bounds__(kRayBlock)
+__global__ void __launch_bounds__(kRayBlock, 24)
 quad_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
     RayQuads<VT, GT, C, G> th;
     th.init(p);
@@ -283,6 +283,9 @@ quad_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
             const int64_t left = th.rest - (int64_t)k * th.kChunk;
             th.template load<GT, 1>(g, at, left, gv);
             th.template load<VT, C>(x, at, left, xv);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4 * C; ++i) xv[i] = 0.f;
         }
         if (keep != nullptr && k < th.chunks) keep[k] = S;
 #pragma unroll
@@ -317,7 +320,7 @@ quad_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
 }
 
 template <class VT, class GT, int C, int G>
-__global__ void __launch_bounds__(kRayBlock)
+__global__ void __launch_bounds__(kRayBlock, 20)
 quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restrict__ d_last,
                  VT* __restrict__ dx, GT* __restrict__ dg, float* __restrict__ dh0) {
     RayQuads<VT, GT, C, G> th;
@@ -340,6 +343,9 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
             const int64_t left = th.rest - (int64_t)k * th.kChunk;
             th.template load<GT, 1>(g, at, left, gv);
             th.template load<VT, C>(x, at, left, xv);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4 * C; ++i) xv[i] = 0.f;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) gv[i] = th.in(at + i) ? gv[i] : 0.f;
@@ -351,21 +357,27 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
             T_end = decay_of(total);
             behind = past(T_end, bg, 0.f);
         }
-        float T = decay_of(before), W[4], Wc[4], own[4];
+        float T = decay_of(before), W[4], c[4], Wc[4], own[4];
+        unsigned none = 0;          // samples that have no gradient of their thickness
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bool in = th.in(at + i);
-            float c = 0.f;
+            c[i] = 0.f;
 #pragma unroll
-            for (int q = 0; q < C; ++q) c = fmaf(d[q], in ? xv[i * C + q] : 0.f, c);
+            for (int q = 0; q < C; ++q) c[i] = fmaf(d[q], xv[i * C + q], c[i]);
             const float a = decay_of(gv[i]);
-            const float w = p.weighted ? (in ? 1.f : 0.f) : weight_of(gv[i], a);
-            W[i] = T * w;
-            Wc[i] = times(W[i], c);
+            W[i] = T * (p.weighted ? (th.in(at + i) ? 1.f : 0.f) : weight_of(gv[i], a));
+            Wc[i] = W[i] * c[i];
             T *= a;
-            own[i] = p.weighted || T == 0.f ? 0.f : T * c;
-            // (a value that is not finite in a place of no thickness is no sample)
-            if (w == 0.f && !finite(c)) own[i] = __int_as_float(0x7fc00000);
+            own[i] = p.weighted ? 0.f : T * c[i];
+        }
+        if (!finite((c[0] + c[1]) + (c[2] + c[3]))) {
+            // What is not finite counts only where it has weight; where there is no thickness it is
+            // no sample, and behind an opaque one neither.
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                Wc[i] = times(W[i], c[i]);
+                if (!finite(c[i]) && !p.weighted && (gv[i] == 0.f || W[i] == 0.f)) none |= 1u << i;
+            }
         }
         const float here = th.from((Wc[0] + Wc[1]) + (Wc[2] + Wc[3])) + behind;
         float rest = __shfl_down_sync(~0u, here, 1, G);     // what all samples behind the quad bring
@@ -375,9 +387,13 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
             float out[4];
 #pragma unroll
             for (int i = 3; i >= 0; --i) {
-                out[i] = own[i] == own[i] ? own[i] - rest : 0.f;
+                out[i] = own[i] - rest;
                 rest += Wc[i];
             }
+            if (none)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (none >> i & 1) out[i] = 0.f;
             const bool whole = at >= 0 && at + 3 < th.len;
             const int64_t to = th.first + at;
             if (dg != nullptr) {
