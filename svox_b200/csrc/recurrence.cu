@@ -75,24 +75,24 @@ Plan make_plan(const svoxb_scan* s) {
     p.reverse = s->reverse; p.weighted = s->weighted;
     plan.steps = p.offsets ? p.T : p.B * p.T;
     const size_t vs = type_size(s->values_type), gs = type_size(s->thickness_type);
-    const int V = vs == 2 ? 2 : 1, L = 16 / V, W = 32 * V;
     // (a lane's two channels share a gate, or have one each)
-    plan.channel_gates = p.D == 1 || p.D % V != 0;
+    plan.channel_gates = p.D == 1 || p.D % 2 != 0;
+    const int W = 64;
     p.parts = 1;
     int width;                      // of the widest tile
     if (p.D == 1) width = p.C < W ? p.C : W;
     else if (p.D <= W) width = p.C < W ? p.C : W / p.D * p.D;
     else { p.parts = (p.D + W - 1) / W; width = W; }
     p.lanes = 8;
-    while (p.lanes * V < width) p.lanes *= 2;
+    while (p.lanes * 2 < width) p.lanes *= 2;
     p.tile = width;
     p.tiles = p.parts > 1 ? p.H * p.parts : (p.C + width - 1) / width;
     p.units = p.B * p.tiles;
     // (rows of a packed call: as long as twice the average)
     const int64_t len = p.offsets ? (p.B > 0 ? (2 * p.T + p.B - 1) / p.B : 0) : p.T;
     p.warps = 1;
-    while (p.warps < kScanWarps && p.warps * (32 / p.lanes) * L < len) p.warps *= 2;
-    plan.chunk = p.warps * (32 / p.lanes) * L;
+    while (p.warps < kScanWarps && p.warps * (32 / p.lanes) * kSteps < len) p.warps *= 2;
+    plan.chunk = p.warps * (32 / p.lanes) * kSteps;
     const int per = kScanWarps / p.warps;
     plan.blocks = (p.units + per - 1) / per;
     p.splits = 1;
@@ -104,7 +104,9 @@ Plan make_plan(const svoxb_scan* s) {
         p.splits = (int)n;
     }
     const int64_t tiles_of = (chunks + p.splits - 1) / p.splits;
-    p.stages = tiles_of < 1 ? 1 : tiles_of < kScanStages ? (int)tiles_of : kScanStages;
+    // (of 32-bit values two tiles under way fill as much of the shared memory)
+    const int most = vs == 2 ? kScanStages : 2;
+    p.stages = tiles_of < 1 ? 1 : tiles_of < most ? (int)tiles_of : most;
     const int64_t last = p.parts > 1 ? p.D % p.tile : p.C % p.tile;
     const int64_t start = p.parts > 1 ? p.D : p.tile;       // distances of the tiles' starts
     p.x_bytes = copied_at_once(p.x, vs, {p.xb, p.xs, p.tile, last, start});

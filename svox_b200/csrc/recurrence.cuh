@@ -124,6 +124,59 @@ __device__ __forceinline__ float past(float a, float h, float b) {
     return a == 0.f ? b : fmaf(a, h, b);
 }
 
+// Two channels at once: sm_100's packed 32-bit arithmetic, one instruction for both.
+struct F2 { float x, y; };
+__device__ __forceinline__ F2 two(float v) { return {v, v}; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("{.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("{.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ F2 past2(F2 a, F2 h, F2 b) {
+    return {past(a.x, h.x, b.x), past(a.y, h.y, b.y)};
+}
+__device__ __forceinline__ F2 shfl2(F2 v, int lane) {
+    return {__shfl_sync(~0u, v.x, lane), __shfl_sync(~0u, v.y, lane)};
+}
+// 0 where all is finite, NaN otherwise.
+__device__ __forceinline__ float spoilt(F2 a, F2 b) {
+    const F2 r = fma2(a, two(0.f), mul2(b, two(0.f)));
+    return r.x + r.y;
+}
+__device__ __forceinline__ F2 decay2(F2 g) {
+    const F2 t = mul2(g, two(-1.4426950408889634f));
+    F2 a;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a.y) : "f"(t.y));
+    return a;
+}
+__device__ __forceinline__ F2 weight2(F2 g, F2 a) {
+    F2 s = fma2(g, two(-1.f / 720), two(1.f / 120));
+    s = fma2(g, s, two(-1.f / 24));
+    s = fma2(g, s, two(1.f / 6));
+    s = fma2(g, s, two(-0.5f));
+    s = mul2(g, fma2(g, s, two(1.f)));
+    const F2 d = fma2(a, two(-1.f), two(1.f));
+    return {fabsf(g.x) < 0.25f ? s.x : d.x, fabsf(g.y) < 0.25f ? s.y : d.y};
+}
+
 // Steps of a packed call that no row covers, before the first row and behind the last, get zeros.
 template <class T>
 __device__ __forceinline__ void clear_uncovered(const ScanArgs& p, int64_t b, int first, int width,
@@ -146,18 +199,19 @@ __device__ __forceinline__ int64_t kept_index(const ScanArgs& p, const ScanRow& 
 }
 
 // ---------------------------------------------------------------------------
-// Tiles.  A unit (a row's tile of up to `lanes` * V channels) is scanned by `warps` warps; of a warp,
-// each group of `lanes` lanes takes L steps, so that a tile has warps * (32 / lanes) * L steps.  Each
-// warp copies its own part of the tiles to shared memory, asynchronously and up to kScanStages ahead:
-// row l holds what the lanes need for their l-th step, whatever the width of a channel row.
+// Tiles.  A lane has two channels; a unit (a row's tile of up to 2 * `lanes` channels) is scanned by
+// `warps` warps; of a warp, each group of `lanes` lanes takes kSteps steps, so that a tile has
+// warps * (32 / lanes) * kSteps steps.  Each warp copies its own part of the tiles to shared memory,
+// asynchronously and up to kScanStages ahead: row l holds what the lanes need for their l-th step,
+// whatever the width of a channel row.
+constexpr int kSteps = 8;
 template <class VT, class GT, bool PC>
 struct ScanShape {
-    static constexpr int V = sizeof(VT) == 2 ? 2 : 1;      // channels of a lane
-    static constexpr int L = 16 / V;                       // steps of a lane
-    static constexpr int GV = PC ? V : 1;
-    static constexpr int kX = L * 32 * V * sizeof(VT);     // bytes of a warp's tile of values,
-    static constexpr int kG = L * 32 * GV * sizeof(GT);    // of gates
-    static constexpr int kSum = L * (32 * V + 1) * 4;      // of a warp's products for dg
+    static constexpr int GV = PC ? 2 : 1;
+    static constexpr int kX = kSteps * 64 * sizeof(VT);         // bytes of a warp's tile of values,
+    static constexpr int kG = kSteps * 32 * GV * sizeof(GT);    // of gates
+    static constexpr int kPitch = PC ? 65 : 36;                 // of its products for dg
+    static constexpr int kSum = kSteps * kPitch * 4;
 };
 
 __device__ __forceinline__ void copy_async(void* to, const void* from, int bytes, bool in) {
@@ -188,9 +242,9 @@ struct ScanThread {
     ScanTile tile;
     ScanRow row;
     int have;                // channels of this lane
-    bool on;                 // it has some
     int ch;                  // its first channel
     int gate;                // where its gate is in a row of a shared tile of gates
+    int step0;               // its first step within a tile
     int split;
     int64_t k0, k1;          // tiles of this block's range
 
@@ -207,30 +261,32 @@ struct ScanThread {
         row = scan_row(p, b);
         sub = lane / p.lanes;
         cl = lane - sub * p.lanes;
-        have = tile.width - cl * S::V;
-        have = have < 0 ? 0 : have < S::V ? have : S::V;
-        on = have > 0;
-        ch = tile.first + (on ? cl * S::V : 0);
+        have = tile.width - cl * 2;
+        have = have < 0 ? 0 : have < 2 ? have : 2;
+        ch = tile.first + (have ? cl * 2 : 0);
         const int heads = p.parts > 1 ? 1 : p.D > 1 ? tile.width / p.D : 0;
-        gate = PC ? 0 : sub * heads + (p.parts > 1 ? 0 : on ? cl * S::V / p.D : 0);
-        chunk = p.warps * (32 / p.lanes) * S::L;
+        gate = PC ? 0 : sub * heads + (p.parts > 1 ? 0 : have ? cl * 2 / p.D : 0);
+        step0 = (wseg * (32 / p.lanes) + sub) * kSteps;
+        chunk = p.warps * (32 / p.lanes) * kSteps;
         const int64_t chunks = (row.len + chunk - 1) / chunk;
         const int64_t per = (chunks + p.splits - 1) / p.splits;
         k0 = per * split < chunks ? per * split : chunks;
         k1 = per * (split + 1) < chunks ? per * (split + 1) : chunks;
         return true;
     }
-    __device__ __forceinline__ int64_t first_step(const ScanArgs& p, int64_t k, int s) const {
-        return k * chunk + (wseg * (32 / p.lanes) + s) * S::L;
-    }
     __device__ __forceinline__ int64_t place(const ScanArgs& p, int64_t t) const {
         return p.reverse ? row.len - 1 - t : t;
     }
-    // The warp's part of tile k of an array, BYTES at a time.  A lane's pieces lie in one column,
-    // so many rows apart.
+    // Steps of tile k that the row has.
+    __device__ __forceinline__ int room(int64_t k) const {
+        const int64_t left = row.len - k * chunk;
+        return left < chunk ? (int)left : chunk;
+    }
+    // The warp's part of a tile, BYTES at a time.  `from`: the row's first step in the tile; a lane's
+    // pieces lie in one column, so many rows apart.
     template <class T, int W, int BYTES>
-    __device__ __forceinline__ void copy_pieces(const ScanArgs& p, int64_t k, T* to, const T* from,
-                                                int64_t step) const {
+    __device__ __forceinline__ void copy_pieces(const ScanArgs& p, T* to, const T* from,
+                                                int64_t step, int room) const {
         constexpr int n = BYTES / (int)sizeof(T);           // elements of a piece
         constexpr int P = 32 * W / n, COLS = P < 32 ? P : 32, ROWS = 32 / COLS;
         const int each = p.lanes * W;                       // elements of a row of channels
@@ -239,90 +295,123 @@ struct ScanThread {
             const int j = (half + lane % COLS) * n;
             const int s = j >> (31 - __clz(each)), c = j & (each - 1);
             if (c >= tile.width) continue;
-            int64_t t = first_step(p, k, s) + lane / COLS;
-            const T* src = from + place(p, t) * step + c;
-            const int64_t down = (p.reverse ? -ROWS : ROWS) * step;
+            int t = (wseg * (32 / p.lanes) + s) * kSteps + lane / COLS;
+            const T* src = from + t * step + c;
             T* dst = to + lane / COLS * 32 * W + j;
 #pragma unroll
-            for (int l = 0; l < S::L; l += ROWS) {
-                const bool in = t < row.len;
+            for (int l = 0; l < kSteps; l += ROWS) {
+                const bool in = t < room;
                 if (BYTES >= 4) copy_async(dst, in ? src : from, BYTES, in);
                 else *dst = in ? *src : from_float<T>(0.f);
                 t += ROWS;
-                src += down;
+                src += ROWS * step;
                 dst += ROWS * 32 * W;
             }
         }
     }
     template <class T, int W>
-    __device__ __forceinline__ void copy_rows(const ScanArgs& p, int64_t k, T* to, const T* from,
-                                              int64_t step, int at_once) const {
-        if (at_once == 16) copy_pieces<T, W, 16>(p, k, to, from, step);
-        else if (at_once == 4) copy_pieces<T, W, 4>(p, k, to, from, step);
-        else copy_pieces<T, W, (int)sizeof(T)>(p, k, to, from, step);
+    __device__ __forceinline__ void copy_rows(const ScanArgs& p, T* to, const T* from, int64_t step,
+                                              int room, int at_once) const {
+        if (at_once == 16) copy_pieces<T, W, 16>(p, to, from, step, room);
+        else if (at_once == 4) copy_pieces<T, W, 4>(p, to, from, step, room);
+        else copy_pieces<T, W, (int)sizeof(T)>(p, to, from, step, room);
     }
-    __device__ __forceinline__ void copy_values(const ScanArgs& p, int64_t k, VT* to,
-                                                const VT* from, int64_t step, int at_once) const {
-        copy_rows<VT, S::V>(p, k, to, from, step, at_once);
-    }
-    __device__ __forceinline__ void copy_gates(const ScanArgs& p, int64_t k, GT* to) const {
-        const GT* from = static_cast<const GT*>(p.g) + (p.offsets ? row.first * p.gs : b * p.gb);
+    // The same of the gates, of a row from `from` (its first gate of the tile in the first step).
+    __device__ __forceinline__ void copy_gates(const ScanArgs& p, GT* to, const GT* from,
+                                               int64_t step, int room) const {
         if (PC && p.D == 1) {
-            copy_rows<GT, S::V>(p, k, to, from + tile.first, p.gs, p.g_bytes);
+            copy_rows<GT, 2>(p, to, from, step, room, p.g_bytes);
             return;
         }
         // one gate for several channels: once each, or (PC) for every channel of the group
-        const int heads = p.parts > 1 ? 1 : tile.width / p.D;
-        const int width = PC ? tile.width : heads, subs = 32 / p.lanes;
-        const int pitch = PC ? p.lanes * S::V : heads;
-        if (!PC && heads * subs == 1) {
-            const int64_t t = first_step(p, k, 0) + lane;
-            if (lane >= S::L) return;
-            const bool in = t < row.len;
-            const GT* src = from + (in ? place(p, t) : 0) * p.gs + tile.head;
-            if (sizeof(GT) == 4) copy_async(to + lane * 32, src, 4, in);
-            else to[lane * 32] = in ? *src : from_float<GT>(0.f);
+        const int heads = p.parts > 1 ? 1 : tile.width / p.D, subs = 32 / p.lanes;
+        const int width = PC ? tile.width : heads;
+        const int pitch = PC ? p.lanes * 2 : heads;
+        if (!PC && heads == 1) {
+            const int t = wseg * subs * kSteps + lane;      // lane: step of sub lane / kSteps
+            if (lane >= kSteps * subs) return;
+            const bool in = t < room;
+            const GT* src = in ? from + t * step : from;
+            GT* dst = to + (lane % kSteps) * 32 + lane / kSteps;
+            if (sizeof(GT) == 4) copy_async(dst, src, 4, in);
+            else *dst = in ? *src : from_float<GT>(0.f);
             return;
         }
-        for (int i = lane; i < S::L * subs * width; i += 32) {
+        for (int i = lane; i < kSteps * subs * width; i += 32) {
             const int l = i / (subs * width), j = i - l * (subs * width);
             const int s = j / width, c = j - s * width;
-            const int64_t t = first_step(p, k, s) + l;
-            const bool in = t < row.len;
-            const GT* src = from + (in ? place(p, t) : 0) * p.gs +
-                            (PC ? (tile.first + c) / p.D : tile.head + c);
+            const int t = (wseg * subs + s) * kSteps + l;
+            const bool in = t < room;
+            const GT* src = in ? from + t * step + (PC ? (tile.first + c) / p.D - tile.head : c)
+                               : from;
             GT* dst = to + l * 32 * S::GV + s * pitch + c;
             if (sizeof(GT) == 4) copy_async(dst, src, 4, in);
             else *dst = in ? *src : from_float<GT>(0.f);
         }
     }
-    __device__ __forceinline__ void load_gates(const GT* tile_g, int l, float (&g)[S::GV]) const {
-        if (PC) load_some<S::GV>(tile_g + (l * 32 + lane) * S::GV, g);
-        else g[0] = to_float(tile_g[l * 32 + gate]);
+    // What a tile never fills holds zeros: no thickness, no value.
+    __device__ __forceinline__ void clear(const ScanArgs& p, unsigned char* mine, int bytes) const {
+        if (tile.width < p.lanes * 2)
+            for (int i = lane * 16; i < bytes; i += 512)
+                *reinterpret_cast<uint4*>(mine + i) = make_uint4(0, 0, 0, 0);
+        __syncwarp();
     }
-    // state before the row
-    __device__ __forceinline__ void start(const ScanArgs& p, float (&h)[S::V]) const {
-#pragma unroll
-        for (int v = 0; v < S::V; ++v)
-            h[v] = p.h0 != nullptr && v < have
-                       ? __ldg(p.h0 + b * p.hb + ch + v) : 0.f;
-    }
-    // V neighbouring elements of an output row, as far as the tile goes
-    template <class T, int W>
-    __device__ __forceinline__ void put(const ScanArgs& p, T* to, const float (&v)[W]) const {
-        if (W == 1 || p.paired) {
-            store_some<W>(to, v);
+    // a and w of the lane's two channels in step l
+    template <bool WEIGHTED>
+    __device__ __forceinline__ void gates(const GT* g, int l, F2& a, F2& w) const {
+        if (PC) {
+            float v[2];
+            load_some<2>(g + (l * 32 + lane) * 2, v);
+            const F2 t{v[0], v[1]};
+            a = decay2(t);
+            w = WEIGHTED ? two(1.f) : weight2(t, a);
         } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i)
-                if (i < have) to[i] = from_float<T>(v[i]);
+            const float t = to_float(g[l * 32 + gate]);
+            a = two(decay_of(t));
+            w = two(WEIGHTED ? 1.f : weight_of(t, a.x));
         }
     }
+    __device__ __forceinline__ F2 at(const VT* tile_x, int l) const {
+        float v[2];
+        load_some<2>(tile_x + (l * 32 + lane) * 2, v);
+        return {v[0], v[1]};
+    }
+    __device__ __forceinline__ F2 get(const float* from) const {
+        return {have > 0 ? __ldg(from) : 0.f, have > 1 ? __ldg(from + 1) : 0.f};
+    }
+    __device__ __forceinline__ void put(const ScanArgs& p, float* to, F2 v) const {
+        if (have > 0) to[0] = v.x;
+        if (have > 1) to[1] = v.y;
+    }
+    // state before the row
+    __device__ __forceinline__ F2 start(const ScanArgs& p) const {
+        return p.h0 != nullptr ? get(p.h0 + b * p.hb + ch) : two(0.f);
+    }
+    // two neighbouring elements of an output row, as far as the tile goes
     template <class T>
-    __device__ __forceinline__ void get(const T* from, float (&v)[S::V]) const {
-#pragma unroll
-        for (int i = 0; i < S::V; ++i)
-            v[i] = i < have ? (float)from[i] : 0.f;
+    __device__ __forceinline__ void store(const ScanArgs& p, T* to, F2 v) const {
+        if (p.paired) {
+            const float w[2] = {v.x, v.y};
+            store_some<2>(to, w);
+        } else {
+            to[0] = from_float<T>(v.x);
+            if (have > 1) to[1] = from_float<T>(v.y);
+        }
+    }
+    // What the block's other ranges, before this one or (back) behind it, do to `h`.
+    __device__ __forceinline__ F2 ranges(const ScanArgs& p, const float2* pairs, F2 h,
+                                         bool back) const {
+        const int n = back ? p.splits - 1 - split : split;
+        const float2* at = pairs + (b * p.splits + (back ? p.splits - 1 : 0)) * p.C + ch;
+        const int64_t step = back ? -(int64_t)p.C : p.C;
+        if (have == 0) return h;
+        const int second = have - 1;
+#pragma unroll 8
+        for (int s = 0; s < n; ++s) {
+            const float2 q = __ldcg(at + s * step), r = __ldcg(at + s * step + second);
+            h = past2({q.x, r.x}, h, {q.y, r.y});
+        }
+        return h;
     }
     __device__ __forceinline__ void unit_sync(const ScanArgs& p) const {
         if (p.warps == 1) __syncwarp();
@@ -330,22 +419,35 @@ struct ScanThread {
     }
 };
 
-// Pairs of the stretches of a unit's lanes, joined.  In: (A, B) of this lane's L steps.  Out: what
-// the steps before it in the tile do to the state (A, B), and the tile's own pair (TA, TB).  BACK:
-// the steps behind it, from the other end.
-template <int V, bool BACK>
-__device__ __forceinline__ void join_lanes(int lanes, int lane, float (&A)[V], float (&B)[V]) {
+// Joins the pairs of a warp's groups of lanes.  In: (A, B) of this lane's steps.  Out: what the
+// warp's steps before them (BACK: behind them, from the other end) do to the state, and the pair of
+// all.
+template <bool BACK>
+__device__ __forceinline__ void join_lanes(int lanes, int lane, F2& A, F2& B, F2& TA, F2& TB) {
+    if (lanes == 32) {
+        TA = A;
+        TB = B;
+        A = two(1.f);
+        B = two(0.f);
+        return;
+    }
     for (int d = lanes; d < 32; d *= 2) {
-        const bool any = BACK ? lane + d < 32 : lane >= d;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const float a = BACK ? __shfl_down_sync(~0u, A[v], d) : __shfl_up_sync(~0u, A[v], d);
-            const float b = BACK ? __shfl_down_sync(~0u, B[v], d) : __shfl_up_sync(~0u, B[v], d);
-            if (any) {
-                B[v] = past(A[v], b, B[v]);
-                A[v] *= a;
-            }
+        const int from = BACK ? lane + d : lane - d;
+        const F2 a = shfl2(A, from & 31), b = shfl2(B, from & 31);
+        if (from >= 0 && from < 32) {
+            B = past2(A, b, B);
+            A = mul2(A, a);
         }
+    }
+    const int edge = BACK ? lane & (lanes - 1) : 32 - lanes + (lane & (lanes - 1));
+    TA = shfl2(A, edge);
+    TB = shfl2(B, edge);
+    const int by = BACK ? lane + lanes : lane - lanes;
+    A = shfl2(A, by & 31);
+    B = shfl2(B, by & 31);
+    if (by < 0 || by >= 32) {
+        A = two(1.f);
+        B = two(0.f);
     }
 }
 
@@ -357,180 +459,407 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
             VT* __restrict__ states, float* __restrict__ last, float* __restrict__ kept) {
     using Th = ScanThread<VT, GT, PC>;
     using S = typename Th::S;
-    constexpr int V = S::V, L = S::L;
+    constexpr int L = kSteps;
     constexpr bool BACK = MODE == 2;
     extern __shared__ __align__(16) unsigned char s_tiles[];
-    __shared__ float2 s_pair[2][kScanWarps][32 * V];
+    __shared__ float4 s_pair[2][kScanWarps][32];
     Th th;
     if (!th.init(p)) return;
     const int64_t n = th.k1 - th.k0;
+    const int stage = S::kX + S::kG;
+    unsigned char* const mine = s_tiles + (size_t)th.warp * p.stages * stage;
+    th.clear(p, mine, p.stages * stage);
     // (a range backwards has its tiles from the last to the first)
-    auto tile_at = [&](int64_t i) { return BACK ? th.k1 - 1 - i : th.k0 + i; };
-    unsigned char* const mine = s_tiles + (size_t)th.warp * p.stages * (S::kX + S::kG);
-    const VT* const from = x == nullptr ? nullptr
-        : x + (p.offsets ? th.row.first * p.xs : th.b * p.xb) + th.tile.first;
-    auto issue = [&](int64_t i) {
-        if (i < n) {
-            unsigned char* at = mine + (int)(i % p.stages) * (S::kX + S::kG);
-            if (from != nullptr)
-                th.copy_values(p, tile_at(i), reinterpret_cast<VT*>(at), from, p.xs, p.x_bytes);
-            th.copy_gates(p, tile_at(i), reinterpret_cast<GT*>(at + S::kX));
+    const int64_t first = BACK ? th.k1 - 1 : th.k0;
+    const int64_t step_x = p.reverse ? -p.xs : p.xs, step_g = p.reverse ? -p.gs : p.gs;
+    const int64_t at0 = th.place(p, first * th.chunk);
+    const VT* from_x = x == nullptr ? nullptr
+        : x + (p.offsets ? th.row.first * p.xs : th.b * p.xb) + at0 * p.xs + th.tile.first;
+    const GT* from_g = static_cast<const GT*>(p.g) +
+        (p.offsets ? th.row.first * p.gs : th.b * p.gb) + at0 * p.gs + th.tile.head;
+    int64_t issued = 0;
+    int slot_in = 0, slot = 0;
+    auto issue = [&] {
+        if (issued < n) {
+            unsigned char* at = mine + slot_in * stage;
+            const int room = th.room(BACK ? first - issued : first + issued);
+            const int by = BACK ? -th.chunk : th.chunk;
+            if (x != nullptr) {
+                th.template copy_rows<VT, 2>(p, reinterpret_cast<VT*>(at), from_x, step_x, room,
+                                             p.x_bytes);
+                from_x += by * step_x;
+            }
+            th.copy_gates(p, reinterpret_cast<GT*>(at + S::kX), from_g, step_g, room);
+            from_g += by * step_g;
+            slot_in = slot_in + 1 == p.stages ? 0 : slot_in + 1;
         }
+        ++issued;
         copies_issued();
     };
-    float carry[V], through[V];          // MODE 1, 2: the pair so far
-#pragma unroll
-    for (int v = 0; v < V; ++v) { carry[v] = 0.f; through[v] = 1.f; }
-    for (int i = 0; i < p.stages - 1; ++i) issue(i);
-    if (MODE == 0) {
-        th.start(p, carry);
-        if (th.on)
-            for (int s = 0; s < th.split; ++s)
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (v < th.have) {
-                        const float2 q = pairs[(th.b * p.splits + s) * p.C + th.ch + v];
-                        carry[v] = past(q.x, carry[v], q.y);
-                    }
-    }
-    VT* const out = states == nullptr ? nullptr : states + th.row.first * p.C + th.ch;
+    for (int i = 0; i < p.stages - 1; ++i) issue();
+    F2 carry = MODE == 0 ? th.ranges(p, pairs, th.start(p), false) : two(0.f);
+    F2 through = two(1.f);              // MODE 1, 2: with carry, the pair so far
+    VT* out = states == nullptr ? nullptr
+        : states + (th.row.first + th.place(p, first * th.chunk + th.step0)) * p.C + th.ch;
+    float* keep = kept == nullptr || th.wseg != 0 || th.sub != 0 ? nullptr
+        : kept + kept_index(p, th.row, th.b, th.chunk, first) * p.C + th.ch;
     const int64_t out_step = p.reverse ? -(int64_t)p.C : p.C;
     for (int64_t i = 0; i < n; ++i) {
-        const int64_t k = tile_at(i), t0 = th.first_step(p, k, th.sub);
-        issue(i + p.stages - 1);
+        issue();
         copies_wait(p.stages - 1);
         __syncwarp();
-        const unsigned char* at = mine + (int)(i % p.stages) * (S::kX + S::kG);
+        const unsigned char* at = mine + slot * stage;
+        slot = slot + 1 == p.stages ? 0 : slot + 1;
         const VT* const tx = reinterpret_cast<const VT*>(at);
         const GT* const tg = reinterpret_cast<const GT*>(at + S::kX);
-        float a[L][V], u[L][V], A[V], B[V];
+        F2 a[L], u[L], A, B;
         // (a step beyond the row has no thickness and no value: it changes nothing)
-        auto scan = [&](auto safe) {
+        auto scan = [&](auto safe, auto weighted) {
             constexpr bool SAFE = decltype(safe)::value;
-#pragma unroll
-            for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; }
+            A = two(1.f);
+            B = two(0.f);
 #pragma unroll
             for (int j = 0; j < L; ++j) {
                 const int l = BACK ? L - 1 - j : j;
-                float g[S::GV];
-                th.load_gates(tg, l, g);
-#pragma unroll
-                for (int v = 0; v < V; ++v) u[l][v] = 0.f;
-                if (!BACK || from != nullptr) load_some<V>(tx + (l * 32 + th.lane) * V, u[l]);
-                float one_a = 0.f, one_w = 0.f;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    if (v < S::GV) {
-                        one_a = decay_of(g[v < S::GV ? v : 0]);
-                        one_w = p.weighted ? 1.f : weight_of(g[v < S::GV ? v : 0], one_a);
-                    }
-                    a[l][v] = one_a;
-                    if (BACK) {
-                        B[v] = SAFE ? past(one_a, B[v] + u[l][v], 0.f) : one_a * (B[v] + u[l][v]);
-                    } else {
-                        u[l][v] = SAFE ? times(one_w, u[l][v]) : one_w * u[l][v];
-                        B[v] = SAFE ? past(one_a, B[v], u[l][v]) : fmaf(one_a, B[v], u[l][v]);
-                    }
-                    A[v] *= one_a;
+                F2 w;
+                th.template gates<BACK || decltype(weighted)::value>(tg, l, a[l], w);
+                const F2 v = BACK && x == nullptr ? two(0.f) : th.at(tx, l);
+                if (BACK) {
+                    const F2 t = add2(B, v);
+                    B = SAFE ? past2(a[l], t, two(0.f)) : mul2(a[l], t);
+                } else if (SAFE) {
+                    u[l] = {times(w.x, v.x), times(w.y, v.y)};
+                    B = past2(a[l], B, u[l]);
+                } else {
+                    u[l] = decltype(weighted)::value ? v : mul2(w, v);
+                    B = fma2(a[l], B, u[l]);
                 }
+                A = mul2(A, a[l]);
             }
         };
-        scan(std::false_type{});
+        auto scan_safely = [&](auto safe) {
+            if (p.weighted) scan(safe, std::true_type{});
+            else scan(safe, std::false_type{});
+        };
+        scan_safely(std::false_type{});
         // What is not finite stays so to the end of the stretch; then the steps that do not count
         // are told from those that do.
-        bool odd = false;
-#pragma unroll
-        for (int v = 0; v < V; ++v) odd |= v < th.have && !(finite(B[v]) && finite(A[v]));
-        if (odd) scan(std::true_type{});
-        float TA[V], TB[V];     // the lane's place in the warp
-        join_lanes<V, BACK>(p.lanes, th.lane, A, B);
-        const int edge = BACK ? th.cl : 32 - p.lanes + th.cl;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            TA[v] = __shfl_sync(~0u, A[v], edge);
-            TB[v] = __shfl_sync(~0u, B[v], edge);
+        bool odd = spoilt(A, B) != 0.f;
+        if (odd) scan_safely(std::true_type{});
+        if (keep != nullptr) {
+            th.put(p, keep, carry);
+            keep += p.C;
         }
-        if (p.lanes < 32) {     // what lies before the lane
-            const int by = BACK ? th.lane + p.lanes : th.lane - p.lanes;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float pa = __shfl_sync(~0u, A[v], by & 31);
-                const float pb = __shfl_sync(~0u, B[v], by & 31);
-                const bool some = BACK ? by < 32 : by >= 0;
-                A[v] = some ? pa : 1.f;
-                B[v] = some ? pb : 0.f;
-            }
-        } else {
-#pragma unroll
-            for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; }
-        }
-        if (kept != nullptr && th.wseg == 0 && th.sub == 0 && th.on) {
-            float* to = kept + kept_index(p, th.row, th.b, th.chunk, k) * p.C + th.ch;
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (v < th.have) to[v] = carry[v];
-        }
-        float h[V];
+        F2 TA, TB;
+        join_lanes<BACK>(p.lanes, th.lane, A, B, TA, TB);
+        F2 h = carry;
         if (p.warps == 1) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                h[v] = past(A[v], carry[v], B[v]);
-                carry[v] = past(TA[v], carry[v], TB[v]);
-                through[v] *= TA[v];
-            }
+            carry = past2(TA, carry, TB);
+            if (MODE != 0) through = mul2(through, TA);
         } else {
             auto& pair = s_pair[i & 1];
-            if (th.sub == 0)
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    pair[th.warp][th.cl * V + v] = make_float2(TA[v], TB[v]);
+            if (th.sub == 0) pair[th.warp][th.cl] = make_float4(TA.x, TA.y, TB.x, TB.y);
             th.unit_sync(p);
+            const F2 before = carry;
+            const float4* const all = &pair[th.group * p.warps][th.cl];
+#pragma unroll 8
             for (int j = 0; j < p.warps; ++j) {
                 const int w = BACK ? p.warps - 1 - j : j;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    if (w == th.wseg) h[v] = past(A[v], carry[v], B[v]);
-                    const float2 q = pair[th.group * p.warps + w][th.cl * V + v];
-                    carry[v] = past(q.x, carry[v], q.y);
-                    if (MODE != 0) through[v] *= q.x;
+                if (w == th.wseg) h = carry;
+                const float4 q = all[w * 32];
+                carry = fma2({q.x, q.y}, carry, {q.z, q.w});
+                if (MODE != 0) through = mul2(through, {q.x, q.y});
+            }
+            if (spoilt(carry, carry) != 0.f) {
+                carry = before;
+                for (int j = 0; j < p.warps; ++j) {
+                    const int w = BACK ? p.warps - 1 - j : j;
+                    if (w == th.wseg) h = carry;
+                    const float4 q = all[w * 32];
+                    carry = past2({q.x, q.y}, carry, {q.z, q.w});
                 }
             }
         }
-        if (MODE == 0 && out != nullptr && th.on) {
-            VT* to = out + th.place(p, t0) * p.C;
-#pragma unroll
-            for (int v = 0; v < V; ++v) odd |= v < th.have && !finite(h[v]);
-            if (t0 + L <= th.row.len && !odd) {
+        if (MODE == 0 && out != nullptr) {
+            if (p.lanes < 32) h = past2(A, h, B);
+            odd |= spoilt(h, h) != 0.f;
+            const int64_t t0 = (first + i) * th.chunk + th.step0;
+            VT* to = out;
+            out += th.chunk * out_step;
+            if (th.have && t0 + L <= th.row.len && !odd) {
 #pragma unroll
                 for (int l = 0; l < L; ++l, to += out_step) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) h[v] = fmaf(a[l][v], h[v], u[l][v]);
-                    th.put(p, to, h);
+                    h = fma2(a[l], h, u[l]);
+                    th.store(p, to, h);
                 }
-            } else {
+            } else if (th.have) {
 #pragma unroll
                 for (int l = 0; l < L; ++l, to += out_step) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) h[v] = past(a[l][v], h[v], u[l][v]);
-                    if (t0 + l < th.row.len) th.put(p, to, h);
+                    h = past2(a[l], h, u[l]);
+                    if (t0 + l < th.row.len) th.store(p, to, h);
                 }
             }
         }
         __syncwarp();
     }
-    if (th.wseg == 0 && th.sub == 0 && th.on)
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            if (v >= th.have) continue;
-            if (MODE != 0)
-                pairs[(th.b * p.splits + th.split) * p.C + th.ch + v] =
-                    make_float2(through[v], carry[v]);
-            else if (th.split == p.splits - 1)
-                last[th.b * p.C + th.ch + v] = carry[v];
+    if (th.wseg == 0 && th.sub == 0) {
+        if (MODE != 0) {
+            float2* to = pairs + (th.b * p.splits + th.split) * p.C + th.ch;
+            if (th.have > 0) to[0] = make_float2(through.x, carry.x);
+            if (th.have > 1) to[1] = make_float2(through.y, carry.y);
+        } else if (th.split == p.splits - 1) {
+            th.put(p, last + th.b * p.C + th.ch, carry);
         }
+    }
     if (MODE == 0 && th.split == 0)
         clear_uncovered(p, th.b, th.tile.first, th.tile.width, (int64_t)p.C, states,
                         th.wseg * 32 + th.lane, p.warps * 32);
+}
+
+// The backward pass of a tile.  `parted`: (parts, steps, H) floats for the sums of a group that
+// several tiles share.
+template <class VT, class GT, bool PC>
+__global__ void __launch_bounds__(kScanBlock, 2)
+scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict__ pairs,
+                 const float* __restrict__ kept, const VT* __restrict__ d,
+                 const float* __restrict__ d_last, VT* __restrict__ dx, GT* __restrict__ dg,
+                 float* __restrict__ parted, float* __restrict__ dh0) {
+    using Th = ScanThread<VT, GT, PC>;
+    using S = typename Th::S;
+    constexpr int L = kSteps;
+    extern __shared__ __align__(16) unsigned char s_tiles[];
+    __shared__ float4 s_pair[2][kScanWarps][32];
+    __shared__ float2 s_flow[2][kScanWarps][32];
+    Th th;
+    if (!th.init(p)) return;
+    const int64_t n = th.k1 - th.k0;
+    const int stage = 2 * S::kX + S::kG;
+    unsigned char* const mine = s_tiles + (size_t)th.warp * p.stages * stage;
+    float* const sums = reinterpret_cast<float*>(s_tiles + (size_t)kScanWarps * p.stages * stage +
+                                                 th.warp * S::kSum);
+    th.clear(p, mine, p.stages * stage);
+    const int64_t first = th.k1 - 1;
+    const int64_t step_x = p.reverse ? -p.xs : p.xs, step_g = p.reverse ? -p.gs : p.gs;
+    const int64_t step_c = p.reverse ? -(int64_t)p.C : p.C, step_h = p.reverse ? -(int64_t)p.H : p.H;
+    const int64_t at0 = th.place(p, first * th.chunk);
+    const VT* from_x = x + (p.offsets ? th.row.first * p.xs : th.b * p.xb) + at0 * p.xs +
+                       th.tile.first;
+    const GT* from_g = static_cast<const GT*>(p.g) +
+        (p.offsets ? th.row.first * p.gs : th.b * p.gb) + at0 * p.gs + th.tile.head;
+    const VT* from_d = d == nullptr ? nullptr : d + (th.row.first + at0) * p.C + th.tile.first;
+    int64_t issued = 0;
+    int slot_in = 0, slot = 0;
+    auto issue = [&] {
+        if (issued < n) {
+            unsigned char* at = mine + slot_in * stage;
+            const int room = th.room(first - issued);
+            th.template copy_rows<VT, 2>(p, reinterpret_cast<VT*>(at), from_x, step_x, room,
+                                         p.x_bytes);
+            from_x -= th.chunk * step_x;
+            if (d != nullptr) {
+                th.template copy_rows<VT, 2>(p, reinterpret_cast<VT*>(at + S::kX), from_d, step_c,
+                                             room, p.d_bytes);
+                from_d -= th.chunk * step_c;
+            }
+            th.copy_gates(p, reinterpret_cast<GT*>(at + 2 * S::kX), from_g, step_g, room);
+            from_g -= th.chunk * step_g;
+            slot_in = slot_in + 1 == p.stages ? 0 : slot_in + 1;
+        }
+        ++issued;
+        copies_issued();
+    };
+    for (int i = 0; i < p.stages - 1; ++i) issue();
+    const float* keep = kept + kept_index(p, th.row, th.b, th.chunk, first) * p.C + th.ch;
+    F2 h_next = n > 0 ? th.get(keep) : two(0.f);
+    F2 R = d_last != nullptr ? th.get(d_last + th.b * p.C + th.ch) : two(0.f);
+    R = th.ranges(p, pairs, R, true);   // what flows back into the last state of the tile
+    // (outputs are written from a stretch's last step to its first)
+    const int64_t out0 = th.row.first + th.place(p, first * th.chunk + th.step0 + L - 1);
+    VT* to_x = dx == nullptr ? nullptr : dx + out0 * p.C + th.ch;
+    GT* to_g = dg == nullptr || p.D > 1 ? nullptr : dg + out0 * p.H + th.ch;
+    for (int64_t i = 0; i < n; ++i) {
+        const int64_t k = first - i;
+        issue();
+        copies_wait(p.stages - 1);
+        __syncwarp();
+        const unsigned char* at = mine + slot * stage;
+        slot = slot + 1 == p.stages ? 0 : slot + 1;
+        const VT* const tx = reinterpret_cast<const VT*>(at);
+        const VT* const td = reinterpret_cast<const VT*>(at + S::kX);
+        const GT* const tg = reinterpret_cast<const GT*>(at + 2 * S::kX);
+        F2 h = h_next;
+        keep -= p.C;
+        if (i + 1 < n) h_next = th.get(keep);
+        F2 a[L], w[L], A, B, E;
+        auto scan = [&](auto safe, auto weighted) {
+            constexpr bool SAFE = decltype(safe)::value;
+            A = two(1.f);
+            B = E = two(0.f);
+#pragma unroll
+            for (int l = 0; l < L; ++l) {
+                th.template gates<decltype(weighted)::value>(tg, l, a[l], w[l]);
+                const F2 v = th.at(tx, l);
+                if (SAFE) B = past2(a[l], B, {times(w[l].x, v.x), times(w[l].y, v.y)});
+                else B = fma2(a[l], B, decltype(weighted)::value ? v : mul2(w[l], v));
+                A = mul2(A, a[l]);
+            }
+            if (d == nullptr) return;
+#pragma unroll
+            for (int l = L - 1; l >= 0; --l) {
+                const F2 t = add2(E, th.at(td, l));
+                E = SAFE ? past2(a[l], t, two(0.f)) : mul2(a[l], t);
+            }
+        };
+        auto scan_safely = [&](auto safe) {
+            if (p.weighted) scan(safe, std::true_type{});
+            else scan(safe, std::false_type{});
+        };
+        scan_safely(std::false_type{});
+        bool odd = spoilt(A, B) != 0.f || spoilt(E, E) != 0.f;
+        if (odd) scan_safely(std::true_type{});
+        F2 EA = A, TA, TB, TE, all_a;
+        join_lanes<false>(p.lanes, th.lane, A, B, TA, TB);
+        join_lanes<true>(p.lanes, th.lane, EA, E, all_a, TE);
+        F2 G = R;
+        if (p.warps == 1) {
+            R = past2(TA, R, TE);
+        } else {
+            if (th.sub == 0) {
+                s_pair[i & 1][th.warp][th.cl] = make_float4(TA.x, TA.y, TB.x, TB.y);
+                s_flow[i & 1][th.warp][th.cl] = make_float2(TE.x, TE.y);
+            }
+            th.unit_sync(p);
+            const float4* const all = &s_pair[i & 1][th.group * p.warps][th.cl];
+            const float2* const flow = &s_flow[i & 1][th.group * p.warps][th.cl];
+            const F2 h_before = h, R_before = R;
+#pragma unroll 8
+            for (int j = 0; j < p.warps; ++j) {
+                if (j >= th.wseg) break;
+                const float4 q = all[j * 32];
+                h = fma2({q.x, q.y}, h, {q.z, q.w});
+            }
+#pragma unroll 8
+            for (int j = p.warps - 1; j >= 0; --j) {
+                if (j == th.wseg) G = R;
+                const float2 a2 = *reinterpret_cast<const float2*>(&all[j * 32]), e2 = flow[j * 32];
+                R = fma2({a2.x, a2.y}, R, {e2.x, e2.y});
+            }
+            if (spoilt(h, R) != 0.f) {
+                h = h_before;
+                R = R_before;
+                for (int j = 0; j < th.wseg; ++j) {
+                    const float4 q = all[j * 32];
+                    h = past2({q.x, q.y}, h, {q.z, q.w});
+                }
+                for (int j = p.warps - 1; j >= 0; --j) {
+                    if (j == th.wseg) G = R;
+                    const float4 q = all[j * 32];
+                    const float2 e2 = flow[j * 32];
+                    R = past2({q.x, q.y}, R, {e2.x, e2.y});
+                }
+            }
+        }
+        if (p.lanes < 32) {
+            h = past2(A, h, B);
+            G = past2(EA, G, E);
+        }
+        odd |= spoilt(h, G) != 0.f;
+        const int64_t t0 = k * th.chunk + th.step0;
+        const bool whole = t0 + L <= th.row.len;
+        auto unwind = [&](auto safe, auto weighted) {
+            constexpr bool SAFE = decltype(safe)::value, WEIGHTED = decltype(weighted)::value;
+            // forwards: what dg has besides the adjoint
+            F2 q[L];
+#pragma unroll
+            for (int l = 0; l < L; ++l) {
+                F2 v = th.at(tx, l);
+                if (SAFE) {
+                    const F2 u{times(w[l].x, v.x), times(w[l].y, v.y)};
+                    // (a value that is not finite in a place of no thickness is no sample)
+                    if (w[l].x == 0.f && !finite(v.x)) v.x = h.x;
+                    if (w[l].y == 0.f && !finite(v.y)) v.y = h.y;
+                    q[l].x = a[l].x == 0.f ? 0.f : a[l].x * (WEIGHTED ? -h.x : v.x - h.x);
+                    q[l].y = a[l].y == 0.f ? 0.f : a[l].y * (WEIGHTED ? -h.y : v.y - h.y);
+                    h = past2(a[l], h, u);
+                } else {
+                    q[l] = mul2(a[l], fma2(h, two(-1.f), WEIGHTED ? two(0.f) : v));
+                    h = fma2(a[l], h, WEIGHTED ? v : mul2(w[l], v));
+                }
+            }
+            // and back
+#pragma unroll
+            for (int l = L - 1; l >= 0; --l) {
+                const bool in = th.have && (whole || t0 + l < th.row.len);
+                if (d != nullptr) G = add2(G, th.at(td, l));
+                if (dx != nullptr && in)
+                    th.store(p, to_x - (L - 1 - l) * step_c, WEIGHTED ? G : mul2(w[l], G));
+                if (dg != nullptr) {
+                    const F2 one = mul2(q[l], G);
+                    if (to_g != nullptr) {
+                        if (in) th.store(p, to_g - (L - 1 - l) * step_h, one);
+                    } else if (PC) {
+                        sums[l * S::kPitch + th.lane * 2] = one.x;
+                        sums[l * S::kPitch + th.lane * 2 + 1] = one.y;
+                    } else {
+                        sums[l * S::kPitch + th.lane] = one.x + one.y;
+                    }
+                }
+                G = SAFE ? past2(a[l], G, two(0.f)) : mul2(a[l], G);
+            }
+        };
+        if (p.weighted) {
+            if (odd) unwind(std::true_type{}, std::true_type{});
+            else unwind(std::false_type{}, std::true_type{});
+        } else {
+            if (odd) unwind(std::true_type{}, std::false_type{});
+            else unwind(std::false_type{}, std::false_type{});
+        }
+        if (to_x != nullptr) to_x -= th.chunk * step_c;
+        if (to_g != nullptr) to_g -= th.chunk * step_h;
+        if (p.D > 1 && dg != nullptr) {
+            __syncwarp();
+            const int heads = p.parts > 1 ? 1 : th.tile.width / p.D, subs = 32 / p.lanes;
+            const int tasks = L * subs * heads;
+            // a sum's terms: channels (PC), or pairs of them
+            const int width = (p.parts > 1 ? th.tile.width : p.D) / (PC ? 1 : 2);
+            const int row_of = PC ? p.lanes * 2 : p.lanes;
+            // few sums: several lanes to each
+            const int share = tasks < 32 && (tasks & (tasks - 1)) == 0 ? 32 / tasks : 1;
+            for (int j0 = 0; j0 < tasks; j0 += 32 / share) {
+                const int j = j0 + th.lane / share;
+                const int l = j / (subs * heads), r = j - l * (subs * heads);
+                const int s = r / heads, hd = r - s * heads;
+                float sum = 0.f;
+                if (j < tasks) {
+                    const float* from = sums + l * S::kPitch + s * row_of + hd * width;
+                    for (int c = th.lane % share; c < width; c += share) sum += from[c];
+                }
+                for (int o = 1; o < share; o *= 2) sum += __shfl_xor_sync(~0u, sum, o);
+                const int64_t t = k * th.chunk + (th.wseg * subs + s) * L + l;
+                if (j >= tasks || t >= th.row.len || th.lane % share != 0) continue;
+                const int64_t where = th.row.first + th.place(p, t);
+                if (p.parts > 1) {
+                    const int part = (th.tile.first - th.tile.head * p.D) / p.tile;
+                    const int64_t steps = p.offsets ? p.T : p.B * p.T;
+                    parted[(part * steps + where) * p.H + th.tile.head] = sum;
+                } else {
+                    dg[where * p.H + th.tile.head + hd] = from_float<GT>(sum);
+                }
+            }
+        }
+        __syncwarp();
+    }
+    if (th.split == 0) {
+        if (th.wseg == 0 && th.sub == 0 && dh0 != nullptr)
+            th.put(p, dh0 + th.b * p.C + th.ch, R);
+        const int thread = th.wseg * 32 + th.lane, threads = p.warps * 32;
+        clear_uncovered(p, th.b, th.tile.first, th.tile.width, (int64_t)p.C, dx, thread, threads);
+        const bool own_head = p.parts == 1 || th.tile.first == th.tile.head * p.D;
+        if (own_head)
+            clear_uncovered(p, th.b, p.D == 1 ? th.tile.first : th.tile.head,
+                            p.D == 1 ? th.tile.width : p.parts > 1 ? 1 : th.tile.width / p.D,
+                            (int64_t)p.H, dg, thread, threads);
+    }
 }
 
 // Rows of a few steps (a sequence that goes on one step at a time): a thread for every W channels,
@@ -581,266 +910,6 @@ static __global__ void scan_last_kernel(ScanArgs p, const float2* __restrict__ p
         h = past(q.x, h, q.y);
     }
     last[i] = h;
-}
-
-// The backward pass of a tile.  `parted`: (parts, steps, H) floats for the sums of a group that
-// several tiles share.
-template <class VT, class GT, bool PC>
-__global__ void __launch_bounds__(kScanBlock, 2)
-scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict__ pairs,
-                 const float* __restrict__ kept, const VT* __restrict__ d,
-                 const float* __restrict__ d_last, VT* __restrict__ dx, GT* __restrict__ dg,
-                 float* __restrict__ parted, float* __restrict__ dh0) {
-    using Th = ScanThread<VT, GT, PC>;
-    using S = typename Th::S;
-    constexpr int V = S::V, L = S::L;
-    extern __shared__ __align__(16) unsigned char s_tiles[];
-    __shared__ float s_pair[2][kScanWarps][3][32 * V];
-    Th th;
-    if (!th.init(p)) return;
-    const int64_t n = th.k1 - th.k0;
-    const int stage = 2 * S::kX + S::kG;
-    unsigned char* const mine = s_tiles + (size_t)th.warp * p.stages * stage;
-    float* const sums = reinterpret_cast<float*>(s_tiles + (size_t)kScanWarps * p.stages * stage +
-                                                 th.warp * S::kSum);
-    const VT* const from_x = x + (p.offsets ? th.row.first * p.xs : th.b * p.xb) + th.tile.first;
-    const VT* const from_d = d == nullptr ? nullptr : d + th.row.first * p.C + th.tile.first;
-    float h_next[V];
-    auto issue = [&](int64_t i) {
-        if (i < n) {
-            const int64_t k = th.k1 - 1 - i;
-            unsigned char* at = mine + (int)(i % p.stages) * stage;
-            th.copy_values(p, k, reinterpret_cast<VT*>(at), from_x, p.xs, p.x_bytes);
-            if (from_d != nullptr)
-                th.copy_values(p, k, reinterpret_cast<VT*>(at + S::kX), from_d, p.C, p.d_bytes);
-            th.copy_gates(p, k, reinterpret_cast<GT*>(at + 2 * S::kX));
-        }
-        copies_issued();
-    };
-    auto kept_at = [&](int64_t i, float (&to)[V]) {
-        if (i < n)
-            th.get(kept + kept_index(p, th.row, th.b, th.chunk, th.k1 - 1 - i) * p.C + th.ch, to);
-    };
-    for (int i = 0; i < p.stages - 1; ++i) issue(i);
-    kept_at(0, h_next);
-    float R[V];         // what flows back into the last state of the tile
-#pragma unroll
-    for (int v = 0; v < V; ++v) R[v] = 0.f;
-    if (d_last != nullptr) th.get(d_last + th.b * p.C + th.ch, R);
-    if (th.on)
-        for (int s = p.splits - 1; s > th.split; --s)
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (v < th.have) {
-                    const float2 q = pairs[(th.b * p.splits + s) * p.C + th.ch + v];
-                    R[v] = past(q.x, R[v], q.y);
-                }
-    const int64_t dx_step = p.reverse ? -(int64_t)p.C : p.C;
-    const int64_t dg_step = p.reverse ? -(int64_t)p.H : p.H;
-    for (int64_t i = 0; i < n; ++i) {
-        const int64_t k = th.k1 - 1 - i, t0 = th.first_step(p, k, th.sub);
-        issue(i + p.stages - 1);
-        copies_wait(p.stages - 1);
-        __syncwarp();
-        const unsigned char* at = mine + (int)(i % p.stages) * stage;
-        const VT* const tx = reinterpret_cast<const VT*>(at) + th.lane * V;
-        const VT* const td = reinterpret_cast<const VT*>(at + S::kX) + th.lane * V;
-        const GT* const tg = reinterpret_cast<const GT*>(at + 2 * S::kX);
-        float h[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = h_next[v];
-        kept_at(i + 1, h_next);
-        float a[L][V], w[L][V], A[V], B[V], EA[V], E[V];
-        auto scan = [&](auto safe) {
-            constexpr bool SAFE = decltype(safe)::value;
-#pragma unroll
-            for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; E[v] = 0.f; }
-#pragma unroll
-            for (int l = 0; l < L; ++l) {
-                float g[S::GV], xv[V], one_a = 0.f, one_w = 0.f;
-                th.load_gates(tg, l, g);
-                load_some<V>(tx + l * 32 * V, xv);
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    if (v < S::GV) {
-                        one_a = decay_of(g[v < S::GV ? v : 0]);
-                        one_w = p.weighted ? 1.f : weight_of(g[v < S::GV ? v : 0], one_a);
-                    }
-                    a[l][v] = one_a;
-                    w[l][v] = one_w;
-                    A[v] *= one_a;
-                    B[v] = SAFE ? past(one_a, B[v], times(one_w, xv[v]))
-                                : fmaf(one_a, B[v], one_w * xv[v]);
-                }
-            }
-            if (from_d != nullptr) {
-#pragma unroll
-                for (int l = L - 1; l >= 0; --l) {
-                    float e[V];
-                    load_some<V>(td + l * 32 * V, e);
-#pragma unroll
-                    for (int v = 0; v < V; ++v)
-                        E[v] = SAFE ? past(a[l][v], E[v] + e[v], 0.f) : a[l][v] * (E[v] + e[v]);
-                }
-            }
-        };
-        scan(std::false_type{});
-        bool odd = false;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            odd |= v < th.have && !(finite(A[v]) && finite(B[v]) && finite(E[v]));
-        if (odd) scan(std::true_type{});
-#pragma unroll
-        for (int v = 0; v < V; ++v) EA[v] = A[v];
-        float TA[V], TB[V], TE[V];
-        join_lanes<V, false>(p.lanes, th.lane, A, B);
-        join_lanes<V, true>(p.lanes, th.lane, EA, E);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            TA[v] = __shfl_sync(~0u, EA[v], th.cl);
-            TB[v] = __shfl_sync(~0u, B[v], 32 - p.lanes + th.cl);
-            TE[v] = __shfl_sync(~0u, E[v], th.cl);
-        }
-        if (p.lanes < 32) {
-            const int lo = th.lane - p.lanes, hi = th.lane + p.lanes;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float pa = __shfl_sync(~0u, A[v], lo & 31), pb = __shfl_sync(~0u, B[v], lo & 31);
-                const float na = __shfl_sync(~0u, EA[v], hi & 31), ne = __shfl_sync(~0u, E[v], hi & 31);
-                A[v] = lo >= 0 ? pa : 1.f;
-                B[v] = lo >= 0 ? pb : 0.f;
-                EA[v] = hi < 32 ? na : 1.f;
-                E[v] = hi < 32 ? ne : 0.f;
-            }
-        } else {
-#pragma unroll
-            for (int v = 0; v < V; ++v) { A[v] = EA[v] = 1.f; B[v] = E[v] = 0.f; }
-        }
-        float G[V];
-        if (p.warps == 1) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                h[v] = past(A[v], h[v], B[v]);
-                G[v] = past(EA[v], R[v], E[v]);
-                R[v] = past(TA[v], R[v], TE[v]);
-            }
-        } else {
-            auto& pair = s_pair[i & 1];
-            if (th.sub == 0)
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    pair[th.warp][0][th.cl * V + v] = TA[v];
-                    pair[th.warp][1][th.cl * V + v] = TB[v];
-                    pair[th.warp][2][th.cl * V + v] = TE[v];
-                }
-            th.unit_sync(p);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const int c = th.cl * V + v;
-                for (int j = 0; j < th.wseg; ++j) {
-                    const auto& q = pair[th.group * p.warps + j];
-                    h[v] = past(q[0][c], h[v], q[1][c]);
-                }
-                h[v] = past(A[v], h[v], B[v]);
-                for (int j = p.warps - 1; j >= 0; --j) {
-                    if (j == th.wseg) G[v] = past(EA[v], R[v], E[v]);
-                    const auto& q = pair[th.group * p.warps + j];
-                    R[v] = past(q[0][c], R[v], q[2][c]);
-                }
-            }
-        }
-        const bool whole = t0 + L <= th.row.len;
-        VT* to_x = dx == nullptr ? nullptr
-                                 : dx + (th.row.first + th.place(p, t0 + L - 1)) * p.C + th.ch;
-        GT* to_g = dg == nullptr || p.D > 1
-                       ? nullptr : dg + (th.row.first + th.place(p, t0 + L - 1)) * p.H + th.ch;
-        auto unwind = [&](auto safe) {
-            constexpr bool SAFE = decltype(safe)::value;
-            // forwards: what dg has besides the adjoint
-            float q[L][V];
-#pragma unroll
-            for (int l = 0; l < L; ++l) {
-                float xv[V];
-                load_some<V>(tx + l * 32 * V, xv);
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const float wv = w[l][v], av = a[l][v];
-                    if (SAFE) {
-                        // (a value that is not finite in a place of no thickness is no sample)
-                        const float xs = wv == 0.f && !finite(xv[v]) ? h[v] : xv[v];
-                        q[l][v] = av == 0.f ? 0.f : av * (p.weighted ? -h[v] : xs - h[v]);
-                        h[v] = past(av, h[v], times(wv, xv[v]));
-                    } else {
-                        q[l][v] = av * (p.weighted ? -h[v] : xv[v] - h[v]);
-                        h[v] = fmaf(av, h[v], wv * xv[v]);
-                    }
-                }
-            }
-            // and back
-#pragma unroll
-            for (int l = L - 1; l >= 0; --l) {
-                const bool in = th.on && (whole || t0 + l < th.row.len);
-                float e[V], dxv[V], dgv[V];
-#pragma unroll
-                for (int v = 0; v < V; ++v) e[v] = 0.f;
-                if (from_d != nullptr) load_some<V>(td + l * 32 * V, e);
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    G[v] += e[v];
-                    dxv[v] = w[l][v] * G[v];
-                    dgv[v] = q[l][v] * G[v];
-                    G[v] = SAFE ? past(a[l][v], G[v], 0.f) : a[l][v] * G[v];
-                }
-                if (in && dx != nullptr) th.put(p, to_x - (L - 1 - l) * dx_step, dxv);
-                if (to_g != nullptr) {
-                    if (in) th.put(p, to_g - (L - 1 - l) * dg_step, dgv);
-                } else if (p.D > 1 && dg != nullptr) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) sums[l * (32 * V + 1) + th.lane * V + v] = dgv[v];
-                }
-            }
-        };
-#pragma unroll
-        for (int v = 0; v < V; ++v) odd |= v < th.have && !(finite(h[v]) && finite(G[v]));
-        if (odd) unwind(std::true_type{});
-        else unwind(std::false_type{});
-        if (p.D > 1 && dg != nullptr) {
-            __syncwarp();
-            const int heads = p.parts > 1 ? 1 : th.tile.width / p.D, subs = 32 / p.lanes;
-            const int width = p.parts > 1 ? th.tile.width : p.D;
-            for (int j = th.lane; j < L * subs * heads; j += 32) {
-                const int l = j / (subs * heads), r = j - l * (subs * heads);
-                const int s = r / heads, hd = r - s * heads;
-                const float* from = sums + l * (32 * V + 1) + s * p.lanes * V + hd * p.D;
-                float sum = 0.f;
-                for (int c = 0; c < width; ++c) sum += from[c];
-                const int64_t t = th.first_step(p, k, s) + l;
-                if (t >= th.row.len) continue;
-                const int64_t where = th.row.first + th.place(p, t);
-                if (p.parts > 1) {
-                    const int part = (th.tile.first - th.tile.head * p.D) / p.tile;
-                    const int64_t steps = p.offsets ? p.T : p.B * p.T;
-                    parted[(part * steps + where) * p.H + th.tile.head] = sum;
-                } else {
-                    dg[where * p.H + th.tile.head + hd] = from_float<GT>(sum);
-                }
-            }
-        }
-        __syncwarp();
-    }
-    if (th.split == 0) {
-        if (th.wseg == 0 && th.sub == 0 && th.on && dh0 != nullptr)
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (v < th.have) dh0[th.b * p.C + th.ch + v] = R[v];
-        const int thread = th.wseg * 32 + th.lane, threads = p.warps * 32;
-        clear_uncovered(p, th.b, th.tile.first, th.tile.width, (int64_t)p.C, dx, thread, threads);
-        const bool own_head = p.parts == 1 || th.tile.first == th.tile.head * p.D;
-        if (own_head)
-            clear_uncovered(p, th.b, p.D == 1 ? th.tile.first : th.tile.head,
-                            p.D == 1 ? th.tile.width : p.parts > 1 ? 1 : th.tile.width / p.D,
-                            (int64_t)p.H, dg, thread, threads);
-    }
 }
 
 // dg from the sums of the parts of each group.
