@@ -316,6 +316,35 @@ struct ScanThread {
         else if (at_once == 4) copy_pieces<T, W, 4>(p, to, from, step, room);
         else copy_pieces<T, W, (int)sizeof(T)>(p, to, from, step, room);
     }
+    // The same 16 bytes at a time with what a lane needs for it at hand.
+    template <class T>
+    struct Pieces {
+        static constexpr int n = 16 / (int)sizeof(T), COLS = 64 / n, ROWS = 32 / COLS;
+        int64_t off, down;      // its first piece, from there to the next
+        int t;                  // the step of its first piece; none: none
+        unsigned dst;
+        __device__ __forceinline__ void init(const ScanArgs& p, const ScanThread& th, int64_t step) {
+            const int each = p.lanes * 2, j = th.lane % COLS * n;
+            const int s = j >> (31 - __clz(each)), c = j & (each - 1);
+            const int t0 = (th.wseg * (32 / p.lanes) + s) * kSteps + th.lane / COLS;
+            off = t0 * step + c;
+            down = ROWS * step;
+            t = c < th.tile.width ? t0 : 1 << 30;
+            dst = (unsigned)((th.lane / COLS * 64 + j) * sizeof(T));
+        }
+        __device__ __forceinline__ void copy(unsigned tile, const T* from, int room) const {
+            if (t >= 1 << 30) return;
+            const T* src = from + off;
+#pragma unroll
+            for (int l = 0; l < kSteps; l += ROWS, src += down) {
+                const bool in = t + l < room;
+                const int bytes = in ? 16 : 0;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::
+                             "r"(tile + dst + (unsigned)(l * 64 * sizeof(T))), "l"(in ? src : from),
+                             "r"(bytes) : "memory");
+            }
+        }
+    };
     // The same of the gates, of a row from `from` (its first gate of the tile in the first step).
     __device__ __forceinline__ void copy_gates(const ScanArgs& p, GT* to, const GT* from,
                                                int64_t step, int room) const {
@@ -375,6 +404,14 @@ struct ScanThread {
         float v[2];
         load_some<2>(tile_x + (l * 32 + lane) * 2, v);
         return {v[0], v[1]};
+    }
+    // a and what step l adds (raw: its value as it is), for the careful loops
+    __device__ __forceinline__ void step(const ScanArgs& p, const VT* x, const GT* g, int l, F2& a,
+                                         F2& u, bool raw) const {
+        F2 w;
+        gates<false>(g, l, a, w);
+        u = x == nullptr ? two(0.f) : at(x, l);
+        if (!p.weighted && !raw) u = {times(w.x, u.x), times(w.y, u.y)};
     }
     __device__ __forceinline__ F2 get(const float* from) const {
         return {have > 0 ? __ldg(from) : 0.f, have > 1 ? __ldg(from + 1) : 0.f};
@@ -465,7 +502,7 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
     __shared__ float4 s_pair[2][kScanWarps][32];
     Th th;
     if (!th.init(p)) return;
-    const int64_t n = th.k1 - th.k0;
+    const int n = (int)(th.k1 - th.k0);
     const int stage = S::kX + S::kG;
     unsigned char* const mine = s_tiles + (size_t)th.warp * p.stages * stage;
     th.clear(p, mine, p.stages * stage);
@@ -473,25 +510,31 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
     const int64_t first = BACK ? th.k1 - 1 : th.k0;
     const int64_t step_x = p.reverse ? -p.xs : p.xs, step_g = p.reverse ? -p.gs : p.gs;
     const int64_t at0 = th.place(p, first * th.chunk);
-    const VT* from_x = x == nullptr ? nullptr
-        : x + (p.offsets ? th.row.first * p.xs : th.b * p.xb) + at0 * p.xs + th.tile.first;
+    const VT* from_x = x + (p.offsets ? th.row.first * p.xs : th.b * p.xb) + at0 * p.xs +
+                       th.tile.first;
     const GT* from_g = static_cast<const GT*>(p.g) +
         (p.offsets ? th.row.first * p.gs : th.b * p.gb) + at0 * p.gs + th.tile.head;
-    int64_t issued = 0;
-    int slot_in = 0, slot = 0;
+    typename Th::template Pieces<VT> px;
+    typename Th::template Pieces<GT> pg;
+    px.init(p, th, step_x);
+    pg.init(p, th, step_g);
+    const bool whole_x = p.x_bytes == 16, whole_g = PC && p.D == 1 && p.g_bytes == 16;
+    const unsigned shared = (unsigned)__cvta_generic_to_shared(mine);
+    const int64_t next_x = (BACK ? -th.chunk : th.chunk) * step_x;
+    const int64_t next_g = (BACK ? -th.chunk : th.chunk) * step_g;
+    int issued = 0, slot_in = 0, slot = 0;      // (offsets of the tiles' places)
     auto issue = [&] {
         if (issued < n) {
-            unsigned char* at = mine + slot_in * stage;
             const int room = th.room(BACK ? first - issued : first + issued);
-            const int by = BACK ? -th.chunk : th.chunk;
-            if (x != nullptr) {
-                th.template copy_rows<VT, 2>(p, reinterpret_cast<VT*>(at), from_x, step_x, room,
-                                             p.x_bytes);
-                from_x += by * step_x;
-            }
-            th.copy_gates(p, reinterpret_cast<GT*>(at + S::kX), from_g, step_g, room);
-            from_g += by * step_g;
-            slot_in = slot_in + 1 == p.stages ? 0 : slot_in + 1;
+            if (whole_x) px.copy(shared + slot_in, from_x, room);
+            else if (!BACK || x != nullptr)
+                th.template copy_rows<VT, 2>(p, reinterpret_cast<VT*>(mine + slot_in), from_x, step_x,
+                                             room, p.x_bytes);
+            if (whole_g) pg.copy(shared + slot_in + S::kX, from_g, room);
+            else th.copy_gates(p, reinterpret_cast<GT*>(mine + slot_in + S::kX), from_g, step_g, room);
+            from_x += next_x;
+            from_g += next_g;
+            slot_in = slot_in + stage == p.stages * stage ? 0 : slot_in + stage;
         }
         ++issued;
         copies_issued();
@@ -503,19 +546,19 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
         : states + (th.row.first + th.place(p, first * th.chunk + th.step0)) * p.C + th.ch;
     float* keep = kept == nullptr || th.wseg != 0 || th.sub != 0 ? nullptr
         : kept + kept_index(p, th.row, th.b, th.chunk, first) * p.C + th.ch;
-    const int64_t out_step = p.reverse ? -(int64_t)p.C : p.C;
-    for (int64_t i = 0; i < n; ++i) {
+    const int out_step = p.reverse ? -p.C : p.C;
+    const int64_t out_next = (int64_t)th.chunk * out_step;
+    for (int i = 0; i < n; ++i) {
         issue();
         copies_wait(p.stages - 1);
         __syncwarp();
-        const unsigned char* at = mine + slot * stage;
-        slot = slot + 1 == p.stages ? 0 : slot + 1;
+        const unsigned char* at = mine + slot;
+        slot = slot + stage == p.stages * stage ? 0 : slot + stage;
         const VT* const tx = reinterpret_cast<const VT*>(at);
         const GT* const tg = reinterpret_cast<const GT*>(at + S::kX);
         F2 a[L], u[L], A, B;
         // (a step beyond the row has no thickness and no value: it changes nothing)
-        auto scan = [&](auto safe, auto weighted) {
-            constexpr bool SAFE = decltype(safe)::value;
+        auto scan = [&](auto weighted) {
             A = two(1.f);
             B = two(0.f);
 #pragma unroll
@@ -525,11 +568,7 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
                 th.template gates<BACK || decltype(weighted)::value>(tg, l, a[l], w);
                 const F2 v = BACK && x == nullptr ? two(0.f) : th.at(tx, l);
                 if (BACK) {
-                    const F2 t = add2(B, v);
-                    B = SAFE ? past2(a[l], t, two(0.f)) : mul2(a[l], t);
-                } else if (SAFE) {
-                    u[l] = {times(w.x, v.x), times(w.y, v.y)};
-                    B = past2(a[l], B, u[l]);
+                    B = mul2(a[l], add2(B, v));
                 } else {
                     u[l] = decltype(weighted)::value ? v : mul2(w, v);
                     B = fma2(a[l], B, u[l]);
@@ -537,15 +576,27 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
                 A = mul2(A, a[l]);
             }
         };
-        auto scan_safely = [&](auto safe) {
-            if (p.weighted) scan(safe, std::true_type{});
-            else scan(safe, std::false_type{});
-        };
-        scan_safely(std::false_type{});
+        if (p.weighted) scan(std::true_type{});
+        else scan(std::false_type{});
         // What is not finite stays so to the end of the stretch; then the steps that do not count
-        // are told from those that do.
+        // are told from those that do, in a loop of its own.
         bool odd = spoilt(A, B) != 0.f;
-        if (odd) scan_safely(std::true_type{});
+        if (odd) {
+            A = two(1.f);
+            B = two(0.f);
+#pragma unroll 1
+            for (int j = 0; j < L; ++j) {
+                F2 al, ul;
+                if (BACK) {
+                    th.step(p, x == nullptr ? nullptr : tx, tg, L - 1 - j, al, ul, true);
+                    B = past2(al, add2(B, ul), two(0.f));
+                } else {
+                    th.step(p, tx, tg, j, al, ul, false);
+                    B = past2(al, B, ul);
+                }
+                A = mul2(A, al);
+            }
+        }
         if (keep != nullptr) {
             th.put(p, keep, carry);
             keep += p.C;
@@ -585,7 +636,7 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
             odd |= spoilt(h, h) != 0.f;
             const int64_t t0 = (first + i) * th.chunk + th.step0;
             VT* to = out;
-            out += th.chunk * out_step;
+            out += out_next;
             if (th.have && t0 + L <= th.row.len && !odd) {
 #pragma unroll
                 for (int l = 0; l < L; ++l, to += out_step) {
@@ -593,10 +644,12 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
                     th.store(p, to, h);
                 }
             } else if (th.have) {
-#pragma unroll
-                for (int l = 0; l < L; ++l, to += out_step) {
-                    h = past2(a[l], h, u[l]);
-                    if (t0 + l < th.row.len) th.store(p, to, h);
+#pragma unroll 1
+                for (int l = 0; l < L && t0 + l < th.row.len; ++l, to += out_step) {
+                    F2 al, ul;
+                    th.step(p, tx, tg, l, al, ul, false);
+                    h = past2(al, h, ul);
+                    th.store(p, to, h);
                 }
             }
         }
@@ -632,7 +685,7 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
     __shared__ float2 s_flow[2][kScanWarps][32];
     Th th;
     if (!th.init(p)) return;
-    const int64_t n = th.k1 - th.k0;
+    const int n = (int)(th.k1 - th.k0);
     const int stage = 2 * S::kX + S::kG;
     unsigned char* const mine = s_tiles + (size_t)th.warp * p.stages * stage;
     float* const sums = reinterpret_cast<float*>(s_tiles + (size_t)kScanWarps * p.stages * stage +
@@ -640,30 +693,43 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
     th.clear(p, mine, p.stages * stage);
     const int64_t first = th.k1 - 1;
     const int64_t step_x = p.reverse ? -p.xs : p.xs, step_g = p.reverse ? -p.gs : p.gs;
-    const int64_t step_c = p.reverse ? -(int64_t)p.C : p.C, step_h = p.reverse ? -(int64_t)p.H : p.H;
+    const int step_c = p.reverse ? -p.C : p.C, step_h = p.reverse ? -p.H : p.H;
     const int64_t at0 = th.place(p, first * th.chunk);
     const VT* from_x = x + (p.offsets ? th.row.first * p.xs : th.b * p.xb) + at0 * p.xs +
                        th.tile.first;
     const GT* from_g = static_cast<const GT*>(p.g) +
         (p.offsets ? th.row.first * p.gs : th.b * p.gb) + at0 * p.gs + th.tile.head;
-    const VT* from_d = d == nullptr ? nullptr : d + (th.row.first + at0) * p.C + th.tile.first;
-    int64_t issued = 0;
-    int slot_in = 0, slot = 0;
+    const VT* from_d = d + (th.row.first + at0) * p.C + th.tile.first;
+    typename Th::template Pieces<VT> px, pd;
+    typename Th::template Pieces<GT> pg;
+    px.init(p, th, step_x);
+    pd.init(p, th, step_c);
+    pg.init(p, th, step_g);
+    const bool whole_x = p.x_bytes == 16, whole_d = p.d_bytes == 16;
+    const bool whole_g = PC && p.D == 1 && p.g_bytes == 16;
+    const unsigned shared = (unsigned)__cvta_generic_to_shared(mine);
+    int issued = 0, slot_in = 0, slot = 0;      // (offsets of the tiles' places)
     auto issue = [&] {
         if (issued < n) {
-            unsigned char* at = mine + slot_in * stage;
             const int room = th.room(first - issued);
-            th.template copy_rows<VT, 2>(p, reinterpret_cast<VT*>(at), from_x, step_x, room,
-                                         p.x_bytes);
-            from_x -= th.chunk * step_x;
+            if (whole_x) px.copy(shared + slot_in, from_x, room);
+            else
+                th.template copy_rows<VT, 2>(p, reinterpret_cast<VT*>(mine + slot_in), from_x, step_x,
+                                             room, p.x_bytes);
             if (d != nullptr) {
-                th.template copy_rows<VT, 2>(p, reinterpret_cast<VT*>(at + S::kX), from_d, step_c,
-                                             room, p.d_bytes);
-                from_d -= th.chunk * step_c;
+                if (whole_d) pd.copy(shared + slot_in + S::kX, from_d, room);
+                else
+                    th.template copy_rows<VT, 2>(p, reinterpret_cast<VT*>(mine + slot_in + S::kX),
+                                                 from_d, step_c, room, p.d_bytes);
             }
-            th.copy_gates(p, reinterpret_cast<GT*>(at + 2 * S::kX), from_g, step_g, room);
+            if (whole_g) pg.copy(shared + slot_in + 2 * S::kX, from_g, room);
+            else
+                th.copy_gates(p, reinterpret_cast<GT*>(mine + slot_in + 2 * S::kX), from_g, step_g,
+                              room);
+            from_x -= th.chunk * step_x;
+            from_d -= (int64_t)th.chunk * step_c;
             from_g -= th.chunk * step_g;
-            slot_in = slot_in + 1 == p.stages ? 0 : slot_in + 1;
+            slot_in = slot_in + stage == p.stages * stage ? 0 : slot_in + stage;
         }
         ++issued;
         copies_issued();
@@ -677,46 +743,50 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
     const int64_t out0 = th.row.first + th.place(p, first * th.chunk + th.step0 + L - 1);
     VT* to_x = dx == nullptr ? nullptr : dx + out0 * p.C + th.ch;
     GT* to_g = dg == nullptr || p.D > 1 ? nullptr : dg + out0 * p.H + th.ch;
-    for (int64_t i = 0; i < n; ++i) {
+    const bool summed = dg != nullptr && p.D > 1;
+    for (int i = 0; i < n; ++i) {
         const int64_t k = first - i;
         issue();
         copies_wait(p.stages - 1);
         __syncwarp();
-        const unsigned char* at = mine + slot * stage;
-        slot = slot + 1 == p.stages ? 0 : slot + 1;
+        const unsigned char* at = mine + slot;
+        slot = slot + stage == p.stages * stage ? 0 : slot + stage;
         const VT* const tx = reinterpret_cast<const VT*>(at);
         const VT* const td = reinterpret_cast<const VT*>(at + S::kX);
         const GT* const tg = reinterpret_cast<const GT*>(at + 2 * S::kX);
         F2 h = h_next;
         keep -= p.C;
         if (i + 1 < n) h_next = th.get(keep);
-        F2 a[L], w[L], A, B, E;
-        auto scan = [&](auto safe, auto weighted) {
-            constexpr bool SAFE = decltype(safe)::value;
-            A = two(1.f);
-            B = E = two(0.f);
+        F2 a[L], w[L], A = two(1.f), B = two(0.f), E = two(0.f);
+        auto scan = [&](auto weighted) {
 #pragma unroll
             for (int l = 0; l < L; ++l) {
                 th.template gates<decltype(weighted)::value>(tg, l, a[l], w[l]);
                 const F2 v = th.at(tx, l);
-                if (SAFE) B = past2(a[l], B, {times(w[l].x, v.x), times(w[l].y, v.y)});
-                else B = fma2(a[l], B, decltype(weighted)::value ? v : mul2(w[l], v));
+                B = fma2(a[l], B, decltype(weighted)::value ? v : mul2(w[l], v));
                 A = mul2(A, a[l]);
             }
-            if (d == nullptr) return;
+        };
+        if (p.weighted) scan(std::true_type{});
+        else scan(std::false_type{});
+        if (d != nullptr)
 #pragma unroll
-            for (int l = L - 1; l >= 0; --l) {
-                const F2 t = add2(E, th.at(td, l));
-                E = SAFE ? past2(a[l], t, two(0.f)) : mul2(a[l], t);
-            }
-        };
-        auto scan_safely = [&](auto safe) {
-            if (p.weighted) scan(safe, std::true_type{});
-            else scan(safe, std::false_type{});
-        };
-        scan_safely(std::false_type{});
+            for (int l = L - 1; l >= 0; --l) E = mul2(a[l], add2(E, th.at(td, l)));
         bool odd = spoilt(A, B) != 0.f || spoilt(E, E) != 0.f;
-        if (odd) scan_safely(std::true_type{});
+        if (odd) {
+            F2 al, ul;
+            B = E = two(0.f);
+#pragma unroll 1
+            for (int l = 0; l < L; ++l) {
+                th.step(p, tx, tg, l, al, ul, false);
+                B = past2(al, B, ul);
+            }
+#pragma unroll 1
+            for (int l = L - 1; l >= 0; --l) {
+                th.step(p, d == nullptr ? nullptr : td, tg, l, al, ul, true);
+                E = past2(al, add2(E, ul), two(0.f));
+            }
+        }
         F2 EA = A, TA, TB, TE, all_a;
         join_lanes<false>(p.lanes, th.lane, A, B, TA, TB);
         join_lanes<true>(p.lanes, th.lane, EA, E, all_a, TE);
@@ -766,57 +836,69 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
         odd |= spoilt(h, G) != 0.f;
         const int64_t t0 = k * th.chunk + th.step0;
         const bool whole = t0 + L <= th.row.len;
-        auto unwind = [&](auto safe, auto weighted) {
-            constexpr bool SAFE = decltype(safe)::value, WEIGHTED = decltype(weighted)::value;
+        // (dg of a step goes where it belongs, or to the sums of its group)
+        auto give = [&](int l, bool in, F2 wG, F2 one) {
+            if (dx != nullptr && in) th.store(p, to_x - (int64_t)(L - 1 - l) * step_c, wG);
+            if (to_g != nullptr) {
+                if (in) th.store(p, to_g - (int64_t)(L - 1 - l) * step_h, one);
+            } else if (!summed) {
+            } else if (PC) {
+                sums[l * S::kPitch + th.lane * 2] = one.x;
+                sums[l * S::kPitch + th.lane * 2 + 1] = one.y;
+            } else {
+                sums[l * S::kPitch + th.lane] = one.x + one.y;
+            }
+        };
+        auto unwind = [&](auto weighted) {
+            constexpr bool WEIGHTED = decltype(weighted)::value;
             // forwards: what dg has besides the adjoint
             F2 q[L];
 #pragma unroll
             for (int l = 0; l < L; ++l) {
-                F2 v = th.at(tx, l);
-                if (SAFE) {
-                    const F2 u{times(w[l].x, v.x), times(w[l].y, v.y)};
-                    // (a value that is not finite in a place of no thickness is no sample)
-                    if (w[l].x == 0.f && !finite(v.x)) v.x = h.x;
-                    if (w[l].y == 0.f && !finite(v.y)) v.y = h.y;
-                    q[l].x = a[l].x == 0.f ? 0.f : a[l].x * (WEIGHTED ? -h.x : v.x - h.x);
-                    q[l].y = a[l].y == 0.f ? 0.f : a[l].y * (WEIGHTED ? -h.y : v.y - h.y);
-                    h = past2(a[l], h, u);
-                } else {
-                    q[l] = mul2(a[l], fma2(h, two(-1.f), WEIGHTED ? two(0.f) : v));
-                    h = fma2(a[l], h, WEIGHTED ? v : mul2(w[l], v));
-                }
+                const F2 v = th.at(tx, l);
+                q[l] = mul2(a[l], fma2(h, two(-1.f), WEIGHTED ? two(0.f) : v));
+                h = fma2(a[l], h, WEIGHTED ? v : mul2(w[l], v));
             }
             // and back
 #pragma unroll
             for (int l = L - 1; l >= 0; --l) {
-                const bool in = th.have && (whole || t0 + l < th.row.len);
                 if (d != nullptr) G = add2(G, th.at(td, l));
-                if (dx != nullptr && in)
-                    th.store(p, to_x - (L - 1 - l) * step_c, WEIGHTED ? G : mul2(w[l], G));
-                if (dg != nullptr) {
-                    const F2 one = mul2(q[l], G);
-                    if (to_g != nullptr) {
-                        if (in) th.store(p, to_g - (L - 1 - l) * step_h, one);
-                    } else if (PC) {
-                        sums[l * S::kPitch + th.lane * 2] = one.x;
-                        sums[l * S::kPitch + th.lane * 2 + 1] = one.y;
-                    } else {
-                        sums[l * S::kPitch + th.lane] = one.x + one.y;
-                    }
-                }
-                G = SAFE ? past2(a[l], G, two(0.f)) : mul2(a[l], G);
+                give(l, th.have && (whole || t0 + l < th.row.len), WEIGHTED ? G : mul2(w[l], G),
+                     mul2(q[l], G));
+                G = mul2(a[l], G);
             }
         };
-        if (p.weighted) {
-            if (odd) unwind(std::true_type{}, std::true_type{});
-            else unwind(std::false_type{}, std::true_type{});
+        if (odd) {
+            F2 before[L], al, ul;
+#pragma unroll 1
+            for (int l = 0; l < L; ++l) {
+                before[l] = h;
+                th.step(p, tx, tg, l, al, ul, false);
+                h = past2(al, h, ul);
+            }
+#pragma unroll 1
+            for (int l = L - 1; l >= 0; --l) {
+                F2 wl, v = th.at(tx, l), q;
+                th.template gates<false>(tg, l, al, wl);
+                if (p.weighted) wl = two(1.f);
+                if (d != nullptr) G = add2(G, th.at(td, l));
+                const F2 hb = before[l];
+                // (a value that is not finite in a place of no thickness is no sample)
+                if (wl.x == 0.f && !finite(v.x)) v.x = hb.x;
+                if (wl.y == 0.f && !finite(v.y)) v.y = hb.y;
+                q.x = al.x == 0.f ? 0.f : al.x * (p.weighted ? -hb.x : v.x - hb.x);
+                q.y = al.y == 0.f ? 0.f : al.y * (p.weighted ? -hb.y : v.y - hb.y);
+                give(l, th.have && t0 + l < th.row.len, mul2(wl, G), mul2(q, G));
+                G = past2(al, G, two(0.f));
+            }
+        } else if (p.weighted) {
+            unwind(std::true_type{});
         } else {
-            if (odd) unwind(std::true_type{}, std::false_type{});
-            else unwind(std::false_type{}, std::false_type{});
+            unwind(std::false_type{});
         }
-        if (to_x != nullptr) to_x -= th.chunk * step_c;
-        if (to_g != nullptr) to_g -= th.chunk * step_h;
-        if (p.D > 1 && dg != nullptr) {
+        if (to_x != nullptr) to_x -= (int64_t)th.chunk * step_c;
+        if (to_g != nullptr) to_g -= (int64_t)th.chunk * step_h;
+        if (summed) {
             __syncwarp();
             const int heads = p.parts > 1 ? 1 : th.tile.width / p.D, subs = 32 / p.lanes;
             const int tasks = L * subs * heads;
