@@ -31,10 +31,22 @@ int status_of_rays(int clear, int* word) {
 
 RayPlan ray_plan(const svoxb_scan* s) {
     RayPlan plan;
-    if (!s->last_only || !s->reverse || s->H != 1 || s->C > kRayChannels) return plan;
+    if (!s->last_only || !s->reverse || s->H != 1) return plan;
     const int64_t mean = s->offsets ? (s->B > 0 ? s->T / s->B : 0) : s->T;
     // (their lengths are counted in 32 bits)
     if (mean > kRayLongest || (s->offsets && s->T > 0x7fffffff - 256)) return plan;
+    if (s->C > kRayChannels) {
+        const int size = s->values_type == SVOXB_TYPE_F32 ? 4 : 2, piece = 16 / size;
+        const bool whole = reinterpret_cast<uintptr_t>(s->values) % 16 == 0 && s->C % piece == 0 &&
+                           s->values_step % piece == 0 && s->values_row % piece == 0;
+        plan.share = whole ? piece : 1;
+        const int shares = s->C / plan.share;
+        if (shares > (whole ? 32 : 128)) return RayPlan{};
+        plan.width = 1;
+        while (plan.width < shares && plan.width < 32) plan.width *= 2;
+        plan.lanes = 32;
+        return plan;
+    }
     const bool dense = s->values_step == s->C && s->thickness_step == 1 &&
                        (s->offsets || ((s->values_row == s->T * s->C || s->B == 1) &&
                                        (s->thickness_row == s->T || s->B == 1)));
@@ -105,6 +117,23 @@ void with_kernel(const svoxb_scan* s, RayPlan plan, F f) {
     else types(Types<__half, float>{});
 }
 
+// The same for more channels: the types, the channels of a lane, and how often it has them.
+template <class F>
+void with_rows(const svoxb_scan* s, RayPlan plan, F f) {
+    auto types = [&](auto t) {
+        constexpr int piece = 16 / (int)sizeof(typename decltype(t)::V);
+        if (plan.share > 1) f(t, Int<piece>{}, Int<1>{});
+        else if (s->C <= 32) f(t, Int<1>{}, Int<1>{});
+        else f(t, Int<1>{}, Int<4>{});
+    };
+    const bool same = s->thickness_type == s->values_type;
+    if (s->values_type == SVOXB_TYPE_F32) types(Types<float, float>{});
+    else if (s->values_type == SVOXB_TYPE_BF16 && same) types(Types<__nv_bfloat16, __nv_bfloat16>{});
+    else if (s->values_type == SVOXB_TYPE_BF16) types(Types<__nv_bfloat16, float>{});
+    else if (same) types(Types<__half, __half>{});
+    else types(Types<__half, float>{});
+}
+
 unsigned blocks_of(const svoxb_scan* s, RayPlan plan) {
     return (unsigned)((s->B * plan.lanes + kRayBlock - 1) / kRayBlock);
 }
@@ -112,7 +141,17 @@ unsigned blocks_of(const svoxb_scan* s, RayPlan plan) {
 }  // namespace
 
 int ray_forward(const svoxb_scan* s, RayPlan plan, float* last, float* kept, cudaStream_t stream) {
-    const ScanArgs p = ray_args(s);
+    ScanArgs p = ray_args(s);
+    if (plan.width) {
+        p.lanes = plan.width;
+        with_rows(s, plan, [&](auto t, auto v, auto n) {
+            row_kernel<typename decltype(t)::V, typename decltype(t)::G, decltype(v)::value,
+                       decltype(n)::value>
+                <<<blocks_of(s, plan), kRayBlock, 0, stream>>>(p, last, kept);
+        });
+        SVOXB_CUDA(cudaGetLastError());
+        return SVOXB_OK;
+    }
     with_kernel(s, plan, [&](auto t, auto c, auto g, auto quads) {
         using VT = typename decltype(t)::V;
         using GT = typename decltype(t)::G;
@@ -129,6 +168,19 @@ int ray_forward(const svoxb_scan* s, RayPlan plan, float* last, float* kept, cud
 int ray_backward(const svoxb_scan* s, RayPlan plan, const float* kept, const float* d_last, void* dx,
                  void* dg, float* dh0, cudaStream_t stream) {
     ScanArgs p = ray_args(s);
+    if (plan.width) {
+        p.lanes = plan.width;
+        p.paired = reinterpret_cast<uintptr_t>(dx) % 16 == 0;
+        with_rows(s, plan, [&](auto t, auto v, auto n) {
+            using VT = typename decltype(t)::V;
+            using GT = typename decltype(t)::G;
+            row_back_kernel<VT, GT, decltype(v)::value, decltype(n)::value>
+                <<<blocks_of(s, plan), kRayBlock, 0, stream>>>(
+                    p, kept, d_last, static_cast<VT*>(dx), static_cast<GT*>(dg), dh0);
+        });
+        SVOXB_CUDA(cudaGetLastError());
+        return SVOXB_OK;
+    }
     with_kernel(s, plan, [&](auto t, auto c, auto g, auto quads) {
         using VT = typename decltype(t)::V;
         using GT = typename decltype(t)::G;

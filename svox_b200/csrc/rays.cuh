@@ -24,7 +24,7 @@
 namespace svoxb {
 
 constexpr int kRayBlock = 64;       // (rays differ in length: blocks of few wait for few)
-constexpr int kRayChannels = 4;     // at most
+constexpr int kRayChannels = 4;     // of those whose channels are summed in every lane
 
 template <class VT, class GT, int C, int G>
 struct RayThread {
@@ -431,6 +431,194 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
             if (th.lane == c) dh0[th.b * C + c] = past(T_end, d[c], 0.f);
     clear_uncovered(p, th.b, 0, C, (int64_t)C, dx, th.lane, G);
     clear_uncovered(p, th.b, 0, 1, (int64_t)1, dg, th.lane, G);
+}
+
+// ---------------------------------------------------------------------------
+// Values of more channels (features): 32 samples are weighted at a time, one to a lane, and then
+// their values go by, `width` lanes to a sample with V channels each (16 bytes where rows lie on
+// 16-byte boundaries), NT times over where a lane's share is one channel and there are more than 32.
+// The exponentials are those of the samples, not of their channels.
+template <class VT, class GT, int V, int NT>
+struct RayRows {
+    int width, per;             // lanes of a sample; samples that go by at once
+    int sub, cl;                // which of those is this lane's; its share
+    int have;                   // lanes' shares of a row that exist: cl + t * 32 < have
+
+    __device__ __forceinline__ void init(const ScanArgs& p) {
+        const int lane = threadIdx.x & 31;
+        width = p.lanes;
+        per = 32 / width;
+        sub = lane / width;
+        cl = lane - sub * width;
+        have = p.C / V;
+    }
+    __device__ __forceinline__ bool on(int t) const { return cl + 32 * t < have; }
+    __device__ __forceinline__ int ch(int t) const { return (cl + 32 * t) * V; }
+};
+
+template <class VT, class GT, int V, int NT>
+__global__ void __launch_bounds__(kRayBlock)
+row_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
+    RayThread<VT, GT, 1, 32> th;
+    RayRows<VT, GT, V, NT> rows;
+    th.init(p);
+    rows.init(p);
+    float S = 0.f, acc[NT][V];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[t][v] = 0.f;
+    float* keep = kept != nullptr && th.lane == 0 ? kept + th.kept_at(p) : nullptr;
+    const VT* x = th.x + ((int64_t)rows.sub - th.lane) * p.xs;      // this lane's row of the chunk
+    float g_next = th.lane < th.len ? to_float(*th.g) : 0.f;
+    for (int k = 0; k < th.chunks; ++k) {
+        const int left = th.len - 32 * k;
+        const float gi = g_next;
+        th.g += 32 * p.gs;
+        g_next = th.lane + 32 < left ? to_float(*th.g) : 0.f;
+        if (keep != nullptr) keep[k] = S;
+        const float v = S + th.upto(gi);
+        float before = __shfl_up_sync(~0u, v, 1);
+        if (th.lane == 0) before = S;
+        S = __shfl_sync(~0u, v, 31);
+        const float T = decay_of(before);
+        const float W = p.weighted ? T : T * weight_of(gi, decay_of(gi));
+        const int n = left < 32 ? (left + rows.per - 1) / rows.per : rows.width;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+            const int s = j * rows.per + rows.sub;
+            const VT* const row = x + (int64_t)(j * rows.per) * p.xs;
+            const float w = __shfl_sync(~0u, W, s);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float xv[V];
+#pragma unroll
+                for (int q = 0; q < V; ++q) xv[q] = 0.f;
+                if (s < left && rows.on(t)) load_some<V>(row + rows.ch(t), xv);
+                if (w != 0.f)
+#pragma unroll
+                    for (int q = 0; q < V; ++q) acc[t][q] = fmaf(w, xv[q], acc[t][q]);
+            }
+        }
+        x += 32 * p.xs;
+    }
+    if (!th.there) return;
+    for (int d = rows.width; d < 32; d *= 2)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int q = 0; q < V; ++q) acc[t][q] += __shfl_xor_sync(~0u, acc[t][q], d);
+    const float T = decay_of(S);
+    if (rows.sub == 0)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            if (rows.on(t))
+#pragma unroll
+                for (int q = 0; q < V; ++q) {
+                    const int c = rows.ch(t) + q;
+                    const float bg = p.h0 != nullptr ? __ldg(p.h0 + th.b * p.hb + c) : 0.f;
+                    last[th.b * p.C + c] = past(T, bg, acc[t][q]);
+                }
+}
+
+template <class VT, class GT, int V, int NT>
+__global__ void __launch_bounds__(kRayBlock)
+row_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restrict__ d_last,
+                VT* __restrict__ dx, GT* __restrict__ dg, float* __restrict__ dh0) {
+    RayThread<VT, GT, 1, 32> th;
+    RayRows<VT, GT, V, NT> rows;
+    th.init(p);
+    rows.init(p);
+    if (!th.there) return;
+    float d[NT][V], bg = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            const int c = rows.ch(t) + q;
+            d[t][q] = d_last != nullptr && rows.on(t) ? __ldg(d_last + th.b * p.C + c) : 0.f;
+            if (p.h0 != nullptr && rows.on(t))
+                bg = fmaf(d[t][q], __ldg(p.h0 + th.b * p.hb + c), bg);
+        }
+    for (int o = 1; o < rows.width; o *= 2) bg += __shfl_xor_sync(~0u, bg, o);
+    const float* const keep = kept + th.kept_at(p);
+    float T_end = 1.f, behind = 0.f;
+    for (int k = th.chunks - 1; k >= 0; --k) {
+        const int left = th.len - 32 * k;
+        const bool in = th.lane < left;
+        const float S = keep[k];
+        const float gi = in ? to_float(th.g[(int64_t)k * 32 * p.gs]) : 0.f;
+        const int n = left < 32 ? (left + rows.per - 1) / rows.per : rows.width;
+        const VT* const x = th.x + ((int64_t)k * 32 + rows.sub - th.lane) * p.xs;
+        // d . x of each sample, to its lane
+        float c = 0.f;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+            const int s = j * rows.per + rows.sub;
+            float part = 0.f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float xv[V];
+#pragma unroll
+                for (int q = 0; q < V; ++q) xv[q] = 0.f;
+                if (s < left && rows.on(t))
+                    load_some<V>(x + (int64_t)(j * rows.per) * p.xs + rows.ch(t), xv);
+#pragma unroll
+                for (int q = 0; q < V; ++q) part = fmaf(d[t][q], xv[q], part);
+            }
+            for (int o = 1; o < rows.width; o *= 2) part += __shfl_xor_sync(~0u, part, o);
+            part = __shfl_sync(~0u, part, (th.lane & (rows.per - 1)) * rows.width);
+            if (th.lane / rows.per == j) c = part;
+        }
+        const float v = S + th.upto(gi);
+        float before = __shfl_up_sync(~0u, v, 1);
+        if (th.lane == 0) before = S;
+        if (k == th.chunks - 1) {
+            T_end = decay_of(__shfl_sync(~0u, v, 31));
+            behind = past(T_end, bg, 0.f);
+        }
+        const float a = decay_of(gi), T = decay_of(before), Tn = T * a;
+        const float w = p.weighted ? (in ? 1.f : 0.f) : weight_of(gi, a), W = T * w;
+        const float here = th.from(times(W, c)) + behind;
+        float rest = __shfl_down_sync(~0u, here, 1);
+        if (th.lane == 31) rest = behind;
+        behind = __shfl_sync(~0u, here, 0);
+        if (dg != nullptr && in) {
+            // (a value that is not finite in a place of no thickness is no sample)
+            const float own = p.weighted || Tn == 0.f ? 0.f : Tn * c;
+            dg[th.first + (int64_t)k * 32 + th.lane] =
+                from_float<GT>(w == 0.f && !finite(c) ? 0.f : own - rest);
+        }
+        if (dx != nullptr) {
+            VT* const to = dx + (th.first + (int64_t)k * 32 + rows.sub) * p.C;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) {
+                const int s = j * rows.per + rows.sub;
+                const float Ws = __shfl_sync(~0u, W, s);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    float out[V];
+#pragma unroll
+                    for (int q = 0; q < V; ++q) out[q] = Ws * d[t][q];
+                    if (s >= left || !rows.on(t)) continue;
+                    VT* const row = to + (int64_t)(j * rows.per) * p.C + rows.ch(t);
+                    if (p.paired) store_some<V>(row, out);
+                    else
+#pragma unroll
+                        for (int q = 0; q < V; ++q) row[q] = from_float<VT>(out[q]);
+                }
+            }
+        }
+    }
+    if (dh0 != nullptr && rows.sub == 0)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            if (rows.on(t))
+#pragma unroll
+                for (int q = 0; q < V; ++q)
+                    dh0[th.b * p.C + rows.ch(t) + q] = past(T_end, d[t][q], 0.f);
+    clear_uncovered(p, th.b, 0, p.C, (int64_t)p.C, dx, th.lane, 32);
+    clear_uncovered(p, th.b, 0, 1, (int64_t)1, dg, th.lane, 32);
 }
 
 }  // namespace svoxb

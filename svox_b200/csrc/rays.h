@@ -9,11 +9,12 @@
 namespace svoxb {
 
 
-// How a call goes to these kernels: lanes of a ray (0: not at all), and whether a lane takes four
-// neighbouring samples.
+// How a call goes to these kernels: lanes of a ray (0: not at all), whether a lane takes four
+// neighbouring samples, and where there are more channels, lanes of a sample and channels of a lane.
 struct RayPlan {
     int lanes = 0;
     bool quads = false;
+    int width = 0, share = 0;
 };
 RayPlan ray_plan(const svoxb_scan* s);
 int64_t ray_kept(const svoxb_scan* s, RayPlan plan);

@@ -186,7 +186,9 @@ def test_packed(cuda_device, C, H, dtype, reverse):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("C,dtype", [(1, F32), (2, F32), (3, F32), (3, BF16), (4, F32), (7, F16),
-                                     (8, BF16), (32, BF16), (35, F32), (64, F16)])
+                                     (8, BF16), (32, BF16), (35, F32), (64, F16), (5, BF16),
+                                     (12, F32), (100, F32), (128, BF16), (200, F32), (77, F16),
+                                     (128, F32), (127, F32)])
 @pytest.mark.parametrize("packed", [True, False])
 def test_composite(cuda_device, C, dtype, packed):
     gen = torch.Generator().manual_seed(C)
