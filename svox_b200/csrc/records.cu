@@ -1,6 +1,8 @@
 // C-ABI entry points of the quantised leaf records (see include/svox_b200.h).
 #include "records.cuh"
 
+#include <type_traits>
+
 #include "status.h"
 
 namespace svoxb {
@@ -70,21 +72,45 @@ int with_type(int type, F f) {
     }
 }
 
+// Calls f with the floats of a record and its group, if the compiler knows that layout.
+template <int N> using Int = std::integral_constant<int, N>;
+template <class F>
+bool with_layout(const RecordArgs& a, F f) {
+    if (a.K == 4 && a.group == 1) f(Int<4>{}, Int<1>{});
+    else if (a.K == 4 && a.group == 3) f(Int<4>{}, Int<3>{});
+    else if (a.K == 13 && a.group == 4) f(Int<13>{}, Int<4>{});
+    else if (a.K == 28 && a.group == 9) f(Int<28>{}, Int<9>{});
+    else if (a.K == 49 && a.group == 16) f(Int<49>{}, Int<16>{});
+    else if (a.K == 76 && a.group == 25) f(Int<76>{}, Int<25>{});
+    else return false;
+    return true;
+}
+
+template <class Kernel>
+int ready(Kernel kernel, int block, size_t smem) {
+    int per_sm = 0;
+    return blocks_per_sm(reinterpret_cast<const void*>(kernel), block, smem, &per_sm);
+}
+
 template <class T, bool E4M3>
 int launch_read(const RecordArgs& a, const TopTable& top, const float* points, const int64_t* ids,
                 int64_t Q, T* out, cudaStream_t stream) {
-    int per = 32;
-    while (per * a.bytes > kRecordStage && per > 1) per /= 2;
     const unsigned grid = (unsigned)((Q + kRecordsBlock - 1) / kRecordsBlock);
-    const size_t smem = (size_t)kRecordsBlock / 32 * per * a.bytes;
-    auto run = [&](auto kernel) {
-        kernel<<<grid, kRecordsBlock, smem, stream>>>(a, top, points, ids, Q, out, per);
-    };
-    if (a.K == 13 && a.group == 4) run(records_read_kernel<T, E4M3, 13, 4>);
-    else if (a.K == 28 && a.group == 9) run(records_read_kernel<T, E4M3, 28, 9>);
-    else if (a.K == 49 && a.group == 16) run(records_read_kernel<T, E4M3, 49, 16>);
-    else if (a.K == 76 && a.group == 25) run(records_read_kernel<T, E4M3, 76, 25>);
-    else run(records_read_kernel<T, E4M3, 0, 0>);
+    int st = SVOXB_OK;
+    const bool known = with_layout(a, [&](auto k, auto g) {
+        auto kernel = records_read_known<T, E4M3, decltype(k)::value, decltype(g)::value>;
+        const size_t smem = (size_t)kRecordsBlock * a.K * sizeof(T);
+        if ((st = ready(kernel, kRecordsBlock, smem))) return;
+        kernel<<<grid, kRecordsBlock, smem, stream>>>(a, top, points, ids, Q, out);
+    });
+    if (st) return st;
+    if (!known) {
+        int per = 32;
+        while (per * a.bytes > kRecordStage && per > 1) per /= 2;
+        const size_t smem = (size_t)kRecordsBlock / 32 * per * a.bytes;
+        records_read_kernel<T, E4M3><<<grid, kRecordsBlock, smem, stream>>>(a, top, points, ids, Q,
+                                                                           out, per);
+    }
     SVOXB_CUDA(cudaGetLastError());
     return SVOXB_OK;
 }
@@ -92,17 +118,26 @@ int launch_read(const RecordArgs& a, const TopTable& top, const float* points, c
 template <class T, bool E4M3>
 int launch_write(const RecordArgs& a, const int64_t* found, int64_t Q, const T* values,
                  cudaStream_t stream) {
-    int per = 32;
-    while ((per * a.bytes > kRecordStage || per * a.K * (int)sizeof(T) > kValueStage) && per > 1)
-        per /= 2;
-    const unsigned grid = (unsigned)((Q + kRecordsBlock - 1) / kRecordsBlock);
-    const size_t warp = per * a.bytes + stepped((size_t)per * a.K * sizeof(T), 16);
-    const size_t smem = kRecordsBlock / 32 * warp;
-    auto kernel = records_write_kernel<T, E4M3>;
-    int per_sm = 0;
-    const int st = blocks_per_sm(reinterpret_cast<const void*>(kernel), kRecordsBlock, smem, &per_sm);
+    int st = SVOXB_OK;
+    const bool known = with_layout(a, [&](auto k, auto g) {
+        auto kernel = records_write_known<T, E4M3, decltype(k)::value, decltype(g)::value>;
+        const size_t smem = (size_t)kWriteBlock * a.K * sizeof(T);
+        if ((st = ready(kernel, kWriteBlock, smem))) return;
+        kernel<<<(unsigned)((Q + kWriteBlock - 1) / kWriteBlock), kWriteBlock, smem, stream>>>(
+            a, found, Q, values);
+    });
     if (st) return st;
-    kernel<<<grid, kRecordsBlock, smem, stream>>>(a, found, Q, values, per);
+    if (!known) {
+        int per = 32;
+        while ((per * a.bytes > kRecordStage || per * a.K * (int)sizeof(T) > kValueStage) && per > 1)
+            per /= 2;
+        const unsigned grid = (unsigned)((Q + kRecordsBlock - 1) / kRecordsBlock);
+        const size_t warp = per * a.bytes + stepped((size_t)per * a.K * sizeof(T), 16);
+        auto kernel = records_write_kernel<T, E4M3>;
+        const size_t smem = kRecordsBlock / 32 * warp;
+        if ((st = ready(kernel, kRecordsBlock, smem))) return st;
+        kernel<<<grid, kRecordsBlock, smem, stream>>>(a, found, Q, values, per);
+    }
     SVOXB_CUDA(cudaGetLastError());
     return SVOXB_OK;
 }
