@@ -290,7 +290,7 @@ struct Record {
 template <class T> struct __align__(4 * sizeof(T)) Quad { T v[4]; };
 
 template <class T, bool E4M3, int K, int G>
-__global__ void __launch_bounds__(kRecordsBlock)
+__global__ void __launch_bounds__(kRecordsBlock, K <= 49 ? 6 : 5)
 records_read_known(RecordArgs r, TopTable top, const float* __restrict__ points,
                    const int64_t* __restrict__ ids, int64_t Q, T* __restrict__ out) {
     extern __shared__ __align__(16) uint8_t s_stage[];
@@ -306,47 +306,54 @@ records_read_known(RecordArgs r, TopTable top, const float* __restrict__ points,
 #pragma unroll
         for (int j = 0; j < rec.WORDS; ++j) rec.w[j] = 0xffffffffu;
     }
-    T* const rows = reinterpret_cast<T*>(s_stage) + (threadIdx.x >> 5) * 32 * K;
-    T* const mine = rows + lane * K;
-    float v[4];
+    // (half of the warp's rows at a time: what they take of the shared memory decides how many warps
+    // wait for their points side by side)
+    constexpr int ROWS = 16, PER = 16 / sizeof(T), WHOLE = ROWS * K / PER;
+    T* const rows = reinterpret_cast<T*>(s_stage) + (threadIdx.x >> 5) * ROWS * K;
+    T* const mine = rows + (lane % ROWS) * K;
+    const int n = (int)(Q - wb < 32 ? Q - wb : 32);
+    const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll 1
+    for (int first = 0; first < n; first += ROWS) {
+        // (decoded in either round anew: kept for both, K floats a lane would fill the registers)
 #pragma unroll
-    for (int c = 0; c < K; ++c) {
-        if (c == K - 1) {
-            v[c % 4] = rec.density();
-        } else {
-            const float2 q = rec.codes(c & ~1);
-            v[c % 4] = (c % 2 ? q.y : q.x) * rec.scale(c / G);
+        for (int j = 0; j < rec.WORDS; ++j) asm volatile("" : "+r"(rec.w[j]));
+        if (lane / ROWS == first / ROWS) {
+            float v[4];
+#pragma unroll
+            for (int c = 0; c < K; ++c) {
+                if (c == K - 1) {
+                    v[c % 4] = rec.density();
+                } else {
+                    const float2 q = rec.codes(c & ~1);
+                    v[c % 4] = (c % 2 ? q.y : q.x) * rec.scale(c / G);
+                }
+                if (K % 4 != 0) {
+                    mine[c] = as_type<T>(slot < 0 ? __uint_as_float(0x7fc00000u) : v[c % 4]);
+                } else if (c % 4 == 3) {
+                    Quad<T> four;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        four.v[j] = as_type<T>(slot < 0 ? __uint_as_float(0x7fc00000u) : v[j]);
+                    *reinterpret_cast<Quad<T>*>(mine + c - 3) = four;
+                }
+            }
         }
-        if (K % 4 != 0) {
-            mine[c] = as_type<T>(slot < 0 ? __uint_as_float(0x7fc00000u) : v[c % 4]);
-        } else if (c % 4 == 3) {
-            Quad<T> four;
+        __syncwarp();
+        // (16 rows are a whole number of 16-byte words)
+        T* const to = out + (wb + first) * K;
+        const int left = (n - first < ROWS ? n - first : ROWS) * K;
+        if (aligned && left == ROWS * K) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                four.v[j] = as_type<T>(slot < 0 ? __uint_as_float(0x7fc00000u) : v[j]);
-            *reinterpret_cast<Quad<T>*>(mine + c - 3) = four;
-        }
-    }
-    __syncwarp();
-    // (32 rows are a whole number of 16-byte words)
-    const int n = (int)(Q - wb < 32 ? Q - wb : 32) * K;
-    constexpr int PER = 16 / sizeof(T);
-    T* const to = out + wb * K;
-    if ((reinterpret_cast<uintptr_t>(out) & 15) == 0) {
-        if (n == 32 * K) {
-#pragma unroll
-            for (int f = 0; f < 32 * K / PER; f += 32)
-                if (f + lane < 32 * K / PER)
+            for (int f = 0; f < WHOLE; f += 32)
+                if (f + lane < WHOLE)
                     reinterpret_cast<uint4*>(to)[f + lane] =
                         reinterpret_cast<const uint4*>(rows)[f + lane];
-            return;
+        } else {
+            for (int f = lane; f < left; f += 32) to[f] = rows[f];
         }
-        for (int f = lane; f < n / PER; f += 32)
-            reinterpret_cast<uint4*>(to)[f] = reinterpret_cast<const uint4*>(rows)[f];
-        if (lane < n % PER) to[n / PER * PER + lane] = rows[n / PER * PER + lane];
-        return;
+        __syncwarp();
     }
-    for (int f = lane; f < n; f += 32) to[f] = rows[f];
 }
 
 constexpr int kWriteBlock = 128;
@@ -375,7 +382,9 @@ records_write_known(RecordArgs r, const int64_t* __restrict__ found, int64_t Q,
     }
     // (without `found` row q is record q)
     const int64_t slot = i >= Q ? -1 : found != nullptr ? found[i] : i;
-    const bool wins = slot >= 0 && (found == nullptr || r.owner[slot] == (uint32_t)(i + 1));
+    const bool wins = slot >= 0 && (found == nullptr ||
+                                    atomicCAS(r.owner + slot, (uint32_t)(i + 1), 0u) ==
+                                        (uint32_t)(i + 1));
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
     if (!wins) return;
@@ -410,7 +419,6 @@ records_write_known(RecordArgs r, const int64_t* __restrict__ found, int64_t Q,
     }
     rec.w[rec.WORDS - 1] |= (uint32_t)__half_as_ushort(__float2half_rn(value(K - 1))) << 16;
     rec.store(r.records + slot * rec.R);
-    if (found != nullptr) r.owner[slot] = 0;
 }
 
 }  // namespace svoxb
