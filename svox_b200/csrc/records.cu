@@ -99,7 +99,8 @@ int launch_read(const RecordArgs& a, const TopTable& top, const float* points, c
     int st = SVOXB_OK;
     const bool known = with_layout(a, [&](auto k, auto g) {
         auto kernel = records_read_known<T, E4M3, decltype(k)::value, decltype(g)::value>;
-        const size_t smem = (size_t)kRecordsBlock / 2 * a.K * sizeof(T);
+        constexpr size_t smem = (size_t)kRecordsBlock / 32 *
+                                read_stage<T, decltype(k)::value, decltype(g)::value>();
         if ((st = ready(kernel, kRecordsBlock, smem))) return;
         kernel<<<grid, kRecordsBlock, smem, stream>>>(a, top, points, ids, Q, out);
     });
