@@ -435,19 +435,36 @@ struct ScanThread {
             if (have > 1) to[1] = from_float<T>(v.y);
         }
     }
-    // What the block's other ranges, before this one or (back) behind it, do to `h`.
-    __device__ __forceinline__ F2 ranges(const ScanArgs& p, const float2* pairs, F2 h,
-                                         bool back) const {
+    // What the row's other ranges, before this one or (back) behind it, do to `h`.  The unit's groups
+    // of lanes fold a part of them each, in the order of the steps (folded by every thread, up to 255
+    // pairs took 30 of the 45 us of a sequence of 131072 steps of 64 channels).
+    __device__ __forceinline__ F2 ranges(const ScanArgs& p, const float2* pairs, F2 h, bool back,
+                                         float4* shared) const {
+        if (p.splits == 1) return h;
         const int n = back ? p.splits - 1 - split : split;
-        const float2* at = pairs + (b * p.splits + (back ? p.splits - 1 : 0)) * p.C + ch;
-        const int64_t step = back ? -(int64_t)p.C : p.C;
-        if (have == 0) return h;
-        const int second = have - 1;
+        const int subs = 32 / p.lanes, workers = p.warps * subs, me = wseg * subs + sub;
+        const int per = (n + workers - 1) / workers;
+        const int from = per * me < n ? per * me : n, to = from + per < n ? from + per : n;
+        const float2* at = pairs + (b * p.splits + (back ? p.splits - 1 - from : from)) * p.C + ch;
+        const int step = back ? -p.C : p.C;
+        F2 A = two(1.f), B = two(0.f);
+        if (have > 0) {
+            const int second = have - 1;
 #pragma unroll 8
-        for (int s = 0; s < n; ++s) {
-            const float2 q = __ldcg(at + s * step), r = __ldcg(at + s * step + second);
-            h = past2({q.x, r.x}, h, {q.y, r.y});
+            for (int s = from; s < to; ++s, at += step) {
+                const float2 q = __ldcg(at), r = __ldcg(at + second);
+                B = past2({q.x, r.x}, B, {q.y, r.y});
+                A = mul2({q.x, r.x}, A);
+            }
         }
+        shared += group * p.warps * 32;
+        shared[me * p.lanes + cl] = make_float4(A.x, A.y, B.x, B.y);
+        unit_sync(p);
+        for (int w = 0; w < workers && w * per < n; ++w) {
+            const float4 q = shared[w * p.lanes + cl];
+            h = past2({q.x, q.y}, h, {q.z, q.w});
+        }
+        unit_sync(p);
         return h;
     }
     __device__ __forceinline__ void unit_sync(const ScanArgs& p) const {
@@ -540,7 +557,7 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
         copies_issued();
     };
     for (int i = 0; i < p.stages - 1; ++i) issue();
-    F2 carry = MODE == 0 ? th.ranges(p, pairs, th.start(p), false) : two(0.f);
+    F2 carry = MODE == 0 ? th.ranges(p, pairs, th.start(p), false, &s_pair[0][0][0]) : two(0.f);
     F2 through = two(1.f);              // MODE 1, 2: with carry, the pair so far
     VT* out = states == nullptr ? nullptr
         : states + (th.row.first + th.place(p, first * th.chunk + th.step0)) * p.C + th.ch;
@@ -738,7 +755,7 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
     const float* keep = kept + kept_index(p, th.row, th.b, th.chunk, first) * p.C + th.ch;
     F2 h_next = n > 0 ? th.get(keep) : two(0.f);
     F2 R = d_last != nullptr ? th.get(d_last + th.b * p.C + th.ch) : two(0.f);
-    R = th.ranges(p, pairs, R, true);   // what flows back into the last state of the tile
+    R = th.ranges(p, pairs, R, true, &s_pair[0][0][0]);     // what flows back into the last state of the tile
     // (outputs are written from a stretch's last step to its first)
     const int64_t out0 = th.row.first + th.place(p, first * th.chunk + th.step0 + L - 1);
     VT* to_x = dx == nullptr ? nullptr : dx + out0 * p.C + th.ch;
