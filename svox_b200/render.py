@@ -14,6 +14,8 @@ from torch import autograd, nn
 
 from . import csrc as _C
 from .formats import DataFormat
+from .recurrence import composite
+from .sh import eval_sh_bases
 
 __all__ = ["VolumeRenderer", "NDCConfig", "Rays", "_VolumeRenderFunction",
            "_VolumeRenderImageFunction"]
@@ -285,6 +287,56 @@ class VolumeRenderer(nn.Module):
             fy = fx
         c2w = c2w.to(dtype=self.tree.data.dtype, device=self.tree.data.device).contiguous()
         return self._render(_make_camera_spec(c2w, width, height, fx, fy), fast, True)
+
+    def render_samples(self, rays: Rays, depths, lengths, offsets=None, cache=None):
+        """Render rays from samples that the caller has placed -> ``(B, rgb_dim)``.
+
+        ``depths`` holds the distances of the samples from the rays' origins, in units of ``dirs``
+        and from the nearest to the farthest, and ``lengths`` what each stands for (its thickness is
+        the density there times its length): both ``(B, T)``, or ``(N,)`` with ``offsets``
+        ``(B + 1,)`` int64 for rays of any number of samples.  The records are looked up in the tree
+        -- differentiable w.r.t. ``tree.data`` and ``lengths`` -- or in ``cache``, a
+        :class:`RecordCache` (no gradient w.r.t. records), and composited by :func:`composite`.
+        Densities, colours, ``min_comp`` / ``max_comp``, ``density_softplus``, ``rgb_padding`` and the
+        background are those of :meth:`forward`; thresholds, ``ndc`` and weight accumulation do not
+        apply.  RGBA and SH records.  (No counterpart in the reference, which samples by its march
+        alone, svox/csrc/rt_kernel.cu:222-321.)
+        """
+        self._require_cuda(True)
+        fmt, opt = self.data_format, self._get_options()
+        if fmt.format not in (DataFormat.RGBA, DataFormat.SH):
+            raise RuntimeError("render_samples takes RGBA and SH records")
+        B = rays.origins.shape[0]
+        if offsets is None:
+            if depths.dim() != 2 or depths.shape[0] != B or lengths.shape != depths.shape:
+                raise RuntimeError("depths and lengths must be (B, T)")
+            ray = torch.arange(B, device=depths.device)[:, None].expand_as(depths).reshape(-1)
+        else:
+            if depths.dim() != 1 or lengths.shape != depths.shape or offsets.numel() != B + 1:
+                raise RuntimeError("depths and lengths must be (N,) and offsets (B + 1,)")
+            steps = torch.arange(depths.shape[0], device=depths.device)
+            ray = (torch.searchsorted(offsets, steps, right=True) - 1).clamp(0, max(B - 1, 0))
+            if B == 0:
+                ray = ray[:0]
+        d = depths.detach().reshape(-1)
+        points = torch.addcmul(rays.origins[ray], d[:ray.numel(), None], rays.dirs[ray])
+        records = self.tree(points) if cache is None else cache(points)
+        sigma = records[:, -1]
+        sigma = nn.functional.softplus(sigma - 1.0) if self.density_softplus else sigma.relu()
+        rgb = records[:, :-1]
+        if fmt.format == DataFormat.SH:
+            n = fmt.basis_dim
+            basis = eval_sh_bases(int(round(n ** 0.5)) - 1, rays.viewdirs)
+            some = slice(opt.min_comp, opt.max_comp + 1)
+            rgb = (rgb.reshape(rgb.shape[0], rgb.shape[1] // n, n)[..., some] *
+                   basis[ray][:, None, some]).sum(dim=-1)
+        pad = self.rgb_padding
+        rgb = torch.sigmoid(rgb) * (1.0 + 2.0 * pad) - pad
+        background = torch.full((1,), self.background_brightness, device=rgb.device)
+        if offsets is None:
+            shape = (B, depths.shape[1])
+            return composite(rgb.reshape(*shape, rgb.shape[-1]), sigma.reshape(shape) * lengths, background)
+        return composite(rgb, sigma * lengths[:ray.numel()], background, offsets)
 
     def se_grad(self, rays: Rays, colors):
         """Rendered colour, gradient and Gauss-Newton diagonal of the total squared error
