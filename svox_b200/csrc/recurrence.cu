@@ -77,31 +77,47 @@ Plan make_plan(const svoxb_scan* s) {
     const size_t vs = type_size(s->values_type), gs = type_size(s->thickness_type);
     // (a lane's two channels share a gate, or have one each)
     plan.channel_gates = p.D == 1 || p.D % 2 != 0;
-    const int W = 64;
-    p.parts = 1;
-    int width;                      // of the widest tile
-    if (p.D == 1) width = p.C < W ? p.C : W;
-    else if (p.D <= W) width = p.C < W ? p.C : W / p.D * p.D;
-    else { p.parts = (p.D + W - 1) / W; width = W; }
-    p.lanes = 8;
-    while (p.lanes * 2 < width) p.lanes *= 2;
-    p.tile = width;
-    p.tiles = p.parts > 1 ? p.H * p.parts : (p.C + width - 1) / width;
-    p.units = p.B * p.tiles;
     // (rows of a packed call: as long as twice the average)
     const int64_t len = p.offsets ? (p.B > 0 ? (2 * p.T + p.B - 1) / p.B : 0) : p.T;
-    p.warps = 1;
-    while (p.warps < kScanWarps && p.warps * (32 / p.lanes) * kSteps < len) p.warps *= 2;
-    plan.chunk = p.warps * (32 / p.lanes) * kSteps;
-    const int per = kScanWarps / p.warps;
-    plan.blocks = (p.units + per - 1) / per;
+    auto tile = [&](int W) {
+        p.parts = 1;
+        if (p.D == 1) p.tile = p.C < W ? p.C : W;
+        else if (p.D <= W) p.tile = p.C < W ? p.C : W / p.D * p.D;
+        else { p.parts = (p.D + W - 1) / W; p.tile = W; }
+        p.lanes = 8;
+        while (p.lanes * 2 < p.tile) p.lanes *= 2;
+        p.tiles = p.parts > 1 ? p.H * p.parts : (p.C + p.tile - 1) / p.tile;
+        p.units = p.B * p.tiles;
+        p.warps = 1;
+        while (p.warps < kScanWarps && p.warps * (32 / p.lanes) * kSteps < len) p.warps *= 2;
+        plan.chunk = p.warps * (32 / p.lanes) * kSteps;
+        const int per = kScanWarps / p.warps;
+        plan.blocks = (p.units + per - 1) / per;
+        return (len + plan.chunk - 1) / plan.chunk;
+    };
+    // As wide tiles as give every multiprocessor a block; narrow ones, which have more steps to
+    // them, while a row is a few of them; else wide ones, and ranges of a row to several blocks,
+    // which costs a pass over the inputs beforehand.  Forward and backward together, us, wide tiles
+    // in ranges / narrow tiles without: 7 rows of 1001 steps of 333 channels 73 / 41, 16 of 512 of 256
+    // (4 groups) 46 / 24, 4 of 2048 of 512 51 / 49 (8 groups: 52 / 53), 1 of 4096 of 1024 57 / 88.
+    const int sms = sm_count();
+    int64_t chunks = 0;
+    for (int W = 64; W >= 16; W /= 2) {
+        chunks = tile(W);
+        if (plan.blocks >= sms) break;
+    }
     p.splits = 1;
-    const int64_t chunks = (len + plan.chunk - 1) / plan.chunk, want = 2 * (int64_t)sm_count();
-    if (plan.blocks > 0 && plan.blocks * 2 <= want && chunks >= 8) {
-        int64_t n = want / plan.blocks;
-        if (n > chunks / 4) n = chunks / 4;
-        if (n > 256) n = 256;
-        p.splits = (int)n;
+    if (plan.blocks > 0 && plan.blocks < sms && (plan.blocks * 2 < sms || chunks > 8)) {
+        const int64_t wide = tile(64);
+        if (wide >= 8) {
+            chunks = wide;
+            int64_t n = 2 * (int64_t)sms / plan.blocks;
+            if (n > chunks / 4) n = chunks / 4;
+            if (n > 256) n = 256;
+            p.splits = (int)n;
+        } else {
+            chunks = tile(16);
+        }
     }
     const int64_t tiles_of = (chunks + p.splits - 1) / p.splits;
     // (of 32-bit values two tiles under way fill as much of the shared memory)
