@@ -427,8 +427,13 @@ typedef struct {
     int32_t reverse;
     int32_t weighted;
     int32_t last_only;       /* no states are wanted, now or for the backward pass */
-    int32_t reserved_;
+    int32_t layout;          /* 0; for a backward pass svoxb_gated_scan_layout of its forward call */
 } svoxb_scan;
+
+/* How the forward call lays out `kept`, which depends on the addresses and strides of its arrays:
+ * a backward call whose arrays lie elsewhere gets it in `layout`.  1 asks for dense arrays (no
+ * strides of their own) on 16-byte boundaries, 8 for 16-bit types (else SVOXB_ERR_OPTION). */
+int32_t svoxb_gated_scan_layout(const svoxb_scan* scan);
 
 /* Floats that `kept` needs, bytes that `workspace` needs (-1: bad arguments). */
 int64_t svoxb_gated_scan_kept(const svoxb_scan* scan);

@@ -38,6 +38,7 @@ struct Library {
     X(item_log_used)                                                                            \
     X(volume_render_logged_clear) X(volume_render_image_logged_clear) X(log_is_sorted)          \
     X(gated_scan) X(gated_scan_backward) X(gated_scan_kept) X(gated_scan_workspace)             \
+    X(gated_scan_layout)                                                                        \
     X(records_read) X(records_write)                                                            \
     X(strerror) X(last_cuda_error)
 #define SVOXB_MEMBER(name) decltype(&svoxb_##name) name = nullptr;
@@ -652,6 +653,7 @@ Tensor dense_rows(const Tensor& t) {
 struct Scan {
     Tensor values, thickness, initial, offsets;
     bool reverse = false, weighted = false, states = true;
+    int32_t layout = 0;     // of what the forward kept
     svoxb_scan c{};
     void bind();
     std::vector<int64_t> last_shape() const { return {c.B, c.C}; }
@@ -694,6 +696,7 @@ void Scan::bind() {
     c.reverse = reverse;
     c.weighted = weighted;
     c.last_only = !states;
+    c.layout = layout;
 }
 
 Scan read_scan(const Tensor& values, const Tensor& thickness, const optional<Tensor>& initial,
@@ -766,6 +769,7 @@ class ScanNode : public torch::autograd::Function<ScanNode> {
                                                   std::shared_ptr<Scan> call) {
         ctx->set_materialize_grads(false);
         auto [states, last, kept] = run_scan(*call, true);
+        call->layout = lib.gated_scan_layout(&call->c);
         ctx->save_for_backward(
             {values, thickness, initial ? *initial : Tensor(), call->offsets, kept});
         torch::autograd::variable_list out;
@@ -783,6 +787,15 @@ class ScanNode : public torch::autograd::Function<ScanNode> {
         s.values = saved[0], s.thickness = saved[1], s.initial = saved[2], s.offsets = saved[3];
         const Tensor& kept = saved[4];
         s.bind();
+        // (a saved-tensor hook may hand back other tensors than it was given: what the forward kept
+        // is laid out for those)
+        svoxb_scan anew = s.c;
+        anew.layout = 0;
+        if (s.layout == 1 && lib.gated_scan_layout(&anew) != 1) {
+            s.values = s.values.clone(at::MemoryFormat::Contiguous);
+            s.thickness = s.thickness.clone(at::MemoryFormat::Contiguous);
+            s.bind();
+        }
         const c10::cuda::CUDAGuard guard(s.values.device());
         Tensor d_states, d_last;
         if (s.states && grads[0].defined()) d_states = grads[0].contiguous();

@@ -53,7 +53,8 @@ RayPlan ray_plan(const svoxb_scan* s) {
     const auto on = [](const void* ptr, int type) {
         return reinterpret_cast<uintptr_t>(ptr) % (type == SVOXB_TYPE_F32 ? 16 : 8) == 0;
     };
-    plan.quads = dense && on(s->values, s->values_type) && on(s->thickness, s->thickness_type);
+    plan.fits = dense && on(s->values, s->values_type) && on(s->thickness, s->thickness_type);
+    plan.quads = s->layout == 0 ? plan.fits : s->layout == 1;
     if (!plan.quads) {
         plan.lanes = mean <= kRayShort ? 8 : 32;
         return plan;

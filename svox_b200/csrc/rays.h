@@ -13,7 +13,7 @@ namespace svoxb {
 // neighbouring samples, and where there are more channels, lanes of a sample and channels of a lane.
 struct RayPlan {
     int lanes = 0;
-    bool quads = false;
+    bool quads = false, fits = true;    // (fits: the arrays lie as that takes them)
     int width = 0, share = 0;
 };
 RayPlan ray_plan(const svoxb_scan* s);

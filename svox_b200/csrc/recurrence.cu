@@ -32,6 +32,7 @@ int validate(const svoxb_scan* s) {
     // gates in 32 bits or in the values' type
     if (s->thickness_type != SVOXB_TYPE_F32 && s->thickness_type != s->values_type)
         return SVOXB_ERR_FORMAT;
+    if (s->layout < 0 || s->layout > 2) return SVOXB_ERR_OPTION;
     const bool any = s->B > 0 && s->T > 0;
     if (any && (!s->values || !s->thickness)) return SVOXB_ERR_NULL;
     if (s->B > 0x7fffffff || s->T > (1LL << 40) || s->C > (1 << 24)) return SVOXB_ERR_TOO_LARGE;
@@ -256,6 +257,11 @@ using namespace svoxb;
 
 extern "C" {
 
+int32_t svoxb_gated_scan_layout(const svoxb_scan* s) {
+    if (validate(s) != SVOXB_OK) return -1;
+    return ray_plan(s).quads ? 1 : 2;
+}
+
 int64_t svoxb_gated_scan_kept(const svoxb_scan* s) {
     if (validate(s) != SVOXB_OK) return -1;
     if (const RayPlan rays = ray_plan(s); rays.lanes) return ray_kept(s, rays);
@@ -281,7 +287,8 @@ int svoxb_gated_scan(const svoxb_scan* s, void* states, float* last, float* kept
     }
     const bool any_states = s->offsets ? s->T > 0 : s->B * s->T > 0;
     if (!last || (any_states && (states == nullptr) != (s->last_only != 0))) return SVOXB_ERR_NULL;
-    if (const RayPlan rays = ray_plan(s); rays.lanes)
+    if (const RayPlan rays = ray_plan(s); rays.quads && !rays.fits) return SVOXB_ERR_OPTION;
+    else if (rays.lanes)
         return ray_forward(s, rays, last, kept, str);
     Plan plan = make_plan(s);
     plan.p.paired = in_twos(plan, states, s->values_type);
@@ -312,6 +319,7 @@ int svoxb_gated_scan_backward(const svoxb_scan* s, const float* kept, const void
     }
     if (s->last_only && d_states) return SVOXB_ERR_OPTION;
     if (const RayPlan rays = ray_plan(s); rays.lanes) {
+        if (rays.quads && !rays.fits) return SVOXB_ERR_OPTION;
         if (ray_kept(s, rays) > 0 && !kept) return SVOXB_ERR_NULL;
         return ray_backward(s, rays, kept, d_last, d_values, d_thickness, d_initial, str);
     }

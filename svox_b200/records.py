@@ -68,6 +68,15 @@ class RecordCache(nn.Module):
         return (f"records={len(self)}, data_dim={self.data_dim}, dtype={self.dtype}, "
                 f"group={self.group}")
 
+    # What the bytes mean goes with them: a state of another kind of cache is refused.
+    def get_extra_state(self):
+        return {"data_dim": self.data_dim, "group": self.group, "dtype": str(self.dtype)}
+
+    def set_extra_state(self, state):
+        mine = self.get_extra_state()
+        if state != mine:
+            raise RuntimeError(f"the state is that of a record cache with {state}, this one has {mine}")
+
     def _write(self, where, points, values, offset, scaling):
         b = self._buffers
         if values.requires_grad and torch.is_grad_enabled():

@@ -222,11 +222,18 @@ def test_cache_is_a_snapshot(cuda_device):
         tree.data.data.zero_()
     tree.refine()
     assert torch.equal(cache(points), want)
-    other = svox.RecordCache(make_tree("SH4", cuda_device, refine=2, seed=9))
-    assert set(cache.state_dict()) == {"child", "offset", "invradius", "records"}
-    if other.child.shape == cache.child.shape:
-        other.load_state_dict(cache.state_dict())
-        assert torch.equal(other(points), want)
+    assert set(cache.state_dict()) == {"child", "offset", "invradius", "records", "_extra_state"}
+    same_shape = svox.RecordCache(make_tree("SH4", cuda_device, refine=2))
+    same_shape.write(torch.arange(50, device=cuda_device), torch.ones(50, 13, device=cuda_device))
+    same_shape.load_state_dict(cache.state_dict())
+    assert torch.equal(same_shape(points), want)
+    kind = svox.RecordCache(make_tree("SH4", cuda_device, refine=2), dtype=E4M3)
+    with pytest.raises(RuntimeError, match="record cache"):
+        kind.load_state_dict(cache.state_dict())
+    import copy
+    twin = copy.deepcopy(cache)
+    twin.set(points, want + 1)
+    assert torch.equal(cache(points), want)
     assert cache(points[:0]).shape == (0, 13)
     cache.set(points[:0], want[:0])
     cache.write(torch.zeros(0, dtype=torch.int64, device=cuda_device), want[:0])

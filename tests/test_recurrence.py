@@ -292,6 +292,11 @@ def test_strides_and_broadcasts(cuda_device):
             assert p.shape == q.shape and torch.equal(p, q)
         want = reference(x, g, state, None, False, False, d[0], d[1])
         close("states", outs[1][0], want["states"])
+        # one state for all rows: its gradient is summed over them (a rounding for each)
+        total = want["d_initial"][0].sum(0), want["d_initial"][1].sum(0) + \
+            want["d_initial"][0].abs().sum(0) * 3 * U
+        states, last = svox.gated_scan(*b[:2], initial=b[2])
+        close("d_initial", torch.autograd.grad([states, last], b[2], d)[0], total)
     # an unaligned gradient
     x = torch.randn(2, 30, 64, generator=gen).to(cuda_device, BF16).requires_grad_(True)
     g = torch.rand(2, 30, 64, generator=gen).to(cuda_device, BF16)
@@ -530,6 +535,46 @@ def test_bad_offsets_are_noticed(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C", [3, 32, 200])
+def test_saved_tensors_elsewhere(cuda_device, C):
+    """A backward pass run twice, and one whose saved tensors lie elsewhere than the forward's: off
+    their boundaries and back on them."""
+    gen = torch.Generator().manual_seed(8)
+    n = torch.tensor([30, 0, 77, 5, 1])
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), n.cumsum(0)]).to(cuda_device)
+    N = int(n.sum())
+    flat = torch.randn(N * C + 1, generator=gen).to(cuda_device)
+    gates = torch.rand(N + 1, generator=gen).to(cuda_device)
+    d = torch.randn(5, C, generator=gen).to(cuda_device)
+
+    def off(t):         # the same values, four bytes off a boundary
+        to = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        to[1:] = t.flatten()
+        return to[1:].view(t.shape)
+
+    def run(x, g, pack=None, unpack=None):
+        x, g = x.detach().requires_grad_(True), g.detach().requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(pack or (lambda t: t),
+                                                      unpack or (lambda t: t)):
+            out = svox.composite(x, g, offsets=offsets)
+        first = torch.autograd.grad(out, [x, g], d, retain_graph=True)
+        again = torch.autograd.grad(out, [x, g], d)
+        for p, q in zip(first, again):
+            assert torch.equal(p, q)
+        return [out.detach(), *first]
+
+    here, there = (flat[:-1].view(N, C), gates[:-1]), (flat[1:].view(N, C), gates[1:])
+    for x, g in (here, there):
+        ref = reference(x, g, None, offsets, True, False, None, d)
+        # (other addresses may mean another order of a sum over channels)
+        for hooks in ((None, None), (None, lambda t: off(t) if t.dtype == F32 else t),
+                      (None, lambda t: t.clone()), (lambda t: t.cpu(), lambda t: t.to(cuda_device))):
+            out = run(x, g, *hooks)
+            for name, got in zip(("last", "d_values", "d_thickness"), out):
+                close(name, got, ref[name])
+
+
+@pytest.mark.gpu
 def test_no_second_derivative_and_edits(cuda_device):
     x = torch.rand(2, 30, 3, device=cuda_device, requires_grad=True)
     g = torch.rand(2, 30, device=cuda_device, requires_grad=True)
@@ -584,7 +629,7 @@ def test_abi_refusals():
                     ("initial_row", C.c_int64), ("C", C.c_int32), ("H", C.c_int32),
                     ("values_type", C.c_int32), ("thickness_type", C.c_int32),
                     ("reverse", C.c_int32), ("weighted", C.c_int32),
-                    ("last_only", C.c_int32), ("reserved_", C.c_int32)]
+                    ("last_only", C.c_int32), ("layout", C.c_int32)]
 
     lib = csrc.library()
     lib.svoxb_gated_scan_kept.restype = lib.svoxb_gated_scan_workspace.restype = C.c_int64
@@ -601,6 +646,7 @@ def test_abi_refusals():
     assert call(values_type=3)[0] == 3 and call(thickness_type=1)[0] == 3
     assert call(T=1 << 41)[0] == 8
     assert call(last_only=0)[0] == 1                        # no states
+    assert call(layout=3)[0] == 4
     assert call(B=0)[0] == 0                                # nothing to do
     assert lib.svoxb_gated_scan(None, None, None, None, None, None) == 1
     s = call(H=3)[1]
