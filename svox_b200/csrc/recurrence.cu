@@ -145,12 +145,21 @@ int ready(Kernel kernel, size_t smem) {
     return blocks_per_sm(reinterpret_cast<const void*>(kernel), kScanBlock, smem, &per_sm);
 }
 
+// Whether a call is what the FULL kernels take.
+bool is_full(const Plan& plan, int d_bytes) {
+    const ScanArgs& p = plan.p;
+    return p.D == 1 && p.lanes == 32 && p.warps == kScanWarps && p.C % 64 == 0 && p.x_bytes == 16 &&
+           p.g_bytes == 16 && d_bytes == 16 && p.paired;
+}
+
 template <class VT, class GT, bool PC, int MODE>
 int launch_scan(const Plan& plan, const void* x, float2* pairs, void* states, float* last,
                 float* kept, cudaStream_t stream) {
     using S = ScanShape<VT, GT, PC>;
     const size_t smem = (size_t)kScanWarps * plan.p.stages * (S::kX + S::kG);
-    auto kernel = scan_kernel<VT, GT, PC, MODE>;
+    auto kernel = scan_kernel<VT, GT, PC, MODE, false>;
+    if constexpr (PC)
+        if (is_full(plan, 16)) kernel = scan_kernel<VT, GT, PC, MODE, true>;
     const int st = ready(kernel, smem);
     if (st) return st;
     kernel<<<dim3((unsigned)plan.blocks, plan.p.splits), kScanBlock, smem, stream>>>(
@@ -211,7 +220,9 @@ int run_backward(const Plan& plan, const float* kept, const void* d, const float
     if (two.p.stages > 2) two.p.stages = 2;
     const size_t smem = (size_t)kScanWarps * (two.p.stages * (2 * S::kX + S::kG) +
                                               (p.D > 1 ? S::kSum : 0));
-    auto kernel = scan_back_kernel<VT, GT, PC>;
+    auto kernel = scan_back_kernel<VT, GT, PC, false>;
+    if constexpr (PC)
+        if (is_full(two, d == nullptr ? 16 : p.d_bytes)) kernel = scan_back_kernel<VT, GT, PC, true>;
     const int st = ready(kernel, smem);
     if (st) return st;
     kernel<<<dim3((unsigned)plan.blocks, p.splits), kScanBlock, smem, stream>>>(

@@ -233,9 +233,15 @@ __device__ __forceinline__ void copies_wait(int younger) {
 }
 
 // A thread's place: its unit, its steps within a tile, its channels.
-template <class VT, class GT, bool PC>
+// FULL: units of 32 lanes and all warps, rows copied 16 bytes at a time, a gate for each channel:
+// what every large call of plain arrays is, without the arithmetic on its shape (%FULL%).
+template <class VT, class GT, bool PC, bool FULL>
 struct ScanThread {
     using S = ScanShape<VT, GT, PC>;
+    static __device__ __forceinline__ int lanes_of(const ScanArgs& p) { return FULL ? 32 : p.lanes; }
+    static __device__ __forceinline__ int warps_of(const ScanArgs& p) {
+        return FULL ? kScanWarps : p.warps;
+    }
     int lane, warp, group, wseg;    // wseg: the warp's number in its unit
     int sub, cl, chunk;
     int64_t b;
@@ -251,23 +257,23 @@ struct ScanThread {
     __device__ __forceinline__ bool init(const ScanArgs& p) {
         lane = threadIdx.x & 31;
         warp = threadIdx.x >> 5;
-        group = warp / p.warps;
-        wseg = warp - group * p.warps;
+        group = warp / warps_of(p);
+        wseg = warp - group * warps_of(p);
         split = blockIdx.y;
-        const int64_t unit = (int64_t)blockIdx.x * (kScanWarps / p.warps) + group;
+        const int64_t unit = (int64_t)blockIdx.x * (kScanWarps / warps_of(p)) + group;
         if (unit >= p.units) return false;
         b = unit / p.tiles;
         tile = scan_tile(p, (int)(unit - b * p.tiles));
         row = scan_row(p, b);
-        sub = lane / p.lanes;
-        cl = lane - sub * p.lanes;
+        sub = lane / lanes_of(p);
+        cl = lane - sub * lanes_of(p);
         have = tile.width - cl * 2;
-        have = have < 0 ? 0 : have < 2 ? have : 2;
+        have = FULL || have >= 2 ? 2 : have < 0 ? 0 : have;
         ch = tile.first + (have ? cl * 2 : 0);
         const int heads = p.parts > 1 ? 1 : p.D > 1 ? tile.width / p.D : 0;
         gate = PC ? 0 : sub * heads + (p.parts > 1 ? 0 : have ? cl * 2 / p.D : 0);
-        step0 = (wseg * (32 / p.lanes) + sub) * kSteps;
-        chunk = p.warps * (32 / p.lanes) * kSteps;
+        step0 = (wseg * (32 / lanes_of(p)) + sub) * kSteps;
+        chunk = warps_of(p) * (32 / lanes_of(p)) * kSteps;
         const int64_t chunks = (row.len + chunk - 1) / chunk;
         const int64_t per = (chunks + p.splits - 1) / p.splits;
         k0 = per * split < chunks ? per * split : chunks;
@@ -289,13 +295,13 @@ struct ScanThread {
                                                 int64_t step, int room) const {
         constexpr int n = BYTES / (int)sizeof(T);           // elements of a piece
         constexpr int P = 32 * W / n, COLS = P < 32 ? P : 32, ROWS = 32 / COLS;
-        const int each = p.lanes * W;                       // elements of a row of channels
+        const int each = lanes_of(p) * W;                       // elements of a row of channels
 #pragma unroll
         for (int half = 0; half < P; half += COLS) {
             const int j = (half + lane % COLS) * n;
             const int s = j >> (31 - __clz(each)), c = j & (each - 1);
             if (c >= tile.width) continue;
-            int t = (wseg * (32 / p.lanes) + s) * kSteps + lane / COLS;
+            int t = (wseg * (32 / lanes_of(p)) + s) * kSteps + lane / COLS;
             const T* src = from + t * step + c;
             T* dst = to + lane / COLS * 32 * W + j;
 #pragma unroll
@@ -324,16 +330,16 @@ struct ScanThread {
         int t;                  // the step of its first piece; none: none
         unsigned dst;
         __device__ __forceinline__ void init(const ScanArgs& p, const ScanThread& th, int64_t step) {
-            const int each = p.lanes * 2, j = th.lane % COLS * n;
+            const int each = lanes_of(p) * 2, j = th.lane % COLS * n;
             const int s = j >> (31 - __clz(each)), c = j & (each - 1);
-            const int t0 = (th.wseg * (32 / p.lanes) + s) * kSteps + th.lane / COLS;
+            const int t0 = (th.wseg * (32 / lanes_of(p)) + s) * kSteps + th.lane / COLS;
             off = t0 * step + c;
             down = ROWS * step;
             t = c < th.tile.width ? t0 : 1 << 30;
             dst = (unsigned)((th.lane / COLS * 64 + j) * sizeof(T));
         }
         __device__ __forceinline__ void copy(unsigned tile, const T* from, int room) const {
-            if (t >= 1 << 30) return;
+            if (!FULL && t >= 1 << 30) return;
             const T* src = from + off;
 #pragma unroll
             for (int l = 0; l < kSteps; l += ROWS, src += down) {
@@ -353,9 +359,9 @@ struct ScanThread {
             return;
         }
         // one gate for several channels: once each, or (PC) for every channel of the group
-        const int heads = p.parts > 1 ? 1 : tile.width / p.D, subs = 32 / p.lanes;
+        const int heads = p.parts > 1 ? 1 : tile.width / p.D, subs = 32 / lanes_of(p);
         const int width = PC ? tile.width : heads;
-        const int pitch = PC ? p.lanes * 2 : heads;
+        const int pitch = PC ? lanes_of(p) * 2 : heads;
         if (!PC && heads == 1) {
             const int t = wseg * subs * kSteps + lane;      // lane: step of sub lane / kSteps
             if (lane >= kSteps * subs) return;
@@ -380,7 +386,7 @@ struct ScanThread {
     }
     // What a tile never fills holds zeros: no thickness, no value.
     __device__ __forceinline__ void clear(const ScanArgs& p, unsigned char* mine, int bytes) const {
-        if (tile.width < p.lanes * 2)
+        if (!FULL && tile.width < lanes_of(p) * 2)
             for (int i = lane * 16; i < bytes; i += 512)
                 *reinterpret_cast<uint4*>(mine + i) = make_uint4(0, 0, 0, 0);
         __syncwarp();
@@ -427,7 +433,7 @@ struct ScanThread {
     // two neighbouring elements of an output row, as far as the tile goes
     template <class T>
     __device__ __forceinline__ void store(const ScanArgs& p, T* to, F2 v) const {
-        if (p.paired) {
+        if (FULL || p.paired) {
             const float w[2] = {v.x, v.y};
             store_some<2>(to, w);
         } else {
@@ -442,7 +448,7 @@ struct ScanThread {
                                          float4* shared) const {
         if (p.splits == 1) return h;
         const int n = back ? p.splits - 1 - split : split;
-        const int subs = 32 / p.lanes, workers = p.warps * subs, me = wseg * subs + sub;
+        const int subs = 32 / lanes_of(p), workers = warps_of(p) * subs, me = wseg * subs + sub;
         const int per = (n + workers - 1) / workers;
         const int from = per * me < n ? per * me : n, to = from + per < n ? from + per : n;
         const float2* at = pairs + (b * p.splits + (back ? p.splits - 1 - from : from)) * p.C + ch;
@@ -457,19 +463,19 @@ struct ScanThread {
                 A = mul2({q.x, r.x}, A);
             }
         }
-        shared += group * p.warps * 32;
-        shared[me * p.lanes + cl] = make_float4(A.x, A.y, B.x, B.y);
+        shared += group * warps_of(p) * 32;
+        shared[me * lanes_of(p) + cl] = make_float4(A.x, A.y, B.x, B.y);
         unit_sync(p);
         for (int w = 0; w < workers && w * per < n; ++w) {
-            const float4 q = shared[w * p.lanes + cl];
+            const float4 q = shared[w * lanes_of(p) + cl];
             h = past2({q.x, q.y}, h, {q.z, q.w});
         }
         unit_sync(p);
         return h;
     }
     __device__ __forceinline__ void unit_sync(const ScanArgs& p) const {
-        if (p.warps == 1) __syncwarp();
-        else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(p.warps * 32) : "memory");
+        if (warps_of(p) == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(warps_of(p) * 32) : "memory");
     }
 };
 
@@ -507,11 +513,11 @@ __device__ __forceinline__ void join_lanes(int lanes, int lane, F2& A, F2& B, F2
 
 // MODE 0: states and the last one; 1: the pair (A, B) of the block's range; 2: the pair (A, E) of it
 // backwards, where E is what the range's own gradients `x` send back past its first step.
-template <class VT, class GT, bool PC, int MODE>
+template <class VT, class GT, bool PC, int MODE, bool FULL>
 __global__ void __launch_bounds__(kScanBlock, MODE == 0 ? 2 : 3)
 scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
             VT* __restrict__ states, float* __restrict__ last, float* __restrict__ kept) {
-    using Th = ScanThread<VT, GT, PC>;
+    using Th = ScanThread<VT, GT, PC, FULL>;
     using S = typename Th::S;
     constexpr int L = kSteps;
     constexpr bool BACK = MODE == 2;
@@ -535,7 +541,8 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
     typename Th::template Pieces<GT> pg;
     px.init(p, th, step_x);
     pg.init(p, th, step_g);
-    const bool whole_x = p.x_bytes == 16, whole_g = PC && p.D == 1 && p.g_bytes == 16;
+    const bool whole_x = FULL || p.x_bytes == 16;
+    const bool whole_g = FULL || (PC && p.D == 1 && p.g_bytes == 16);
     const unsigned shared = (unsigned)__cvta_generic_to_shared(mine);
     const int64_t next_x = (BACK ? -th.chunk : th.chunk) * step_x;
     const int64_t next_g = (BACK ? -th.chunk : th.chunk) * step_g;
@@ -543,10 +550,13 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
     auto issue = [&] {
         if (issued < n) {
             const int room = th.room(BACK ? first - issued : first + issued);
-            if (whole_x) px.copy(shared + slot_in, from_x, room);
-            else if (!BACK || x != nullptr)
+            if (BACK && x == nullptr) {
+            } else if (whole_x) {
+                px.copy(shared + slot_in, from_x, room);
+            } else {
                 th.template copy_rows<VT, 2>(p, reinterpret_cast<VT*>(mine + slot_in), from_x, step_x,
                                              room, p.x_bytes);
+            }
             if (whole_g) pg.copy(shared + slot_in + S::kX, from_g, room);
             else th.copy_gates(p, reinterpret_cast<GT*>(mine + slot_in + S::kX), from_g, step_g, room);
             from_x += next_x;
@@ -619,9 +629,9 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
             keep += p.C;
         }
         F2 TA, TB;
-        join_lanes<BACK>(p.lanes, th.lane, A, B, TA, TB);
+        join_lanes<BACK>(Th::lanes_of(p), th.lane, A, B, TA, TB);
         F2 h = carry;
-        if (p.warps == 1) {
+        if (Th::warps_of(p) == 1) {
             carry = past2(TA, carry, TB);
             if (MODE != 0) through = mul2(through, TA);
         } else {
@@ -629,10 +639,10 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
             if (th.sub == 0) pair[th.warp][th.cl] = make_float4(TA.x, TA.y, TB.x, TB.y);
             th.unit_sync(p);
             const F2 before = carry;
-            const float4* const all = &pair[th.group * p.warps][th.cl];
+            const float4* const all = &pair[th.group * Th::warps_of(p)][th.cl];
 #pragma unroll 8
-            for (int j = 0; j < p.warps; ++j) {
-                const int w = BACK ? p.warps - 1 - j : j;
+            for (int j = 0; j < Th::warps_of(p); ++j) {
+                const int w = BACK ? Th::warps_of(p) - 1 - j : j;
                 if (w == th.wseg) h = carry;
                 const float4 q = all[w * 32];
                 carry = fma2({q.x, q.y}, carry, {q.z, q.w});
@@ -640,8 +650,8 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
             }
             if (spoilt(carry, carry) != 0.f) {
                 carry = before;
-                for (int j = 0; j < p.warps; ++j) {
-                    const int w = BACK ? p.warps - 1 - j : j;
+                for (int j = 0; j < Th::warps_of(p); ++j) {
+                    const int w = BACK ? Th::warps_of(p) - 1 - j : j;
                     if (w == th.wseg) h = carry;
                     const float4 q = all[w * 32];
                     carry = past2({q.x, q.y}, carry, {q.z, q.w});
@@ -649,7 +659,7 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
             }
         }
         if (MODE == 0 && out != nullptr) {
-            if (p.lanes < 32) h = past2(A, h, B);
+            if (Th::lanes_of(p) < 32) h = past2(A, h, B);
             odd |= spoilt(h, h) != 0.f;
             const int64_t t0 = (first + i) * th.chunk + th.step0;
             VT* to = out;
@@ -683,18 +693,18 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
     }
     if (MODE == 0 && th.split == 0)
         clear_uncovered(p, th.b, th.tile.first, th.tile.width, (int64_t)p.C, states,
-                        th.wseg * 32 + th.lane, p.warps * 32);
+                        th.wseg * 32 + th.lane, Th::warps_of(p) * 32);
 }
 
 // The backward pass of a tile.  `parted`: (parts, steps, H) floats for the sums of a group that
 // several tiles share.
-template <class VT, class GT, bool PC>
+template <class VT, class GT, bool PC, bool FULL>
 __global__ void __launch_bounds__(kScanBlock, 2)
 scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict__ pairs,
                  const float* __restrict__ kept, const VT* __restrict__ d,
                  const float* __restrict__ d_last, VT* __restrict__ dx, GT* __restrict__ dg,
                  float* __restrict__ parted, float* __restrict__ dh0) {
-    using Th = ScanThread<VT, GT, PC>;
+    using Th = ScanThread<VT, GT, PC, FULL>;
     using S = typename Th::S;
     constexpr int L = kSteps;
     extern __shared__ __align__(16) unsigned char s_tiles[];
@@ -722,8 +732,8 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
     px.init(p, th, step_x);
     pd.init(p, th, step_c);
     pg.init(p, th, step_g);
-    const bool whole_x = p.x_bytes == 16, whole_d = p.d_bytes == 16;
-    const bool whole_g = PC && p.D == 1 && p.g_bytes == 16;
+    const bool whole_x = FULL || p.x_bytes == 16, whole_d = FULL || p.d_bytes == 16;
+    const bool whole_g = FULL || (PC && p.D == 1 && p.g_bytes == 16);
     const unsigned shared = (unsigned)__cvta_generic_to_shared(mine);
     int issued = 0, slot_in = 0, slot = 0;      // (offsets of the tiles' places)
     auto issue = [&] {
@@ -759,8 +769,8 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
     // (outputs are written from a stretch's last step to its first)
     const int64_t out0 = th.row.first + th.place(p, first * th.chunk + th.step0 + L - 1);
     VT* to_x = dx == nullptr ? nullptr : dx + out0 * p.C + th.ch;
-    GT* to_g = dg == nullptr || p.D > 1 ? nullptr : dg + out0 * p.H + th.ch;
-    const bool summed = dg != nullptr && p.D > 1;
+    GT* to_g = dg == nullptr || (!FULL && p.D > 1) ? nullptr : dg + out0 * p.H + th.ch;
+    const bool summed = !FULL && dg != nullptr && p.D > 1;
     for (int i = 0; i < n; ++i) {
         const int64_t k = first - i;
         issue();
@@ -805,10 +815,10 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
             }
         }
         F2 EA = A, TA, TB, TE, all_a;
-        join_lanes<false>(p.lanes, th.lane, A, B, TA, TB);
-        join_lanes<true>(p.lanes, th.lane, EA, E, all_a, TE);
+        join_lanes<false>(Th::lanes_of(p), th.lane, A, B, TA, TB);
+        join_lanes<true>(Th::lanes_of(p), th.lane, EA, E, all_a, TE);
         F2 G = R;
-        if (p.warps == 1) {
+        if (Th::warps_of(p) == 1) {
             R = past2(TA, R, TE);
         } else {
             if (th.sub == 0) {
@@ -816,17 +826,17 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
                 s_flow[i & 1][th.warp][th.cl] = make_float2(TE.x, TE.y);
             }
             th.unit_sync(p);
-            const float4* const all = &s_pair[i & 1][th.group * p.warps][th.cl];
-            const float2* const flow = &s_flow[i & 1][th.group * p.warps][th.cl];
+            const float4* const all = &s_pair[i & 1][th.group * Th::warps_of(p)][th.cl];
+            const float2* const flow = &s_flow[i & 1][th.group * Th::warps_of(p)][th.cl];
             const F2 h_before = h, R_before = R;
 #pragma unroll 8
-            for (int j = 0; j < p.warps; ++j) {
+            for (int j = 0; j < Th::warps_of(p); ++j) {
                 if (j >= th.wseg) break;
                 const float4 q = all[j * 32];
                 h = fma2({q.x, q.y}, h, {q.z, q.w});
             }
 #pragma unroll 8
-            for (int j = p.warps - 1; j >= 0; --j) {
+            for (int j = Th::warps_of(p) - 1; j >= 0; --j) {
                 if (j == th.wseg) G = R;
                 const float2 a2 = *reinterpret_cast<const float2*>(&all[j * 32]), e2 = flow[j * 32];
                 R = fma2({a2.x, a2.y}, R, {e2.x, e2.y});
@@ -838,7 +848,7 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
                     const float4 q = all[j * 32];
                     h = past2({q.x, q.y}, h, {q.z, q.w});
                 }
-                for (int j = p.warps - 1; j >= 0; --j) {
+                for (int j = Th::warps_of(p) - 1; j >= 0; --j) {
                     if (j == th.wseg) G = R;
                     const float4 q = all[j * 32];
                     const float2 e2 = flow[j * 32];
@@ -846,13 +856,14 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
                 }
             }
         }
-        if (p.lanes < 32) {
+        if (Th::lanes_of(p) < 32) {
             h = past2(A, h, B);
             G = past2(EA, G, E);
         }
         odd |= spoilt(h, G) != 0.f;
         const int64_t t0 = k * th.chunk + th.step0;
-        const bool whole = t0 + L <= th.row.len;
+        const int mine = th.have == 0 || t0 >= th.row.len ? 0      // steps that this lane has
+                         : t0 + L <= th.row.len ? L : (int)(th.row.len - t0);
         // (dg of a step goes where it belongs, or to the sums of its group)
         auto give = [&](int l, bool in, F2 wG, F2 one) {
             if (dx != nullptr && in) th.store(p, to_x - (int64_t)(L - 1 - l) * step_c, wG);
@@ -880,7 +891,7 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
 #pragma unroll
             for (int l = L - 1; l >= 0; --l) {
                 if (d != nullptr) G = add2(G, th.at(td, l));
-                give(l, th.have && (whole || t0 + l < th.row.len), WEIGHTED ? G : mul2(w[l], G),
+                give(l, l < mine, WEIGHTED ? G : mul2(w[l], G),
                      mul2(q[l], G));
                 G = mul2(a[l], G);
             }
@@ -905,7 +916,7 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
                 if (wl.y == 0.f && !finite(v.y)) v.y = hb.y;
                 q.x = al.x == 0.f ? 0.f : al.x * (p.weighted ? -hb.x : v.x - hb.x);
                 q.y = al.y == 0.f ? 0.f : al.y * (p.weighted ? -hb.y : v.y - hb.y);
-                give(l, th.have && t0 + l < th.row.len, mul2(wl, G), mul2(q, G));
+                give(l, l < mine, mul2(wl, G), mul2(q, G));
                 G = past2(al, G, two(0.f));
             }
         } else if (p.weighted) {
@@ -917,11 +928,11 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
         if (to_g != nullptr) to_g -= (int64_t)th.chunk * step_h;
         if (summed) {
             __syncwarp();
-            const int heads = p.parts > 1 ? 1 : th.tile.width / p.D, subs = 32 / p.lanes;
+            const int heads = p.parts > 1 ? 1 : th.tile.width / p.D, subs = 32 / Th::lanes_of(p);
             const int tasks = L * subs * heads;
             // a sum's terms: channels (PC), or pairs of them
             const int width = (p.parts > 1 ? th.tile.width : p.D) / (PC ? 1 : 2);
-            const int row_of = PC ? p.lanes * 2 : p.lanes;
+            const int row_of = PC ? Th::lanes_of(p) * 2 : Th::lanes_of(p);
             // few sums: several lanes to each
             const int share = tasks < 32 && (tasks & (tasks - 1)) == 0 ? 32 / tasks : 1;
             for (int j0 = 0; j0 < tasks; j0 += 32 / share) {
@@ -951,7 +962,7 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
     if (th.split == 0) {
         if (th.wseg == 0 && th.sub == 0 && dh0 != nullptr)
             th.put(p, dh0 + th.b * p.C + th.ch, R);
-        const int thread = th.wseg * 32 + th.lane, threads = p.warps * 32;
+        const int thread = th.wseg * 32 + th.lane, threads = Th::warps_of(p) * 32;
         clear_uncovered(p, th.b, th.tile.first, th.tile.width, (int64_t)p.C, dx, thread, threads);
         const bool own_head = p.parts == 1 || th.tile.first == th.tile.head * p.D;
         if (own_head)

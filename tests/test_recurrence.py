@@ -141,7 +141,7 @@ def check_call(dev, x, g, initial, offsets, reverse, weighted, gen, with_states=
 
 
 # (B, T, C, H): one step to several stretches and splits, odd sizes, gates of all kinds
-SHAPES = [(1, 1, 1, 1), (3, 1, 5, 5), (2, 2, 3, 1), (2, 63, 33, 33), (1, 64, 64, 64), (3, 65, 66, 66),
+SHAPES = [(2, 200, 128, 128), (1, 3000, 64, 64), (1, 1, 1, 1), (3, 1, 5, 5), (2, 2, 3, 1), (2, 63, 33, 33), (1, 64, 64, 64), (3, 65, 66, 66),
           (2, 130, 7, 7), (1, 257, 48, 3), (2, 71, 96, 4), (1, 40, 200, 1), (2, 33, 130, 2),
           (5, 19, 34, 17), (1, 1500, 3, 1), (1, 1029, 70, 70), (40, 9, 16, 16), (2, 700, 1, 1),
           (3, 100, 12, 4)]
@@ -401,8 +401,10 @@ def test_masked_places(cuda_device, C):
 def test_partial_gradients(cuda_device):
     """Only some outputs used, only some inputs asked for."""
     gen = torch.Generator().manual_seed(4)
-    for C, H in ((66, 66), (3, 1), (96, 2)):
-        x, g = inputs(gen, (2, 90), C, H, F32, F32, cuda_device)
+    # (1500 and 2100 steps: ranges of a row in several blocks)
+    for C, H, T in ((66, 66, 90), (3, 1, 90), (96, 2, 90), (64, 64, 1500), (128, 128, 2100),
+                    (64, 1, 1500), (7, 1, 1500)):
+        x, g = inputs(gen, (2, T), C, H, F32, F32, cuda_device)
         s0 = torch.randn(2, C, generator=gen).to(cuda_device)
         check_call(cuda_device, x, g, s0, None, False, False, gen, with_last=False)
         check_call(cuda_device, x.detach(), g.detach(), s0.detach(), None, True, False, gen,
