@@ -103,7 +103,7 @@ Plan make_plan(const svoxb_scan* s) {
     // (4 groups) 46 / 24, 4 of 2048 of 512 51 / 49 (8 groups: 52 / 53), 1 of 4096 of 1024 57 / 88.
     const int sms = sm_count();
     int64_t chunks = 0;
-    for (int W = 64; W >= 16; W /= 2) {
+    for (const int W : {64, 16}) {
         chunks = tile(W);
         if (plan.blocks >= sms) break;
     }
@@ -145,11 +145,17 @@ int ready(Kernel kernel, size_t smem) {
     return blocks_per_sm(reinterpret_cast<const void*>(kernel), kScanBlock, smem, &per_sm);
 }
 
-// Whether a call is what the FULL kernels take.
-bool is_full(const Plan& plan, int d_bytes) {
+// Calls f with the lanes of a row where every tile of the call is whole (see ScanThread), else 0.
+template <class F>
+int with_lanes(const Plan& plan, int d_bytes, F f) {
     const ScanArgs& p = plan.p;
-    return p.D == 1 && p.lanes == 32 && p.warps == kScanWarps && p.C % 64 == 0 && p.x_bytes == 16 &&
-           p.g_bytes == 16 && d_bytes == 16 && p.paired;
+    const bool whole = p.warps == kScanWarps && p.tile == 2 * p.lanes && p.x_bytes == 16 &&
+                       d_bytes == 16 && p.paired &&
+                       (p.parts > 1 ? p.D : p.C) % p.tile == 0 &&
+                       (plan.channel_gates ? p.D == 1 && p.g_bytes == 16 : true);
+    if (whole && p.lanes == 32) return f(std::integral_constant<int, 32>{});
+    if (whole && p.lanes == 8) return f(std::integral_constant<int, 8>{});
+    return f(std::integral_constant<int, 0>{});
 }
 
 template <class VT, class GT, bool PC, int MODE>
@@ -157,15 +163,15 @@ int launch_scan(const Plan& plan, const void* x, float2* pairs, void* states, fl
                 float* kept, cudaStream_t stream) {
     using S = ScanShape<VT, GT, PC>;
     const size_t smem = (size_t)kScanWarps * plan.p.stages * (S::kX + S::kG);
-    auto kernel = scan_kernel<VT, GT, PC, MODE, false>;
-    if constexpr (PC)
-        if (is_full(plan, 16)) kernel = scan_kernel<VT, GT, PC, MODE, true>;
-    const int st = ready(kernel, smem);
-    if (st) return st;
-    kernel<<<dim3((unsigned)plan.blocks, plan.p.splits), kScanBlock, smem, stream>>>(
-        plan.p, static_cast<const VT*>(x), pairs, static_cast<VT*>(states), last, kept);
-    SVOXB_CUDA(cudaGetLastError());
-    return SVOXB_OK;
+    return with_lanes(plan, 16, [&](auto lanes) {
+        auto kernel = scan_kernel<VT, GT, PC, MODE, decltype(lanes)::value>;
+        const int st = ready(kernel, smem);
+        if (st) return st;
+        kernel<<<dim3((unsigned)plan.blocks, plan.p.splits), kScanBlock, smem, stream>>>(
+            plan.p, static_cast<const VT*>(x), pairs, static_cast<VT*>(states), last, kept);
+        SVOXB_CUDA(cudaGetLastError());
+        return (int)SVOXB_OK;
+    });
 }
 
 template <class VT, class GT, bool PC>
@@ -220,15 +226,17 @@ int run_backward(const Plan& plan, const float* kept, const void* d, const float
     if (two.p.stages > 2) two.p.stages = 2;
     const size_t smem = (size_t)kScanWarps * (two.p.stages * (2 * S::kX + S::kG) +
                                               (p.D > 1 ? S::kSum : 0));
-    auto kernel = scan_back_kernel<VT, GT, PC, false>;
-    if constexpr (PC)
-        if (is_full(two, d == nullptr ? 16 : p.d_bytes)) kernel = scan_back_kernel<VT, GT, PC, true>;
-    const int st = ready(kernel, smem);
+    const int st = with_lanes(two, d == nullptr ? 16 : p.d_bytes, [&](auto lanes) {
+        auto kernel = scan_back_kernel<VT, GT, PC, decltype(lanes)::value>;
+        const int bad = ready(kernel, smem);
+        if (bad) return bad;
+        kernel<<<dim3((unsigned)plan.blocks, p.splits), kScanBlock, smem, stream>>>(
+            two.p, static_cast<const VT*>(p.x), pairs, kept, static_cast<const VT*>(d), d_last,
+            static_cast<VT*>(dx), static_cast<GT*>(dg), parted, dh0);
+        SVOXB_CUDA(cudaGetLastError());
+        return (int)SVOXB_OK;
+    });
     if (st) return st;
-    kernel<<<dim3((unsigned)plan.blocks, p.splits), kScanBlock, smem, stream>>>(
-        two.p, static_cast<const VT*>(p.x), pairs, kept, static_cast<const VT*>(d), d_last,
-        static_cast<VT*>(dx), static_cast<GT*>(dg), parted, dh0);
-    SVOXB_CUDA(cudaGetLastError());
     if (p.parts > 1 && dg != nullptr) {
         scan_parts_kernel<GT><<<(unsigned)((plan.steps * p.H + 255) / 256), 256, 0, stream>>>(
             p, parted, static_cast<GT*>(dg));
