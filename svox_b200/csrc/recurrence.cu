@@ -41,7 +41,7 @@ int validate(const svoxb_scan* s) {
 
 struct Plan {
     ScanArgs p{};
-    bool channel_gates = false;     // a gate for each channel, or spread to one
+    bool channel_gates = false;     // a lane's two channels have a gate each
     int chunk = 1;                  // steps of a tile
     int64_t steps = 0;              // of all rows
     int64_t blocks = 0;
@@ -76,7 +76,7 @@ Plan make_plan(const svoxb_scan* s) {
     p.reverse = s->reverse; p.weighted = s->weighted;
     plan.steps = p.offsets ? p.T : p.B * p.T;
     const size_t vs = type_size(s->values_type), gs = type_size(s->thickness_type);
-    // (a lane's two channels share a gate, or have one each)
+    // (a lane's two channels share a gate, or have one each, of their own or of their groups)
     plan.channel_gates = p.D == 1 || p.D % 2 != 0;
     // (rows of a packed call: as long as twice the average)
     const int64_t len = p.offsets ? (p.B > 0 ? (2 * p.T + p.B - 1) / p.B : 0) : p.T;
@@ -99,8 +99,9 @@ Plan make_plan(const svoxb_scan* s) {
     // As wide tiles as give every multiprocessor a block; narrow ones, which have more steps to
     // them, while a row is a few of them; else wide ones, and ranges of a row to several blocks,
     // which costs a pass over the inputs beforehand.  Forward and backward together, us, wide tiles
-    // in ranges / narrow tiles without: 7 rows of 1001 steps of 333 channels 73 / 41, 16 of 512 of 256
-    // (4 groups) 46 / 24, 4 of 2048 of 512 51 / 49 (8 groups: 52 / 53), 1 of 4096 of 1024 57 / 88.
+    // in ranges / narrow tiles without: 7 rows of 1001 steps of 333 channels 72 / 40, 16 of 512 of 256
+    // (4 groups) 34 / 19, 4 of 2048 of 512 39 / 32 (8 groups: 41 / 38); with 64 narrow tiles instead of
+    // 148, 1 of 4096 of 1024, 57 / 88 (before whole tiles had kernels of their own).
     const int sms = sm_count();
     int64_t chunks = 0;
     for (const int W : {64, 16}) {

@@ -250,9 +250,10 @@ struct ScanThread {
     ScanRow row;
     int have;                // channels of this lane
     int ch;                  // its first channel
-    int gate;                // where its gate is in a row of a shared tile of gates
+    int gate, gate2;         // where the gates of its two are in a row of a tile of shared gates
     int step0;               // its first step within a tile
     int split;
+    bool one_each;           // a gate for each channel
     int64_t k0, k1;          // tiles of this block's range
 
     __device__ __forceinline__ bool init(const ScanArgs& p) {
@@ -261,6 +262,7 @@ struct ScanThread {
         group = warp / warps_of(p);
         wseg = warp - group * warps_of(p);
         split = blockIdx.y;
+        one_each = p.D == 1;
         const int64_t unit = (int64_t)blockIdx.x * (kScanWarps / warps_of(p)) + group;
         if (unit >= p.units) return false;
         b = unit / p.tiles;
@@ -272,7 +274,8 @@ struct ScanThread {
         have = LN || have >= 2 ? 2 : have < 0 ? 0 : have;
         ch = tile.first + (have ? cl * 2 : 0);
         const int heads = p.parts > 1 ? 1 : p.D > 1 ? tile.width / p.D : 0;
-        gate = PC ? 0 : sub * heads + (p.parts > 1 ? 0 : have ? cl * 2 / p.D : 0);
+        gate = sub * heads + (p.parts > 1 || !have ? 0 : cl * 2 / p.D);
+        gate2 = sub * heads + (p.parts > 1 || have < 2 ? 0 : (cl * 2 + 1) / p.D);
         step0 = (wseg * (32 / lanes_of(p)) + sub) * kSteps;
         chunk = warps_of(p) * (32 / lanes_of(p)) * kSteps;
         const int64_t chunks = (row.len + chunk - 1) / chunk;
@@ -359,28 +362,24 @@ struct ScanThread {
             copy_rows<GT, 2>(p, to, from, step, room, p.g_bytes);
             return;
         }
-        // one gate for several channels: once each, or (PC) for every channel of the group
+        // one gate for several channels: once each
         const int heads = p.parts > 1 ? 1 : tile.width / p.D, subs = 32 / lanes_of(p);
-        const int width = PC ? tile.width : heads;
-        const int pitch = PC ? lanes_of(p) * 2 : heads;
-        if (!PC && heads == 1) {
+        if (heads == 1) {
             const int t = wseg * subs * kSteps + lane;      // lane: step of sub lane / kSteps
             if (lane >= kSteps * subs) return;
             const bool in = t < room;
             const GT* src = in ? from + t * step : from;
-            GT* dst = to + (lane % kSteps) * 32 + lane / kSteps;
+            GT* dst = to + (lane % kSteps) * 32 * S::GV + lane / kSteps;
             if (sizeof(GT) == 4) copy_async(dst, src, 4, in);
             else *dst = in ? *src : from_float<GT>(0.f);
             return;
         }
-        for (int i = lane; i < kSteps * subs * width; i += 32) {
-            const int l = i / (subs * width), j = i - l * (subs * width);
-            const int s = j / width, c = j - s * width;
-            const int t = (wseg * subs + s) * kSteps + l;
+        for (int i = lane; i < kSteps * subs * heads; i += 32) {
+            const int l = i / (subs * heads), j = i - l * (subs * heads);
+            const int s = j / heads, t = (wseg * subs + s) * kSteps + l;
             const bool in = t < room;
-            const GT* src = in ? from + t * step + (PC ? (tile.first + c) / p.D - tile.head : c)
-                               : from;
-            GT* dst = to + l * 32 * S::GV + s * pitch + c;
+            const GT* src = in ? from + t * step + (j - s * heads) : from;
+            GT* dst = to + l * 32 * S::GV + j;
             if (sizeof(GT) == 4) copy_async(dst, src, 4, in);
             else *dst = in ? *src : from_float<GT>(0.f);
         }
@@ -397,7 +396,12 @@ struct ScanThread {
     __device__ __forceinline__ void gates(const GT* g, int l, F2& a, F2& w) const {
         if (PC) {
             float v[2];
-            load_some<2>(g + (l * 32 + lane) * 2, v);
+            if (LN || one_each) {
+                load_some<2>(g + (l * 32 + lane) * 2, v);
+            } else {
+                v[0] = to_float(g[l * 64 + gate]);
+                v[1] = to_float(g[l * 64 + gate2]);
+            }
             const F2 t{v[0], v[1]};
             a = decay2(t);
             w = WEIGHTED ? two(1.f) : weight2(t, a);
