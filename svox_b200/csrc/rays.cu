@@ -12,13 +12,17 @@ namespace svoxb {
 constexpr int64_t kRayLongest = 4096;
 // Up to this many a ray gets 8 lanes instead of 32, a sample each.
 constexpr int64_t kRayShort = 12;
-// By quads a ray gets 4 lanes, and twice as many beyond each of these averages.  Rays of 3 channels of
-// exponentially distributed lengths, forward and backward, us with 4 / 8 / 16 / 32 lanes:
-//   2^20 rays of 4: 177 / 298 / 557 / 1058, of 20: 422 / 459 / 631 / 1130, of 42: 744 / 712 / 809 / 1225;
-//   2^16 of 84: 172 / 124 / 101 / 111; 2^17 of 160: 585 / 400 / 300 / 285; 2^15 of 600: 859 / 533 / 357 / 268
-constexpr int64_t kQuadsMean[] = {28, 60, 130};
+// By quads a ray gets 4 lanes, and twice as many beyond each of these averages; a warp's window is four
+// times as many rays as it has groups of lanes (none for 32 lanes).  Rays of 3 channels of exponentially
+// distributed lengths, forward and backward, us with 4 / 8 / 16 lanes, and 32:
+//   2^20 rays of 4: 145 / 238 / 439 / 1189, of 20: 323 / 356 / 515 / 1262, of 42: 598 / 547 / 648 / 1344;
+//   2^16 of 84: 146 / 111 / 95 / 118; 2^17 of 160: 504 / 377 / 271 / 292; 2^15 of 600: 822 / 491 / 326 / 266
+// and without windows: of 42, 725 / 726 / 860.
+constexpr int64_t kQuadsMean[] = {28, 60, 240};
 // Lanes that all rays together can have at once; 4096 rays of 21, forward: 9.1 / 6.0 / 4.3 / 4.0 us.
 constexpr int64_t kQuadsFew = 1 << 17;
+// Warps that a window of rays has to leave.
+constexpr int64_t kWarpsBusy = 148 * 24;
 
 int status_of_rays(int clear, int* word) {
     SVOXB_CUDA(cudaMemcpyFromSymbol(word, g_status, sizeof(int)));
@@ -64,6 +68,9 @@ RayPlan ray_plan(const svoxb_scan* s) {
         if (mean > upto) plan.lanes *= 2;
     // few rays: as many lanes as leave none of them without a place
     while (plan.lanes < 32 && s->B * plan.lanes * 2 <= kQuadsFew) plan.lanes *= 2;
+    // (a ray to a warp ends when it ends)
+    const int groups = 32 / plan.lanes;
+    plan.window = groups > 1 && s->B / (4 * groups) >= kWarpsBusy ? 4 * groups : groups;
     return plan;
 }
 
@@ -136,6 +143,10 @@ void with_rows(const svoxb_scan* s, RayPlan plan, F f) {
 }
 
 unsigned blocks_of(const svoxb_scan* s, RayPlan plan) {
+    if (plan.quads) {
+        const int64_t warps = (s->B + plan.window - 1) / plan.window;
+        return (unsigned)((warps * 32 + kRayBlock - 1) / kRayBlock);
+    }
     return (unsigned)((s->B * plan.lanes + kRayBlock - 1) / kRayBlock);
 }
 
@@ -143,6 +154,7 @@ unsigned blocks_of(const svoxb_scan* s, RayPlan plan) {
 
 int ray_forward(const svoxb_scan* s, RayPlan plan, float* last, float* kept, cudaStream_t stream) {
     ScanArgs p = ray_args(s);
+    p.tile = plan.window;
     if (plan.width) {
         p.lanes = plan.width;
         with_rows(s, plan, [&](auto t, auto v, auto n) {
@@ -169,6 +181,7 @@ int ray_forward(const svoxb_scan* s, RayPlan plan, float* last, float* kept, cud
 int ray_backward(const svoxb_scan* s, RayPlan plan, const float* kept, const float* d_last, void* dx,
                  void* dg, float* dh0, cudaStream_t stream) {
     ScanArgs p = ray_args(s);
+    p.tile = plan.window;
     if (plan.width) {
         p.lanes = plan.width;
         p.paired = reinterpret_cast<uintptr_t>(dx) % 16 == 0;

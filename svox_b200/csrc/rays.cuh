@@ -125,8 +125,8 @@ ray_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restr
     float d[C], bg = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        d[c] = d_last != nullptr ? __ldg(d_last + th.b * C + c) : 0.f;
-        if (p.h0 != nullptr) bg = fmaf(d[c], __ldg(p.h0 + th.b * p.hb + c), bg);
+        d[c] = d_last != nullptr && th.there ? __ldg(d_last + th.b * C + c) : 0.f;
+        if (p.h0 != nullptr && th.there) bg = fmaf(d[c], __ldg(p.h0 + th.b * p.hb + c), bg);
     }
     // The values' gradients leave as one stretch: in its j-th store a lane has element j * G + lane,
     // of sample `whose[j]`.
@@ -199,7 +199,11 @@ ray_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restr
 }
 
 // ---------------------------------------------------------------------------
-// The same by quads.
+// The same by quads.  The rays of a warp's groups end together only if they are as long; so a warp
+// takes `window` rays, orders them by their lengths and goes through them, as many at a time as it
+// has groups.  For exponentially distributed lengths of 48 samples on average, four rays at a time
+// take 3.4 rounds of 32 samples as they come and 2.5 out of 16 (2^20 such rays with gradients: 726 ->
+// 547 us).
 
 template <class VT, class GT, int C, int G>
 struct RayQuads {
@@ -211,14 +215,38 @@ struct RayQuads {
     int chunks, most;
     int64_t rest;                   // samples of the array from the lane's first one on
 
-    __device__ __forceinline__ void init(const ScanArgs& p) {
+    // The warp's rays, by falling length.
+    struct Ray { int64_t first; int len, from; };
+    int64_t base;
+    const Ray* rays;
+    __device__ __forceinline__ void init(const ScanArgs& p, Ray (&shared)[kRayBlock]) {
+        const int me = threadIdx.x & 31;
         lane = threadIdx.x % G;
-        b = ((int64_t)blockIdx.x * kRayBlock + threadIdx.x) / G;
-        there = b < p.B;
-        if (!there) b = p.B - 1;
-        const ScanRow row = scan_row(p, b);
-        first = row.first;
-        len = there ? (int)row.len : 0;
+        base = ((int64_t)blockIdx.x * (kRayBlock / 32) + threadIdx.x / 32) * p.tile;
+        const bool here = me < p.tile && base + me < p.B;
+        const ScanRow row = scan_row(p, here ? base + me : p.B - 1);
+        const int len = here ? (int)row.len : -1;
+        int rank = me;
+        if (p.offsets != nullptr && p.tile > 32 / G) {
+            rank = 0;
+            for (int j = 0; j < p.tile; ++j) {
+                const int o = __shfl_sync(~0u, len, j);
+                rank += o > len || (o == len && j < me);
+            }
+        }
+        Ray* const all = shared + (threadIdx.x & ~31);
+        if (me < p.tile) all[rank] = Ray{row.first, len, me};
+        rays = all + (threadIdx.x & 31) / G;
+        __syncwarp();
+    }
+    // The group's ray of round r.
+    __device__ __forceinline__ void take(const ScanArgs& p, int r) {
+        const Ray ray = rays[r * (32 / G)];
+        b = base + ray.from;
+        first = ray.first;
+        len = ray.len;
+        there = len >= 0;
+        if (!there) len = 0;
         lead = (int)(first & 3);
         chunks = len > 0 ? (int)(((int64_t)lead + len + kChunk - 1) / kChunk) : 0;
         most = G == 32 ? chunks : __reduce_max_sync(~0u, chunks);
@@ -266,171 +294,178 @@ struct RayQuads {
 };
 
 template <class VT, class GT, int C, int G>
-__global__ void __launch_bounds__(kRayBlock, 24)
+__global__ void __launch_bounds__(kRayBlock, 20)
 quad_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
+    __shared__ typename RayQuads<VT, GT, C, G>::Ray s_rays[kRayBlock];
     RayQuads<VT, GT, C, G> th;
-    th.init(p);
+    th.init(p, s_rays);
     const VT* const x = static_cast<const VT*>(p.x);
     const GT* const g = static_cast<const GT*>(p.g);
-    float S = 0.f, acc[C];
+    for (int r = 0; r < p.tile / (32 / G); ++r) {
+        th.take(p, r);
+        float S = 0.f, acc[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] = 0.f;
-    float* const keep = kept != nullptr && th.lane == 0 ? kept + th.kept_at(p) : nullptr;
-    for (int k = 0; k < th.most; ++k) {
-        const int at = th.pos(k);
-        float gv[4] = {0.f, 0.f, 0.f, 0.f}, xv[4 * C];
-        if (at < th.len) {
-            const int64_t left = th.rest - (int64_t)k * th.kChunk;
-            th.template load<GT, 1>(g, at, left, gv);
-            th.template load<VT, C>(x, at, left, xv);
-        } else {
+        for (int c = 0; c < C; ++c) acc[c] = 0.f;
+        float* const keep = kept != nullptr && th.lane == 0 ? kept + th.kept_at(p) : nullptr;
+        for (int k = 0; k < th.most; ++k) {
+            const int at = th.pos(k);
+            float gv[4] = {0.f, 0.f, 0.f, 0.f}, xv[4 * C];
+            if (at < th.len) {
+                const int64_t left = th.rest - (int64_t)k * th.kChunk;
+                th.template load<GT, 1>(g, at, left, gv);
+                th.template load<VT, C>(x, at, left, xv);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4 * C; ++i) xv[i] = 0.f;
+                for (int i = 0; i < 4 * C; ++i) xv[i] = 0.f;
+            }
+            if (keep != nullptr && k < th.chunks) keep[k] = S;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) gv[i] = th.in(at + i) ? gv[i] : 0.f;
+            const float v = S + th.upto((gv[0] + gv[1]) + (gv[2] + gv[3]));
+            float before = __shfl_up_sync(~0u, v, 1, G);
+            if (th.lane == 0) before = S;
+            S = __shfl_sync(~0u, v, G - 1, G);
+            float T = decay_of(before);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = decay_of(gv[i]);
+                const float W = p.weighted ? (th.in(at + i) ? T : 0.f) : T * weight_of(gv[i], a);
+                if (W != 0.f)
+#pragma unroll
+                    for (int c = 0; c < C; ++c) acc[c] = fmaf(W, xv[i * C + c], acc[c]);
+                T *= a;
+            }
         }
-        if (keep != nullptr && k < th.chunks) keep[k] = S;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) gv[i] = th.in(at + i) ? gv[i] : 0.f;
-        const float v = S + th.upto((gv[0] + gv[1]) + (gv[2] + gv[3]));
-        float before = __shfl_up_sync(~0u, v, 1, G);
-        if (th.lane == 0) before = S;
-        S = __shfl_sync(~0u, v, G - 1, G);
-        float T = decay_of(before);
+        for (int d = G / 2; d > 0; d /= 2)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a = decay_of(gv[i]);
-            const float W = p.weighted ? (th.in(at + i) ? T : 0.f) : T * weight_of(gv[i], a);
-            if (W != 0.f)
+            for (int c = 0; c < C; ++c) acc[c] += __shfl_xor_sync(~0u, acc[c], d);
+        const float T = decay_of(S);
 #pragma unroll
-                for (int c = 0; c < C; ++c) acc[c] = fmaf(W, xv[i * C + c], acc[c]);
-            T *= a;
-        }
+        for (int c = 0; c < C; ++c)
+            if (th.lane == c && th.there) {
+                const float bg = p.h0 != nullptr ? __ldg(p.h0 + th.b * p.hb + c) : 0.f;
+                last[th.b * C + c] = past(T, bg, acc[c]);
+            }
     }
-#pragma unroll
-    for (int d = G / 2; d > 0; d /= 2)
-#pragma unroll
-        for (int c = 0; c < C; ++c) acc[c] += __shfl_xor_sync(~0u, acc[c], d);
-    if (!th.there) return;
-    const float T = decay_of(S);
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-        if (th.lane == c) {
-            const float bg = p.h0 != nullptr ? __ldg(p.h0 + th.b * p.hb + c) : 0.f;
-            last[th.b * C + c] = past(T, bg, acc[c]);
-        }
 }
 
 template <class VT, class GT, int C, int G>
-__global__ void __launch_bounds__(kRayBlock, 20)
+__global__ void __launch_bounds__(kRayBlock, 16)
 quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restrict__ d_last,
                  VT* __restrict__ dx, GT* __restrict__ dg, float* __restrict__ dh0) {
+    __shared__ typename RayQuads<VT, GT, C, G>::Ray s_rays[kRayBlock];
     RayQuads<VT, GT, C, G> th;
-    th.init(p);
+    th.init(p, s_rays);
     const VT* const x = static_cast<const VT*>(p.x);
     const GT* const g = static_cast<const GT*>(p.g);
-    float d[C], bg = 0.f;
+    for (int r = 0; r < p.tile / (32 / G); ++r) {
+        th.take(p, r);
+        float d[C], bg = 0.f;
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        d[c] = d_last != nullptr ? __ldg(d_last + th.b * C + c) : 0.f;
-        if (p.h0 != nullptr) bg = fmaf(d[c], __ldg(p.h0 + th.b * p.hb + c), bg);
-    }
-    const float* const keep = kept + th.kept_at(p);
-    float T_end = 1.f, behind = 0.f;        // what the samples behind the chunk bring
-    for (int k = th.most - 1; k >= 0; --k) {
-        const int at = th.pos(k);
-        const float S = k < th.chunks ? keep[k] : 0.f;
-        float gv[4] = {0.f, 0.f, 0.f, 0.f}, xv[4 * C];
-        if (at < th.len) {
-            const int64_t left = th.rest - (int64_t)k * th.kChunk;
-            th.template load<GT, 1>(g, at, left, gv);
-            th.template load<VT, C>(x, at, left, xv);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4 * C; ++i) xv[i] = 0.f;
+        for (int c = 0; c < C; ++c) {
+            d[c] = d_last != nullptr && th.there ? __ldg(d_last + th.b * C + c) : 0.f;
+            if (p.h0 != nullptr && th.there) bg = fmaf(d[c], __ldg(p.h0 + th.b * p.hb + c), bg);
         }
+        const float* const keep = kept + th.kept_at(p);
+        float T_end = 1.f, behind = 0.f;        // what the samples behind the chunk bring
+        for (int k = th.most - 1; k >= 0; --k) {
+            const int at = th.pos(k);
+            const float S = k < th.chunks ? keep[k] : 0.f;
+            float gv[4] = {0.f, 0.f, 0.f, 0.f}, xv[4 * C];
+            if (at < th.len) {
+                const int64_t left = th.rest - (int64_t)k * th.kChunk;
+                th.template load<GT, 1>(g, at, left, gv);
+                th.template load<VT, C>(x, at, left, xv);
+            } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) gv[i] = th.in(at + i) ? gv[i] : 0.f;
-        const float v = S + th.upto((gv[0] + gv[1]) + (gv[2] + gv[3]));
-        float before = __shfl_up_sync(~0u, v, 1, G);
-        if (th.lane == 0) before = S;
-        const float total = __shfl_sync(~0u, v, G - 1, G);
-        if (k == th.chunks - 1) {
-            T_end = decay_of(total);
-            behind = past(T_end, bg, 0.f);
-        }
-        float T = decay_of(before), W[4], c[4], Wc[4], own[4];
-        unsigned none = 0;          // samples that have no gradient of their thickness
+                for (int i = 0; i < 4 * C; ++i) xv[i] = 0.f;
+            }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            c[i] = 0.f;
-#pragma unroll
-            for (int q = 0; q < C; ++q) c[i] = fmaf(d[q], xv[i * C + q], c[i]);
-            const float a = decay_of(gv[i]);
-            W[i] = T * (p.weighted ? (th.in(at + i) ? 1.f : 0.f) : weight_of(gv[i], a));
-            Wc[i] = W[i] * c[i];
-            T *= a;
-            own[i] = p.weighted ? 0.f : T * c[i];
-        }
-        if (!finite((c[0] + c[1]) + (c[2] + c[3]))) {
-            // What is not finite counts only where it has weight; where there is no thickness it is
-            // no sample, and behind an opaque one neither.
+            for (int i = 0; i < 4; ++i) gv[i] = th.in(at + i) ? gv[i] : 0.f;
+            const float v = S + th.upto((gv[0] + gv[1]) + (gv[2] + gv[3]));
+            float before = __shfl_up_sync(~0u, v, 1, G);
+            if (th.lane == 0) before = S;
+            const float total = __shfl_sync(~0u, v, G - 1, G);
+            if (k == th.chunks - 1) {
+                T_end = decay_of(total);
+                behind = past(T_end, bg, 0.f);
+            }
+            float T = decay_of(before), W[4], c[4], Wc[4], own[4];
+            unsigned none = 0;          // samples that have no gradient of their thickness
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                Wc[i] = times(W[i], c[i]);
-                if (!finite(c[i]) && !p.weighted && (gv[i] == 0.f || W[i] == 0.f)) none |= 1u << i;
-            }
-        }
-        const float here = th.from((Wc[0] + Wc[1]) + (Wc[2] + Wc[3])) + behind;
-        float rest = __shfl_down_sync(~0u, here, 1, G);     // what all samples behind the quad bring
-        if (th.lane == G - 1) rest = behind;
-        behind = __shfl_sync(~0u, here, 0, G);
-        if (at < th.len) {
-            float out[4];
+                c[i] = 0.f;
 #pragma unroll
-            for (int i = 3; i >= 0; --i) {
-                out[i] = own[i] - rest;
-                rest += Wc[i];
+                for (int q = 0; q < C; ++q) c[i] = fmaf(d[q], xv[i * C + q], c[i]);
+                const float a = decay_of(gv[i]);
+                W[i] = T * (p.weighted ? (th.in(at + i) ? 1.f : 0.f) : weight_of(gv[i], a));
+                Wc[i] = W[i] * c[i];
+                T *= a;
+                own[i] = p.weighted ? 0.f : T * c[i];
             }
-            if (none)
+            if (!finite((c[0] + c[1]) + (c[2] + c[3]))) {
+                // What is not finite counts only where it has weight; where there is no thickness it is
+                // no sample, and behind an opaque one neither.
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (none >> i & 1) out[i] = 0.f;
-            const bool whole = at >= 0 && at + 3 < th.len;
-            const int64_t to = th.first + at;
-            if (dg != nullptr) {
-                if (whole && p.paired) store_some<4>(dg + to, out);
-                else
+                for (int i = 0; i < 4; ++i) {
+                    Wc[i] = times(W[i], c[i]);
+                    if (!finite(c[i]) && !p.weighted && (gv[i] == 0.f || W[i] == 0.f)) none |= 1u << i;
+                }
+            }
+            const float here = th.from((Wc[0] + Wc[1]) + (Wc[2] + Wc[3])) + behind;
+            float rest = __shfl_down_sync(~0u, here, 1, G);     // what all samples behind the quad bring
+            if (th.lane == G - 1) rest = behind;
+            behind = __shfl_sync(~0u, here, 0, G);
+            if (at < th.len) {
+                float out[4];
+#pragma unroll
+                for (int i = 3; i >= 0; --i) {
+                    out[i] = own[i] - rest;
+                    rest += Wc[i];
+                }
+                if (none)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (th.in(at + i)) dg[to + i] = from_float<GT>(out[i]);
-            }
-            if (dx != nullptr) {
-                if (whole && p.paired) {
-#pragma unroll
-                    for (int j = 0; j < C; ++j) {
-                        float q[4];
+                        if (none >> i & 1) out[i] = 0.f;
+                const bool whole = at >= 0 && at + 3 < th.len;
+                const int64_t to = th.first + at;
+                if (dg != nullptr) {
+                    if (whole && p.paired) store_some<4>(dg + to, out);
+                    else
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            q[i] = W[(4 * j + i) / C] * d[(4 * j + i) % C];
-                        store_some<4>(dx + to * C + 4 * j, q);
+                            if (th.in(at + i)) dg[to + i] = from_float<GT>(out[i]);
+                }
+                if (dx != nullptr) {
+                    if (whole && p.paired) {
+#pragma unroll
+                        for (int j = 0; j < C; ++j) {
+                            float q[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                q[i] = W[(4 * j + i) / C] * d[(4 * j + i) % C];
+                            store_some<4>(dx + to * C + 4 * j, q);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (th.in(at + i))
+#pragma unroll
+                                for (int c = 0; c < C; ++c)
+                                    dx[(to + i) * C + c] = from_float<VT>(W[i] * d[c]);
                     }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (th.in(at + i))
-#pragma unroll
-                            for (int c = 0; c < C; ++c)
-                                dx[(to + i) * C + c] = from_float<VT>(W[i] * d[c]);
                 }
             }
         }
-    }
-    if (!th.there) return;
-    if (dh0 != nullptr)
+        if (!th.there) continue;
+        if (dh0 != nullptr)
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (th.lane == c) dh0[th.b * C + c] = past(T_end, d[c], 0.f);
-    clear_uncovered(p, th.b, 0, C, (int64_t)C, dx, th.lane, G);
-    clear_uncovered(p, th.b, 0, 1, (int64_t)1, dg, th.lane, G);
+            for (int c = 0; c < C; ++c)
+                if (th.lane == c) dh0[th.b * C + c] = past(T_end, d[c], 0.f);
+        clear_uncovered(p, th.b, 0, C, (int64_t)C, dx, th.lane, G);
+        clear_uncovered(p, th.b, 0, 1, (int64_t)1, dg, th.lane, G);
+    }
 }
 
 // ---------------------------------------------------------------------------

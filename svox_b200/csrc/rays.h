@@ -15,6 +15,7 @@ struct RayPlan {
     int lanes = 0;
     bool quads = false, fits = true;    // (fits: the arrays lie as that takes them)
     int width = 0, share = 0;
+    int window = 0;             // rays that a warp orders by length (quads)
 };
 RayPlan ray_plan(const svoxb_scan* s);
 int64_t ray_kept(const svoxb_scan* s, RayPlan plan);

@@ -215,6 +215,54 @@ def test_composite(cuda_device, C, dtype, packed):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,mean", [(200_000, 5), (130_000, 40), (60_000, 80), (130_000, 0)])
+def test_many_rays(cuda_device, B, mean):
+    """So many rays that a warp orders a number of them by length; `mean` 0: 37 samples each.
+
+    Weights are at most 1 together and values at most 1.  A weight is off by 30 u (see above) and by
+    the roundings of the thickness in front of it, at most one for each of the 5 + len / 16 sums that it
+    is made of, S u each, where S exp(-S) is below 0.4; a gradient by as much times |d|, twice."""
+    gen = torch.Generator(device=cuda_device).manual_seed(B)
+    if mean:
+        n = (torch.empty(B, device=cuda_device).exponential_(1 / mean, generator=gen)).long()
+        n[torch.rand(B, device=cuda_device, generator=gen) < 0.2] = 0
+        offsets = torch.cat([n.new_zeros(1), n.cumsum(0)])
+        N, longest = int(offsets[-1]), int(n.max())
+    else:
+        N, longest = B * 37, 37
+        offsets = torch.arange(B + 1, device=cuda_device) * 37
+        n = offsets.diff()
+    x = torch.rand(N, 3, device=cuda_device, generator=gen)
+    g = torch.rand(N, device=cuda_device, generator=gen) ** 4 * 2
+    bg = torch.rand(B, 3, device=cuda_device, generator=gen)
+    d = torch.randn(B, 3, device=cuda_device, generator=gen)
+    leaves = [t.requires_grad_(True) for t in (x, g, bg)]
+    if mean:
+        out = svox.composite(*leaves, offsets)
+    else:
+        out = svox.composite(x.view(B, 37, 3), g.view(B, 37), bg)
+    got = torch.autograd.grad(out, leaves, d)
+    with torch.no_grad():
+        ray = torch.repeat_interleave(torch.arange(B, device=cuda_device), n)
+        upto = torch.cat([g.new_zeros(1).double(), g.double().cumsum(0)])
+        T = torch.exp(upto[offsets[:-1]][ray] - upto[:-1])
+        end = torch.exp(upto[offsets[:-1]] - upto[offsets[1:]])
+        w = T * -torch.expm1(-g.double())
+        total = torch.zeros(B, 3, dtype=torch.float64, device=cuda_device)
+        total.index_add_(0, ray, w[:, None] * x)
+        tol = (30 + 5 + longest / 16) * U
+        assert (out - (total + end[:, None] * bg)).abs().max() <= tol + U
+        c = (d.double()[ray] * x).sum(1)
+        wc = torch.cat([w.new_zeros(1), (w * c).cumsum(0)])
+        behind = wc[offsets[1:]][ray] - wc[1:] + (end * (d * bg).sum(1))[ray]
+        size = d.abs().sum(1).double()
+        assert ((got[0] - w[:, None] * d[ray]).abs() <= (tol + U) * d.abs()[ray]).all()
+        assert ((got[1] - (T * torch.exp(-g.double()) * c - behind)).abs() <=
+                2 * (tol + 3 * U) * size[ray] + N * 2.0 ** -52 * size.max()).all()
+        assert ((got[2] - end[:, None] * d).abs() <= (tol + U) * d.abs()).all()
+
+
+@pytest.mark.gpu
 def test_composite_is_emission_and_absorption(cuda_device):
     """The sum of what each sample emits, weighted by what reaches it."""
     gen = torch.Generator().manual_seed(0)
