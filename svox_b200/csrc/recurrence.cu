@@ -85,7 +85,7 @@ Plan make_plan(const svoxb_scan* s) {
         if (p.D == 1) p.tile = p.C < W ? p.C : W;
         else if (p.D <= W) p.tile = p.C < W ? p.C : W / p.D * p.D;
         else { p.parts = (p.D + W - 1) / W; p.tile = W; }
-        p.lanes = 8;
+        p.lanes = 1;
         while (p.lanes * 2 < p.tile) p.lanes *= 2;
         p.tiles = p.parts > 1 ? p.H * p.parts : (p.C + p.tile - 1) / p.tile;
         p.units = p.B * p.tiles;

@@ -365,13 +365,14 @@ struct ScanThread {
         // one gate for several channels: once each
         const int heads = p.parts > 1 ? 1 : tile.width / p.D, subs = 32 / lanes_of(p);
         if (heads == 1) {
-            const int t = wseg * subs * kSteps + lane;      // lane: step of sub lane / kSteps
-            if (lane >= kSteps * subs) return;
-            const bool in = t < room;
-            const GT* src = in ? from + t * step : from;
-            GT* dst = to + (lane % kSteps) * 32 * S::GV + lane / kSteps;
-            if (sizeof(GT) == 4) copy_async(dst, src, 4, in);
-            else *dst = in ? *src : from_float<GT>(0.f);
+            for (int i = lane; i < kSteps * subs; i += 32) {
+                const int t = wseg * subs * kSteps + i;     // step of sub i / kSteps
+                const bool in = t < room;
+                const GT* src = in ? from + t * step : from;
+                GT* dst = to + (i % kSteps) * 32 * S::GV + i / kSteps;
+                if (sizeof(GT) == 4) copy_async(dst, src, 4, in);
+                else *dst = in ? *src : from_float<GT>(0.f);
+            }
             return;
         }
         for (int i = lane; i < kSteps * subs * heads; i += 32) {
