@@ -1,13 +1,14 @@
 // Compositing of samples with few channels that share their thickness: the colours of rays.
 //
 // The last state of the recurrence (recurrence.cuh), back to front, is a sum from the front,
-//   out = sum of W[i] x[i] + T[n] background,   T[i] = exp(-(g[0] + ... + g[i-1])),  W[i] = T[i] w[i]
-// so a group of G lanes walks a ray, a sample to a lane, and scans nothing but the thickness; the
-// channels are summed in each lane and over the lanes at the end.  With d the upstream gradient and
+//   out = sum of W[i] x[i] + T[n] background,   T[i] = a[0] ... a[i-1],   W[i] = T[i] w[i]
+// so a group of G lanes walks a ray, a sample to a lane, and scans nothing but what reaches a sample
+// (its products: exp of a sum of thicknesses would be off by the sum's rounding, 4e-6 of a background
+// behind a thickness of 70); the channels are summed in each lane and over the lanes at the end.  With d the upstream gradient and
 // c[i] = d . x[i] the backward pass is
 //   dx[i] = W[i] d,   dg[i] = T[i+1] c[i] - (sum over j > i of W[j] c[j] + T[n] d . background)
 // one more scan of plain sums, from the far end, whatever the number of channels.  The forward keeps
-// the thickness in front of every G samples for it.
+// what reaches every G-th sample for it.
 //
 // Where the samples lie densely and on 16-byte boundaries (`quads`), a lane takes four neighbouring
 // ones, whose four thicknesses are one request and their 4 C values C more.  The quads are those of
@@ -25,6 +26,20 @@ namespace svoxb {
 
 constexpr int kRayBlock = 64;       // (rays differ in length: blocks of few wait for few)
 constexpr int kRayChannels = 4;     // of those whose channels are summed in every lane
+
+// a = exp(-g) and w = 1 - a for products of many a.  The hardware's power of two is off to one side
+// near 1, by about 1e-8, and so is the nearest float to log2(e): over 200 samples that made 2e-6 of
+// what reaches the background.  Near 1, a comes from the series of w, rounded to nearest, and log2(e)
+// in two parts.
+struct Gate { float a, w; };
+__device__ __forceinline__ Gate gate_of(float g) {
+    const float s = g * fmaf(g, fmaf(g, fmaf(g, fmaf(g, fmaf(g, -1.f / 720, 1.f / 120), -1.f / 24),
+                                            1.f / 6), -0.5f), 1.f);
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;"
+        : "=f"(e) : "f"(fmaf(g, -1.44269502162933349609375f, g * -1.92596299112662e-8f)));
+    return fabsf(g) < 0.25f ? Gate{1.f - s, s} : Gate{e, 1.f - e};
+}
 
 template <class VT, class GT, int C, int G>
 struct RayThread {
@@ -52,12 +67,12 @@ struct RayThread {
     __device__ __forceinline__ int64_t kept_at(const ScanArgs& p) const {
         return p.offsets ? first / G + b : b * ((p.T + G - 1) / G);
     }
-    // Sum over this lane and the ones before it, or behind it.
-    __device__ __forceinline__ float upto(float v) const {
+    // Product over this lane and the ones before it; sum over it and the ones behind it.
+    __device__ __forceinline__ float through(float v) const {
 #pragma unroll
         for (int d = 1; d < G; d *= 2) {
             const float o = __shfl_up_sync(~0u, v, d, G);
-            if (lane >= d) v += o;
+            if (lane >= d) v *= o;
         }
         return v;
     }
@@ -76,7 +91,7 @@ __global__ void __launch_bounds__(kRayBlock)
 ray_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
     RayThread<VT, GT, C, G> th;
     th.init(p);
-    float S = 0.f, acc[C];
+    float reach = 1.f, acc[C];          // what reaches the chunk
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = 0.f;
     const int64_t dx = G * p.xs, dg = G * p.gs;
@@ -91,13 +106,13 @@ ray_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
         left -= G;
         th.x += dx;
         th.g += dg;
-        if (keep != nullptr && in) *keep++ = S;
-        const float v = S + th.upto(gi);
-        float before = __shfl_up_sync(~0u, v, 1, G);
-        if (th.lane == 0) before = S;
-        S = __shfl_sync(~0u, v, G - 1, G);
-        const float T = decay_of(before);
-        const float W = p.weighted ? T : T * weight_of(gi, decay_of(gi));
+        if (keep != nullptr && in) *keep++ = reach;
+        const Gate gate = gate_of(gi);
+        const float v = reach * th.through(gate.a);
+        float T = __shfl_up_sync(~0u, v, 1, G);
+        if (th.lane == 0) T = reach;
+        reach = __shfl_sync(~0u, v, G - 1, G);
+        const float W = p.weighted ? T : T * gate.w;
         if (W != 0.f)
 #pragma unroll
             for (int c = 0; c < C; ++c) acc[c] = fmaf(W, xv[c], acc[c]);
@@ -107,12 +122,11 @@ ray_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[c] += __shfl_xor_sync(~0u, acc[c], d);
     if (!th.there) return;
-    const float T = decay_of(S);
 #pragma unroll
     for (int c = 0; c < C; ++c)
         if (th.lane == c) {
             const float bg = p.h0 != nullptr ? __ldg(p.h0 + th.b * p.hb + c) : 0.f;
-            last[th.b * C + c] = past(T, bg, acc[c]);
+            last[th.b * C + c] = past(reach, bg, acc[c]);
         }
 }
 
@@ -151,7 +165,7 @@ ray_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restr
     int left = th.len - (th.most - 1) * G;  // samples from the chunk's first on
     for (int k = th.most - 1; k >= 0; --k, left += G) {
         const bool in = th.lane < left;
-        const float S = left > 0 ? keep[k] : 0.f;
+        const float reach = left > 0 ? keep[k] : 1.f;
         const float gi = in ? to_float(*th.g) : 0.f;
         float xv[C], c = 0.f;
 #pragma unroll
@@ -160,16 +174,17 @@ ray_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restr
         for (int q = 0; q < C; ++q) c = fmaf(d[q], xv[q], c);
         th.x -= step_x;
         th.g -= step_g;
-        const float v = S + th.upto(gi);
-        float before = __shfl_up_sync(~0u, v, 1, G);
-        if (th.lane == 0) before = S;
+        const Gate gate = gate_of(gi);
+        const float v = reach * th.through(gate.a);
+        float T = __shfl_up_sync(~0u, v, 1, G);
+        if (th.lane == 0) T = reach;
         const float total = __shfl_sync(~0u, v, G - 1, G);
         if (left > 0 && left <= G) {        // the ray's last chunk
-            T_end = decay_of(total);
+            T_end = total;
             behind = past(T_end, bg, 0.f);
         }
-        const float a = decay_of(gi), T = decay_of(before), Tn = T * a;
-        const float w = p.weighted ? (in ? 1.f : 0.f) : weight_of(gi, a), W = T * w;
+        const float Tn = T * gate.a;
+        const float w = p.weighted ? (in ? 1.f : 0.f) : gate.w, W = T * w;
         const float here = th.from(times(W, c)) + behind;       // of this sample and all behind it
         float rest = __shfl_down_sync(~0u, here, 1, G);
         if (th.lane == G - 1) rest = behind;
@@ -275,11 +290,11 @@ struct RayQuads {
             for (int i = 0; i < 4 * N; ++i) v[i] = i < left * N ? to_float(from[i]) : 0.f;
         }
     }
-    __device__ __forceinline__ float upto(float v) const {
+    __device__ __forceinline__ float through(float v) const {
 #pragma unroll
         for (int d = 1; d < G; d *= 2) {
             const float o = __shfl_up_sync(~0u, v, d, G);
-            if (lane >= d) v += o;
+            if (lane >= d) v *= o;
         }
         return v;
     }
@@ -303,7 +318,7 @@ quad_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
     const GT* const g = static_cast<const GT*>(p.g);
     for (int r = 0; r < p.tile / (32 / G); ++r) {
         th.take(p, r);
-        float S = 0.f, acc[C];
+        float reach = 1.f, acc[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[c] = 0.f;
         float* const keep = kept != nullptr && th.lane == 0 ? kept + th.kept_at(p) : nullptr;
@@ -318,34 +333,36 @@ quad_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
 #pragma unroll
                 for (int i = 0; i < 4 * C; ++i) xv[i] = 0.f;
             }
-            if (keep != nullptr && k < th.chunks) keep[k] = S;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) gv[i] = th.in(at + i) ? gv[i] : 0.f;
-            const float v = S + th.upto((gv[0] + gv[1]) + (gv[2] + gv[3]));
-            float before = __shfl_up_sync(~0u, v, 1, G);
-            if (th.lane == 0) before = S;
-            S = __shfl_sync(~0u, v, G - 1, G);
-            float T = decay_of(before);
+            if (keep != nullptr && k < th.chunks) keep[k] = reach;
+            Gate gate[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float a = decay_of(gv[i]);
-                const float W = p.weighted ? (th.in(at + i) ? T : 0.f) : T * weight_of(gv[i], a);
+                gv[i] = th.in(at + i) ? gv[i] : 0.f;
+                gate[i] = gate_of(gv[i]);
+            }
+            const float v =
+                reach * th.through((gate[0].a * gate[1].a) * (gate[2].a * gate[3].a));
+            float T = __shfl_up_sync(~0u, v, 1, G);
+            if (th.lane == 0) T = reach;
+            reach = __shfl_sync(~0u, v, G - 1, G);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float W = p.weighted ? (th.in(at + i) ? T : 0.f) : T * gate[i].w;
                 if (W != 0.f)
 #pragma unroll
                     for (int c = 0; c < C; ++c) acc[c] = fmaf(W, xv[i * C + c], acc[c]);
-                T *= a;
+                T *= gate[i].a;
             }
         }
 #pragma unroll
         for (int d = G / 2; d > 0; d /= 2)
 #pragma unroll
             for (int c = 0; c < C; ++c) acc[c] += __shfl_xor_sync(~0u, acc[c], d);
-        const float T = decay_of(S);
 #pragma unroll
         for (int c = 0; c < C; ++c)
             if (th.lane == c && th.there) {
                 const float bg = p.h0 != nullptr ? __ldg(p.h0 + th.b * p.hb + c) : 0.f;
-                last[th.b * C + c] = past(T, bg, acc[c]);
+                last[th.b * C + c] = past(reach, bg, acc[c]);
             }
     }
 }
@@ -371,7 +388,7 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
         float T_end = 1.f, behind = 0.f;        // what the samples behind the chunk bring
         for (int k = th.most - 1; k >= 0; --k) {
             const int at = th.pos(k);
-            const float S = k < th.chunks ? keep[k] : 0.f;
+            const float reach = k < th.chunks ? keep[k] : 1.f;
             float gv[4] = {0.f, 0.f, 0.f, 0.f}, xv[4 * C];
             if (at < th.len) {
                 const int64_t left = th.rest - (int64_t)k * th.kChunk;
@@ -381,27 +398,31 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
 #pragma unroll
                 for (int i = 0; i < 4 * C; ++i) xv[i] = 0.f;
             }
+            Gate gate[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) gv[i] = th.in(at + i) ? gv[i] : 0.f;
-            const float v = S + th.upto((gv[0] + gv[1]) + (gv[2] + gv[3]));
-            float before = __shfl_up_sync(~0u, v, 1, G);
-            if (th.lane == 0) before = S;
+            for (int i = 0; i < 4; ++i) {
+                gv[i] = th.in(at + i) ? gv[i] : 0.f;
+                gate[i] = gate_of(gv[i]);
+            }
+            const float v =
+                reach * th.through((gate[0].a * gate[1].a) * (gate[2].a * gate[3].a));
+            float T = __shfl_up_sync(~0u, v, 1, G);
+            if (th.lane == 0) T = reach;
             const float total = __shfl_sync(~0u, v, G - 1, G);
             if (k == th.chunks - 1) {
-                T_end = decay_of(total);
+                T_end = total;
                 behind = past(T_end, bg, 0.f);
             }
-            float T = decay_of(before), W[4], c[4], Wc[4], own[4];
+            float W[4], c[4], Wc[4], own[4];
             unsigned none = 0;          // samples that have no gradient of their thickness
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 c[i] = 0.f;
 #pragma unroll
                 for (int q = 0; q < C; ++q) c[i] = fmaf(d[q], xv[i * C + q], c[i]);
-                const float a = decay_of(gv[i]);
-                W[i] = T * (p.weighted ? (th.in(at + i) ? 1.f : 0.f) : weight_of(gv[i], a));
+                W[i] = T * (p.weighted ? (th.in(at + i) ? 1.f : 0.f) : gate[i].w);
                 Wc[i] = W[i] * c[i];
-                T *= a;
+                T *= gate[i].a;
                 own[i] = p.weighted ? 0.f : T * c[i];
             }
             if (!finite((c[0] + c[1]) + (c[2] + c[3]))) {
@@ -498,7 +519,7 @@ row_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
     RayRows<VT, GT, V, NT> rows;
     th.init(p);
     rows.init(p);
-    float S = 0.f, acc[NT][V];
+    float reach = 1.f, acc[NT][V];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -511,13 +532,13 @@ row_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
         const float gi = g_next;
         th.g += 32 * p.gs;
         g_next = th.lane + 32 < left ? to_float(*th.g) : 0.f;
-        if (keep != nullptr) keep[k] = S;
-        const float v = S + th.upto(gi);
-        float before = __shfl_up_sync(~0u, v, 1);
-        if (th.lane == 0) before = S;
-        S = __shfl_sync(~0u, v, 31);
-        const float T = decay_of(before);
-        const float W = p.weighted ? T : T * weight_of(gi, decay_of(gi));
+        if (keep != nullptr) keep[k] = reach;
+        const Gate gate = gate_of(gi);
+        const float v = reach * th.through(gate.a);
+        float T = __shfl_up_sync(~0u, v, 1);
+        if (th.lane == 0) T = reach;
+        reach = __shfl_sync(~0u, v, 31);
+        const float W = p.weighted ? T : T * gate.w;
         const int n = left < 32 ? (left + rows.per - 1) / rows.per : rows.width;
 #pragma unroll 4
         for (int j = 0; j < n; ++j) {
@@ -543,7 +564,6 @@ row_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int q = 0; q < V; ++q) acc[t][q] += __shfl_xor_sync(~0u, acc[t][q], d);
-    const float T = decay_of(S);
     if (rows.sub == 0)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -552,7 +572,7 @@ row_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
                 for (int q = 0; q < V; ++q) {
                     const int c = rows.ch(t) + q;
                     const float bg = p.h0 != nullptr ? __ldg(p.h0 + th.b * p.hb + c) : 0.f;
-                    last[th.b * p.C + c] = past(T, bg, acc[t][q]);
+                    last[th.b * p.C + c] = past(reach, bg, acc[t][q]);
                 }
 }
 
@@ -581,7 +601,7 @@ row_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restr
     for (int k = th.chunks - 1; k >= 0; --k) {
         const int left = th.len - 32 * k;
         const bool in = th.lane < left;
-        const float S = keep[k];
+        const float reach = keep[k];
         const float gi = in ? to_float(th.g[(int64_t)k * 32 * p.gs]) : 0.f;
         const int n = left < 32 ? (left + rows.per - 1) / rows.per : rows.width;
         const VT* const x = th.x + ((int64_t)k * 32 + rows.sub - th.lane) * p.xs;
@@ -605,15 +625,16 @@ row_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restr
             part = __shfl_sync(~0u, part, (th.lane & (rows.per - 1)) * rows.width);
             if (th.lane / rows.per == j) c = part;
         }
-        const float v = S + th.upto(gi);
-        float before = __shfl_up_sync(~0u, v, 1);
-        if (th.lane == 0) before = S;
+        const Gate gate = gate_of(gi);
+        const float v = reach * th.through(gate.a);
+        float T = __shfl_up_sync(~0u, v, 1);
+        if (th.lane == 0) T = reach;
         if (k == th.chunks - 1) {
-            T_end = decay_of(__shfl_sync(~0u, v, 31));
+            T_end = __shfl_sync(~0u, v, 31);
             behind = past(T_end, bg, 0.f);
         }
-        const float a = decay_of(gi), T = decay_of(before), Tn = T * a;
-        const float w = p.weighted ? (in ? 1.f : 0.f) : weight_of(gi, a), W = T * w;
+        const float Tn = T * gate.a;
+        const float w = p.weighted ? (in ? 1.f : 0.f) : gate.w, W = T * w;
         const float here = th.from(times(W, c)) + behind;
         float rest = __shfl_down_sync(~0u, here, 1);
         if (th.lane == 31) rest = behind;
