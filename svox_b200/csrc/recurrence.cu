@@ -96,7 +96,8 @@ Plan make_plan(const svoxb_scan* s) {
         plan.blocks = (p.units + per - 1) / per;
         return (len + plan.chunk - 1) / plan.chunk;
     };
-    // As wide tiles as give every multiprocessor a block; narrow ones, which have more steps to
+    // As wide tiles as give every multiprocessor a block and some a second one (160 blocks: 137 us wide
+    // and 126 narrow, 88 and 74 with shared gates; 192: 138 and 143); narrow ones, which have more steps to
     // them, while a row is a few of them; else wide ones, and ranges of a row to several blocks,
     // which costs a pass over the inputs beforehand.  Forward and backward together, us, wide tiles
     // in ranges / narrow tiles without: 7 rows of 1001 steps of 333 channels 72 / 40, 16 of 512 of 256
@@ -106,7 +107,7 @@ Plan make_plan(const svoxb_scan* s) {
     int64_t chunks = 0;
     for (const int W : {64, 16}) {
         chunks = tile(W);
-        if (plan.blocks >= sms) break;
+        if (plan.blocks * 8 >= sms * 9) break;
     }
     p.splits = 1;
     if (plan.blocks > 0 && plan.blocks < sms && (plan.blocks * 2 < sms || chunks > 8)) {
