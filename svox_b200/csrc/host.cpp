@@ -1015,11 +1015,12 @@ PYBIND11_MODULE(_host, m) {
         });
     });
 
-    // -> (states, last), or (last,) without `states`
+    // -> (states, last), or without `states` the last one
     m.def("gated_scan", [](const Tensor& values, const Tensor& thickness,
                            const optional<Tensor>& initial, const optional<Tensor>& offsets,
-                           bool reverse, bool weighted, bool states, const char* state_name) {
-        return unlocked([&]() -> torch::autograd::variable_list {
+                           bool reverse, bool weighted, bool states,
+                           const char* state_name) -> py::object {
+        const torch::autograd::variable_list out = unlocked([&]() -> torch::autograd::variable_list {
             auto call = std::make_shared<Scan>(
                 read_scan(values, thickness, initial, offsets, state_name));
             call->reverse = reverse;
@@ -1037,6 +1038,8 @@ PYBIND11_MODULE(_host, m) {
             if (states) return {all, last};
             return {last};
         });
+        if (!states) return py::cast(out[0]);
+        return py::make_tuple(out[0], out[1]);
     });
 
     m.def("records_read", [](const Tensor& records, const Tensor& child, const Tensor& offset,

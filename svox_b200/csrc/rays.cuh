@@ -134,6 +134,8 @@ template <class VT, class GT, int C, int G>
 __global__ void __launch_bounds__(kRayBlock)
 ray_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restrict__ d_last,
                 VT* __restrict__ dx, GT* __restrict__ dg, float* __restrict__ dh0) {
+    clear_uncovered(p, C, dx);
+    clear_uncovered(p, 1, dg);
     RayThread<VT, GT, C, G> th;
     th.init(p);
     float d[C], bg = 0.f;
@@ -209,8 +211,6 @@ ray_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restr
 #pragma unroll
         for (int c = 0; c < C; ++c)
             if (th.lane == c) dh0[th.b * C + c] = past(T_end, d[c], 0.f);
-    clear_uncovered(p, th.b, 0, C, (int64_t)C, dx, th.lane, G);
-    clear_uncovered(p, th.b, 0, 1, (int64_t)1, dg, th.lane, G);
 }
 
 // ---------------------------------------------------------------------------
@@ -371,6 +371,8 @@ template <class VT, class GT, int C, int G>
 __global__ void __launch_bounds__(kRayBlock, 16)
 quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restrict__ d_last,
                  VT* __restrict__ dx, GT* __restrict__ dg, float* __restrict__ dh0) {
+    clear_uncovered(p, C, dx);
+    clear_uncovered(p, 1, dg);
     __shared__ typename RayQuads<VT, GT, C, G>::Ray s_rays[kRayBlock];
     RayQuads<VT, GT, C, G> th;
     th.init(p, s_rays);
@@ -484,8 +486,6 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
 #pragma unroll
             for (int c = 0; c < C; ++c)
                 if (th.lane == c) dh0[th.b * C + c] = past(T_end, d[c], 0.f);
-        clear_uncovered(p, th.b, 0, C, (int64_t)C, dx, th.lane, G);
-        clear_uncovered(p, th.b, 0, 1, (int64_t)1, dg, th.lane, G);
     }
 }
 
@@ -580,6 +580,8 @@ template <class VT, class GT, int V, int NT>
 __global__ void __launch_bounds__(kRayBlock)
 row_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restrict__ d_last,
                 VT* __restrict__ dx, GT* __restrict__ dg, float* __restrict__ dh0) {
+    clear_uncovered(p, p.C, dx);
+    clear_uncovered(p, 1, dg);
     RayThread<VT, GT, 1, 32> th;
     RayRows<VT, GT, V, NT> rows;
     th.init(p);
@@ -673,8 +675,6 @@ row_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restr
 #pragma unroll
                 for (int q = 0; q < V; ++q)
                     dh0[th.b * p.C + rows.ch(t) + q] = past(T_end, d[t][q], 0.f);
-    clear_uncovered(p, th.b, 0, p.C, (int64_t)p.C, dx, th.lane, 32);
-    clear_uncovered(p, th.b, 0, 1, (int64_t)1, dg, th.lane, 32);
 }
 
 }  // namespace svoxb

@@ -8,8 +8,8 @@
 //   (A, B) then (A', B')  ->  (A' A, A' B + B')
 // so a stretch is scanned from registers: every thread takes kSteps steps of its channels, the
 // warps of a unit take consecutive stretches, and what comes before a stretch is folded from the
-// stretches' pairs in shared memory, always in the order of the steps (one result, whatever the
-// launch).  The backward pass runs the same from the other end over
+// stretches' pairs in shared memory, always in the order of the steps, so that a call repeats to the
+// bit.  The backward pass runs the same from the other end over
 //   G[t] = d[t] + a[t+1] G[t+1],   dx = w G,   dg = sum over the group of a (x - h[t-1]) G
 // (-a h[t-1] G for weighted inputs) and finds h[t-1] again from x and g and the state at the start
 // of each stretch, which the forward kept in 32 bits: 10 instead of 12 bytes per 16-bit element,
@@ -41,7 +41,7 @@ struct ScanArgs {
     int32_t C, H, D;
     int64_t xb, xs, gb, gs, hb;
     int32_t reverse, weighted;
-    // tiles of channels: whole groups, or a part of one
+    // tiles of channels: whole groups, or a part of one (`tile` of rays by quads: a warp's window)
     int32_t tile, tiles, parts;
     int32_t lanes;           // lanes of a row of channels, a power of two (the others: later steps)
     int32_t warps;           // of a unit, a power of two
@@ -177,19 +177,19 @@ __device__ __forceinline__ F2 weight2(F2 g, F2 a) {
     return {fabsf(g.x) < 0.25f ? s.x : d.x, fabsf(g.y) < 0.25f ? s.y : d.y};
 }
 
-// Steps of a packed call that no row covers, before the first row and behind the last, get zeros.
+// Steps of a packed call that no row covers, before the first row and behind the last (a buffer that
+// is not full), get zeros: from all threads of the launch.
 template <class T>
-__device__ __forceinline__ void clear_uncovered(const ScanArgs& p, int64_t b, int first, int width,
-                                                int64_t row_len, T* out, int thread, int threads) {
+__device__ __forceinline__ void clear_uncovered(const ScanArgs& p, int64_t row_len, T* out) {
     if (p.offsets == nullptr || out == nullptr) return;
-    for (int end = 0; end < 2; ++end) {
-        if (b != (end ? p.B - 1 : 0)) continue;
-        const int64_t at = __ldg(p.offsets + (end ? p.B : 0));
-        const int64_t cut = at < 0 ? 0 : at > p.T ? p.T : at;
-        const int64_t from = end ? cut : 0, to = end ? p.T : cut;
-        for (int64_t i = thread; i < (to - from) * width; i += threads)
-            out[(from + i / width) * row_len + first + i % width] = from_float<T>(0.f);
-    }
+    const int64_t first = __ldg(p.offsets), end = __ldg(p.offsets + p.B);
+    const int64_t lo = first < 0 ? 0 : first > p.T ? p.T : first;
+    const int64_t hi = end < 0 ? 0 : end > p.T ? p.T : end;
+    const int64_t before = lo * row_len, all = before + (p.T - hi) * row_len;
+    const int64_t stride = (int64_t)gridDim.x * gridDim.y * blockDim.x;
+    int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x;
+    for (; i < all; i += stride)
+        out[i < before ? i : hi * row_len + (i - before)] = from_float<T>(0.f);
 }
 
 // Index of the kept state at the start of stretch k of a row.
@@ -529,6 +529,7 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
     constexpr bool BACK = MODE == 2;
     extern __shared__ __align__(16) unsigned char s_tiles[];
     __shared__ float4 s_pair[2][kScanWarps][32];
+    if (MODE == 0) clear_uncovered(p, p.C, states);
     Th th;
     if (!th.init(p)) return;
     const int n = (int)(th.k1 - th.k0);
@@ -697,9 +698,6 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
             th.put(p, last + th.b * p.C + th.ch, carry);
         }
     }
-    if (MODE == 0 && th.split == 0)
-        clear_uncovered(p, th.b, th.tile.first, th.tile.width, (int64_t)p.C, states,
-                        th.wseg * 32 + th.lane, Th::warps_of(p) * 32);
 }
 
 // The backward pass of a tile.  `parted`: (parts, steps, H) floats for the sums of a group that
@@ -716,6 +714,8 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
     extern __shared__ __align__(16) unsigned char s_tiles[];
     __shared__ float4 s_pair[2][kScanWarps][32];
     __shared__ float2 s_flow[2][kScanWarps][32];
+    clear_uncovered(p, p.C, dx);
+    clear_uncovered(p, p.H, dg);
     Th th;
     if (!th.init(p)) return;
     const int n = (int)(th.k1 - th.k0);
@@ -968,13 +968,6 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
     if (th.split == 0) {
         if (th.wseg == 0 && th.sub == 0 && dh0 != nullptr)
             th.put(p, dh0 + th.b * p.C + th.ch, R);
-        const int thread = th.wseg * 32 + th.lane, threads = Th::warps_of(p) * 32;
-        clear_uncovered(p, th.b, th.tile.first, th.tile.width, (int64_t)p.C, dx, thread, threads);
-        const bool own_head = p.parts == 1 || th.tile.first == th.tile.head * p.D;
-        if (own_head)
-            clear_uncovered(p, th.b, p.D == 1 ? th.tile.first : th.tile.head,
-                            p.D == 1 ? th.tile.width : p.parts > 1 ? 1 : th.tile.width / p.D,
-                            (int64_t)p.H, dg, thread, threads);
     }
 }
 

@@ -36,8 +36,8 @@ def gated_scan(values, thickness, initial=None, offsets=None, reverse=False, pre
     ``csrc.check_device_status()``.
     """
     _C.refuse_tangents(values, thickness, initial)
-    return tuple(_C.host().gated_scan(values, thickness, initial, offsets, reverse, premultiplied,
-                                      True, "initial"))
+    return _C.host().gated_scan(values, thickness, initial, offsets, reverse, premultiplied, True,
+                                "initial")
 
 
 def composite(values, thickness, background=None, offsets=None, premultiplied=False):
@@ -49,4 +49,4 @@ def composite(values, thickness, background=None, offsets=None, premultiplied=Fa
     """
     _C.refuse_tangents(values, thickness, background)
     return _C.host().gated_scan(values, thickness, background, offsets, True, premultiplied, False,
-                                "background")[0]
+                                "background")

@@ -140,7 +140,8 @@ def check_call(dev, x, g, initial, offsets, reverse, weighted, gen, with_states=
 
 
 # (B, T, C, H): one step to several stretches and splits, odd sizes, gates of all kinds
-SHAPES = [(2, 200, 128, 128), (1, 3000, 64, 64), (1, 1, 1, 1), (3, 1, 5, 5), (2, 2, 3, 1), (2, 63, 33, 33), (1, 64, 64, 64), (3, 65, 66, 66),
+SHAPES = [(2, 300, 128, 2), (1, 700, 128, 8), (1, 3000, 128, 2), (170, 20, 64, 64),
+          (3, 150, 6, 2), (2, 200, 128, 128), (1, 3000, 64, 64), (1, 1, 1, 1), (3, 1, 5, 5), (2, 2, 3, 1), (2, 63, 33, 33), (1, 64, 64, 64), (3, 65, 66, 66),
           (2, 130, 7, 7), (1, 257, 48, 3), (2, 71, 96, 4), (1, 40, 200, 1), (2, 33, 130, 2),
           (5, 19, 34, 17), (1, 1500, 3, 1), (1, 1029, 70, 70), (40, 9, 16, 16), (2, 700, 1, 1),
           (3, 100, 12, 4)]
@@ -401,6 +402,27 @@ def test_composite_wherever_it_lies(cuda_device, C, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C,H,T", [(64, 4, 1500), (64, 64, 1500), (6, 2, 90), (3, 3, 40), (32, 1, 70),
+                                   (300, 1, 50), (37, 1, 70), (200, 1, 1500)])
+@pytest.mark.parametrize("premultiplied", [False, True])
+def test_composite_groups(cuda_device, C, H, T, premultiplied):
+    """Thickness of groups of channels or of each, and values weighted beforehand; long rays."""
+    gen = torch.Generator().manual_seed(C + H)
+    x, g = inputs(gen, (2, T), C, H, BF16, F32, cuda_device)
+    bg = torch.rand(C, generator=gen).to(cuda_device)
+    with torch.no_grad():
+        alone = svox.composite(x, g, bg, premultiplied=premultiplied)
+    leaves = [t.requires_grad_(True) for t in (x, g)]
+    out = svox.composite(x, g, bg, premultiplied=premultiplied)
+    d = torch.randn(out.shape, generator=gen).to(cuda_device)
+    want = reference(x, g, bg, None, True, premultiplied, None, d)
+    close("last", out, want["last"])
+    close("last", alone, want["last"])
+    for name, got in zip(("d_values", "d_thickness"), torch.autograd.grad(out, leaves, d)):
+        close(name, got, want[name])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("C", [3, 64])
 def test_masked_places(cuda_device, C):
     """Samples of no thickness may hold anything; nothing from behind an opaque sample shows."""
@@ -505,6 +527,36 @@ def test_empty(cuda_device):
     bg = torch.rand(3, device=cuda_device)
     assert torch.equal(svox.composite(x, g, bg, rays), bg.expand(5, 3))
     csrc.check_device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,H", [(3, 1), (32, 1), (64, 64), (66, 2)])
+def test_buffers_that_are_not_full(cuda_device, C, H):
+    """Far more room than samples (a buffer of fixed size): zeros in all of it, whatever lies there."""
+    gen = torch.Generator().manual_seed(9)
+    offsets = torch.tensor([4001, 4041, 4041, 4100], device=cuda_device)
+    N = 300_000
+    x = torch.full((N, C), float("nan"), device=cuda_device)
+    g = torch.full((N, H) if H > 1 else (N,), float("nan"), device=cuda_device)
+    some, gates = inputs(gen, (99,), C, H, F32, F32, cuda_device)
+    x[4001:4100], g[4001:4100] = some, gates
+    x.requires_grad_(True)
+    g.requires_grad_(True)
+    junk = [torch.full((N * C,), float("nan"), device=cuda_device) for _ in range(4)]
+    del junk
+    states, last = svox.gated_scan(x, g, offsets=offsets, reverse=True)
+    d = torch.randn(3, C, generator=gen).to(cuda_device)
+    want = reference(some, gates, None, offsets - 4001, True, False, None, d)
+    close("states", states[4001:4100], want["states"])
+    grads = [torch.autograd.grad(last, [x, g], d)]
+    if H == 1:
+        grads.append(torch.autograd.grad(svox.composite(x, g, offsets=offsets), [x, g], d))
+    for t in (states, *[t for pair in grads for t in pair]):
+        assert (t[:4001] == 0).all() and (t[4100:] == 0).all()
+    for dx, dg in grads:
+        close("d_values", dx[4001:4100], want["d_values"])
+        close("d_thickness", dg[4001:4100], want["d_thickness"])
+    assert csrc.device_status() == 0
 
 
 @pytest.mark.gpu
