@@ -459,10 +459,9 @@ def refuse_tangent(data):
 
 def refuse_tangents(*tensors):
     """``refuse_tangent`` of each tensor that is not None."""
-    if _fwd._current_level >= 0:
-        for t in tensors:
-            if t is not None:
-                refuse_tangent(t)
+    for t in tensors:
+        if t is not None:
+            refuse_tangent(t)
 
 
 def record_bytes(K, group):

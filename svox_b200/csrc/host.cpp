@@ -741,7 +741,11 @@ Scan read_scan(const Tensor& values, const Tensor& thickness, const optional<Ten
     s.values = dense_rows(values);
     s.thickness = thickness.dim() == lead + 1 ? dense_rows(thickness) : thickness;
     if (packed) s.offsets = offsets->contiguous();
-    if (initial) s.initial = dense_rows(initial->to(at::kFloat).expand({B, C}));
+    if (initial) {
+        const bool plain = initial->scalar_type() == at::kFloat && initial->dim() == 2 &&
+                           initial->size(0) == B && initial->size(1) == C;
+        s.initial = dense_rows(plain ? *initial : initial->to(at::kFloat).expand({B, C}));
+    }
     return s;
 }
 

@@ -14,6 +14,7 @@ from .formats import DataFormat
 __all__ = ["RecordCache"]
 
 _CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_VALUES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 class RecordCache(nn.Module):
@@ -79,10 +80,11 @@ class RecordCache(nn.Module):
 
     def _write(self, where, points, values, offset, scaling):
         b = self._buffers
-        if values.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("a record cache takes no gradient: detach the values")
-        values = values.detach()
-        if values.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        if values.requires_grad:
+            if torch.is_grad_enabled():
+                raise RuntimeError("a record cache takes no gradient: detach the values")
+            values = values.detach()
+        if values.dtype not in _VALUES:
             values = values.float()
         _C.host().records_write(b["records"], b["_owner"], b["child"], offset, scaling,
                                 self.data_dim, self.group, _CODES[self.dtype], where, points,
@@ -124,4 +126,6 @@ class RecordCache(nn.Module):
     def _points(self, points):
         assert not points.requires_grad  # Grad wrt points not supported
         assert points.dim() == 2
-        return points.to(torch.float32).contiguous()
+        if points.dtype != torch.float32:
+            points = points.to(torch.float32)
+        return points.contiguous()

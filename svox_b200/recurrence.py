@@ -9,6 +9,8 @@ which is what the renderer accumulates inside its march (svox/csrc/rt_kernel.cu:
 samples that the caller has chosen and evaluated, and for any sequence that is gated in this way.
 No counterpart in the reference, whose users composite with tensor operations.
 """
+from torch.autograd import forward_ad as _fwd
+
 from . import csrc as _C
 
 __all__ = ["gated_scan", "composite"]
@@ -35,7 +37,8 @@ def gated_scan(values, thickness, initial=None, offsets=None, reverse=False, pre
     read on the device: one out of order or range is cut to it and noticed by
     ``csrc.check_device_status()``.
     """
-    _C.refuse_tangents(values, thickness, initial)
+    if _fwd._current_level >= 0:
+        _C.refuse_tangents(values, thickness, initial)
     return _C.host().gated_scan(values, thickness, initial, offsets, reverse, premultiplied, True,
                                 "initial")
 
@@ -47,6 +50,7 @@ def composite(values, thickness, background=None, offsets=None, premultiplied=Fa
     ``background`` (``(B, C)`` or what broadcasts to it; nothing by default).  Arguments and
     gradients as there; a ray without samples shows its background.
     """
-    _C.refuse_tangents(values, thickness, background)
+    if _fwd._current_level >= 0:
+        _C.refuse_tangents(values, thickness, background)
     return _C.host().gated_scan(values, thickness, background, offsets, True, premultiplied, False,
                                 "background")
