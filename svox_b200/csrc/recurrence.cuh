@@ -152,6 +152,12 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 __device__ __forceinline__ F2 past2(F2 a, F2 h, F2 b) {
     return {past(a.x, h.x, b.x), past(a.y, h.y, b.y)};
 }
+// The product of a stretch's gates and those of the stretch before it: 0 where its own are, whatever
+// the others.
+__device__ __forceinline__ F2 gates2(F2 a, F2 before) {
+    const F2 r = mul2(a, before);
+    return {a.x == 0.f ? 0.f : r.x, a.y == 0.f ? 0.f : r.y};
+}
 __device__ __forceinline__ F2 shfl2(F2 v, int lane) {
     return {__shfl_sync(~0u, v.x, lane), __shfl_sync(~0u, v.y, lane)};
 }
@@ -466,7 +472,7 @@ struct ScanThread {
             for (int s = from; s < to; ++s, at += step) {
                 const float2 q = __ldcg(at), r = __ldcg(at + second);
                 B = past2({q.x, r.x}, B, {q.y, r.y});
-                A = mul2({q.x, r.x}, A);
+                A = gates2({q.x, r.x}, A);
             }
         }
         shared += group * warps_of(p) * 32;
@@ -502,7 +508,7 @@ __device__ __forceinline__ void join_lanes(int lanes, int lane, F2& A, F2& B, F2
         const F2 a = shfl2(A, from & 31), b = shfl2(B, from & 31);
         if (from >= 0 && from < 32) {
             B = past2(A, b, B);
-            A = mul2(A, a);
+            A = gates2(A, a);
         }
     }
     const int edge = BACK ? lane & (lanes - 1) : 32 - lanes + (lane & (lanes - 1));
@@ -628,7 +634,7 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
                     th.step(p, tx, tg, j, al, ul, false);
                     B = past2(al, B, ul);
                 }
-                A = mul2(A, al);
+                A = gates2(al, A);
             }
         }
         if (keep != nullptr) {
@@ -640,12 +646,12 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
         F2 h = carry;
         if (Th::warps_of(p) == 1) {
             carry = past2(TA, carry, TB);
-            if (MODE != 0) through = mul2(through, TA);
+            if (MODE != 0) through = gates2(TA, through);
         } else {
             auto& pair = s_pair[i & 1];
             if (th.sub == 0) pair[th.warp][th.cl] = make_float4(TA.x, TA.y, TB.x, TB.y);
             th.unit_sync(p);
-            const F2 before = carry;
+            const F2 before = carry, through_before = through;
             const float4* const all = &pair[th.group * Th::warps_of(p)][th.cl];
 #pragma unroll 8
             for (int j = 0; j < Th::warps_of(p); ++j) {
@@ -657,11 +663,13 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
             }
             if (spoilt(carry, carry) != 0.f) {
                 carry = before;
+                through = through_before;
                 for (int j = 0; j < Th::warps_of(p); ++j) {
                     const int w = BACK ? Th::warps_of(p) - 1 - j : j;
                     if (w == th.wseg) h = carry;
                     const float4 q = all[w * 32];
                     carry = past2({q.x, q.y}, carry, {q.z, q.w});
+                    if (MODE != 0) through = gates2({q.x, q.y}, through);
                 }
             }
         }
@@ -771,7 +779,8 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
     const float* keep = kept + kept_index(p, th.row, th.b, th.chunk, first) * p.C + th.ch;
     F2 h_next = n > 0 ? th.get(keep) : two(0.f);
     F2 R = d_last != nullptr ? th.get(d_last + th.b * p.C + th.ch) : two(0.f);
-    R = th.ranges(p, pairs, R, true, &s_pair[0][0][0]);     // what flows back into the last state of the tile
+    // what flows back into the last state of the tile
+    R = th.ranges(p, pairs, R, true, &s_pair[0][0][0]);
     // (outputs are written from a stretch's last step to its first)
     const int64_t out0 = th.row.first + th.place(p, first * th.chunk + th.step0 + L - 1);
     VT* to_x = dx == nullptr ? nullptr : dx + out0 * p.C + th.ch;
@@ -808,11 +817,13 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
         bool odd = spoilt(A, B) != 0.f || spoilt(E, E) != 0.f;
         if (odd) {
             F2 al, ul;
+            A = two(1.f);
             B = E = two(0.f);
 #pragma unroll 1
             for (int l = 0; l < L; ++l) {
                 th.step(p, tx, tg, l, al, ul, false);
                 B = past2(al, B, ul);
+                A = gates2(al, A);
             }
 #pragma unroll 1
             for (int l = L - 1; l >= 0; --l) {

@@ -468,6 +468,33 @@ def test_masked_places(cuda_device, C):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,T,C,H", [(3, 90, 6, 1), (3, 90, 6, 3), (2, 700, 70, 70), (1, 6000, 64, 64),
+                                     (1, 6000, 64, 2), (1, 6000, 5, 1), (2, 5, 8, 1)])
+@pytest.mark.parametrize("premultiplied", [False, True])
+def test_states_past_an_opaque_step(cuda_device, B, T, C, H, premultiplied):
+    """Whatever the thickness before it, NaN too: from the opaque step on, all states are those of a row
+    that begins there, in rows of several ranges as well."""
+    gen = torch.Generator().manual_seed(T + C)
+    x, g = inputs(gen, (B, T), C, H, F32, F32, cuda_device)
+    k = T * 2 // 3
+    g[:, k] = float("inf")
+    g[:, 1:k] = float("nan")
+    h0 = torch.full((B, C), float("nan"), device=cuda_device)
+    leaves = [t.requires_grad_(True) for t in (x, g, h0)]
+    states, last = svox.gated_scan(x, g, h0, premultiplied=premultiplied)
+    d_states = torch.randn(states.shape, generator=gen).to(cuda_device)
+    d_last = torch.randn(last.shape, generator=gen).to(cuda_device)
+    grads = torch.autograd.grad((states, last), leaves, (d_states, d_last))
+    part = slice(None), slice(k, None)
+    want = reference(x[part], g[part], None, None, False, premultiplied, d_states[part], d_last)
+    close("states", states[part], want["states"])
+    close("last", last, want["last"])
+    close("d_values", grads[0][part], want["d_values"])
+    close("d_thickness", grads[1][part], want["d_thickness"])
+    assert states[:, 1:k].isnan().all()
+
+
+@pytest.mark.gpu
 def test_partial_gradients(cuda_device):
     """Only some outputs used, only some inputs asked for."""
     gen = torch.Generator().manual_seed(4)
