@@ -4,8 +4,8 @@
 //   out = sum of W[i] x[i] + T[n] background,   T[i] = a[0] ... a[i-1],   W[i] = T[i] w[i]
 // so a group of G lanes walks a ray, a sample to a lane, and scans nothing but what reaches a sample
 // (its products: exp of a sum of thicknesses would be off by the sum's rounding, 4e-6 of a background
-// behind a thickness of 70); the channels are summed in each lane and over the lanes at the end.  With d the upstream gradient and
-// c[i] = d . x[i] the backward pass is
+// behind a thickness of 70); the channels are summed in each lane and over the lanes at the end.
+// With d the upstream gradient and c[i] = d . x[i] the backward pass is
 //   dx[i] = W[i] d,   dg[i] = T[i+1] c[i] - (sum over j > i of W[j] c[j] + T[n] d . background)
 // one more scan of plain sums, from the far end, whatever the number of channels.  The forward keeps
 // what reaches every G-th sample for it.
@@ -35,10 +35,44 @@ struct Gate { float a, w; };
 __device__ __forceinline__ Gate gate_of(float g) {
     const float s = g * fmaf(g, fmaf(g, fmaf(g, fmaf(g, fmaf(g, -1.f / 720, 1.f / 120), -1.f / 24),
                                             1.f / 6), -0.5f), 1.f);
+    constexpr double log2e = 1.4426950408889634;
+    constexpr float most = (float)log2e, rest = (float)(log2e - most);
     float e;
-    asm("ex2.approx.ftz.f32 %0, %1;"
-        : "=f"(e) : "f"(fmaf(g, -1.44269502162933349609375f, g * -1.92596299112662e-8f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(g, -most, g * -rest)));
     return fabsf(g) < 0.25f ? Gate{1.f - s, s} : Gate{e, 1.f - e};
+}
+
+// What reaches beyond each lane's N samples, and `reach` what reaches the group.  Behind an opaque
+// sample nothing counts, a thickness that is not a number either: where one spoils a product, the
+// gates behind a 0 are closed first.
+template <int G, int N>
+__device__ __forceinline__ float reach_beyond(int lane, float reach, Gate (&gate)[N]) {
+    auto scan = [&](bool careful) {
+        float v = gate[0].a;
+        if (N == 4 && !careful) v = (gate[0].a * gate[1 % N].a) * (gate[2 % N].a * gate[3 % N].a);
+        if (careful)
+#pragma unroll
+            for (int i = 1; i < N; ++i) v = v == 0.f ? 0.f : v * gate[i].a;
+#pragma unroll
+        for (int d = 1; d < G; d *= 2) {
+            const float o = __shfl_up_sync(~0u, v, d, G);
+            if (lane >= d) v = careful && o == 0.f ? 0.f : v * o;
+        }
+        return v;
+    };
+    float v = reach * scan(false);
+    if (__any_sync(~0u, v != v)) {
+        const float all = scan(true);
+        float front = __shfl_up_sync(~0u, all, 1, G);
+        front = reach == 0.f ? 0.f : lane > 0 ? reach * front : reach;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (front == 0.f) gate[i] = Gate{0.f, 0.f};
+            else front *= gate[i].a;
+        }
+        v = reach * scan(false);
+    }
+    return v;
 }
 
 template <class VT, class GT, int C, int G>
@@ -67,15 +101,7 @@ struct RayThread {
     __device__ __forceinline__ int64_t kept_at(const ScanArgs& p) const {
         return p.offsets ? first / G + b : b * ((p.T + G - 1) / G);
     }
-    // Product over this lane and the ones before it; sum over it and the ones behind it.
-    __device__ __forceinline__ float through(float v) const {
-#pragma unroll
-        for (int d = 1; d < G; d *= 2) {
-            const float o = __shfl_up_sync(~0u, v, d, G);
-            if (lane >= d) v *= o;
-        }
-        return v;
-    }
+    // Sum over this lane and the ones behind it.
     __device__ __forceinline__ float from(float v) const {
 #pragma unroll
         for (int d = 1; d < G; d *= 2) {
@@ -107,8 +133,9 @@ ray_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
         th.x += dx;
         th.g += dg;
         if (keep != nullptr && in) *keep++ = reach;
-        const Gate gate = gate_of(gi);
-        const float v = reach * th.through(gate.a);
+        Gate gates[1] = {gate_of(gi)};
+        const float v = reach_beyond<G>(th.lane, reach, gates);
+        const Gate gate = gates[0];
         float T = __shfl_up_sync(~0u, v, 1, G);
         if (th.lane == 0) T = reach;
         reach = __shfl_sync(~0u, v, G - 1, G);
@@ -176,8 +203,9 @@ ray_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restr
         for (int q = 0; q < C; ++q) c = fmaf(d[q], xv[q], c);
         th.x -= step_x;
         th.g -= step_g;
-        const Gate gate = gate_of(gi);
-        const float v = reach * th.through(gate.a);
+        Gate gates[1] = {gate_of(gi)};
+        const float v = reach_beyond<G>(th.lane, reach, gates);
+        const Gate gate = gates[0];
         float T = __shfl_up_sync(~0u, v, 1, G);
         if (th.lane == 0) T = reach;
         const float total = __shfl_sync(~0u, v, G - 1, G);
@@ -290,14 +318,6 @@ struct RayQuads {
             for (int i = 0; i < 4 * N; ++i) v[i] = i < left * N ? to_float(from[i]) : 0.f;
         }
     }
-    __device__ __forceinline__ float through(float v) const {
-#pragma unroll
-        for (int d = 1; d < G; d *= 2) {
-            const float o = __shfl_up_sync(~0u, v, d, G);
-            if (lane >= d) v *= o;
-        }
-        return v;
-    }
     __device__ __forceinline__ float from(float v) const {
 #pragma unroll
         for (int d = 1; d < G; d *= 2) {
@@ -340,8 +360,7 @@ quad_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
                 gv[i] = th.in(at + i) ? gv[i] : 0.f;
                 gate[i] = gate_of(gv[i]);
             }
-            const float v =
-                reach * th.through((gate[0].a * gate[1].a) * (gate[2].a * gate[3].a));
+            const float v = reach_beyond<G>(th.lane, reach, gate);
             float T = __shfl_up_sync(~0u, v, 1, G);
             if (th.lane == 0) T = reach;
             reach = __shfl_sync(~0u, v, G - 1, G);
@@ -406,8 +425,7 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
                 gv[i] = th.in(at + i) ? gv[i] : 0.f;
                 gate[i] = gate_of(gv[i]);
             }
-            const float v =
-                reach * th.through((gate[0].a * gate[1].a) * (gate[2].a * gate[3].a));
+            const float v = reach_beyond<G>(th.lane, reach, gate);
             float T = __shfl_up_sync(~0u, v, 1, G);
             if (th.lane == 0) T = reach;
             const float total = __shfl_sync(~0u, v, G - 1, G);
@@ -428,16 +446,17 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
                 own[i] = p.weighted ? 0.f : T * c[i];
             }
             if (!finite((c[0] + c[1]) + (c[2] + c[3]))) {
-                // What is not finite counts only where it has weight; where there is no thickness it is
-                // no sample, and behind an opaque one neither.
+                // What is not finite counts only where it has weight; where there is no thickness it
+                // is no sample, and behind an opaque one neither.
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     Wc[i] = times(W[i], c[i]);
-                    if (!finite(c[i]) && !p.weighted && (gv[i] == 0.f || W[i] == 0.f)) none |= 1u << i;
+                    if (!finite(c[i]) && !p.weighted && (gv[i] == 0.f || W[i] == 0.f))
+                        none |= 1u << i;
                 }
             }
             const float here = th.from((Wc[0] + Wc[1]) + (Wc[2] + Wc[3])) + behind;
-            float rest = __shfl_down_sync(~0u, here, 1, G);     // what all samples behind the quad bring
+            float rest = __shfl_down_sync(~0u, here, 1, G);     // what all behind the quad bring
             if (th.lane == G - 1) rest = behind;
             behind = __shfl_sync(~0u, here, 0, G);
             if (at < th.len) {
@@ -533,8 +552,9 @@ row_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
         th.g += 32 * p.gs;
         g_next = th.lane + 32 < left ? to_float(*th.g) : 0.f;
         if (keep != nullptr) keep[k] = reach;
-        const Gate gate = gate_of(gi);
-        const float v = reach * th.through(gate.a);
+        Gate gates[1] = {gate_of(gi)};
+        const float v = reach_beyond<32>(th.lane, reach, gates);
+        const Gate gate = gates[0];
         float T = __shfl_up_sync(~0u, v, 1);
         if (th.lane == 0) T = reach;
         reach = __shfl_sync(~0u, v, 31);
@@ -627,8 +647,9 @@ row_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restr
             part = __shfl_sync(~0u, part, (th.lane & (rows.per - 1)) * rows.width);
             if (th.lane / rows.per == j) c = part;
         }
-        const Gate gate = gate_of(gi);
-        const float v = reach * th.through(gate.a);
+        Gate gates[1] = {gate_of(gi)};
+        const float v = reach_beyond<32>(th.lane, reach, gates);
+        const Gate gate = gates[0];
         float T = __shfl_up_sync(~0u, v, 1);
         if (th.lane == 0) T = reach;
         if (k == th.chunks - 1) {

@@ -468,6 +468,38 @@ def test_masked_places(cuda_device, C):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C", [1, 3, 32, 64, 300])
+@pytest.mark.parametrize("premultiplied", [False, True])
+def test_behind_an_opaque_sample(cuda_device, C, premultiplied):
+    """Nothing of what is behind it counts, a thickness that is not a number neither: not for what is
+    seen, and not for the gradients of what is in front."""
+    gen = torch.Generator().manual_seed(C)
+    x, g = inputs(gen, (5, 90), C, 1, F32, F32, cuda_device)
+    at = [0, 1, 37, 70, 88]
+    for row, k in enumerate(at):
+        g[row, k] = float("inf")
+        g[row, k + 1:] = float("nan")
+        x[row, k + 1:] = float("nan")
+    bg = torch.full((5, C), float("nan"), device=cuda_device)
+    d = torch.randn(5, C, generator=gen).to(cuda_device)
+    leaves = [t.requires_grad_(True) for t in (x, g, bg)]
+    for xv, gv, offsets in ((x, g, None), (x.view(-1, C), g.view(-1),
+                                           torch.arange(6, device=cuda_device) * 90)):
+        out = svox.composite(xv, gv, bg, offsets, premultiplied)
+        grads = torch.autograd.grad(out, leaves, d)
+        for row, k in enumerate(at):
+            part = slice(row, row + 1), slice(0, k + 1)
+            want = reference(x[part], g[part], None, None, True, premultiplied, None, d[part[0]])
+            close("last", out[part[0]], want["last"])
+            close("d_values", grads[0][part], want["d_values"])
+            close("d_thickness", grads[1][part], want["d_thickness"])
+    # in front of it, it counts
+    with torch.no_grad():
+        g[2, 5] = float("nan")
+        assert svox.composite(x, g, bg)[2].isnan().all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("B,T,C,H", [(3, 90, 6, 1), (3, 90, 6, 3), (2, 700, 70, 70), (1, 6000, 64, 64),
                                      (1, 6000, 64, 2), (1, 6000, 5, 1), (2, 5, 8, 1)])
 @pytest.mark.parametrize("premultiplied", [False, True])
