@@ -19,6 +19,12 @@ constexpr int64_t kRayShort = 12;
 //   2^16 of 84: 146 / 111 / 95 / 118; 2^17 of 160: 504 / 377 / 271 / 292; 2^15 of 600: 822 / 491 / 326 / 266
 // and without windows: of 42, 725 / 726 / 860.
 constexpr int64_t kQuadsMean[] = {28, 60, 240};
+// Features of 136 to 256 channels (in 16 bits, whole 16-byte pieces): a warp to a ray from so many rays
+// on, and from half as many where they are of no more samples than this; tiles before.  200 channels,
+// forward and backward, us, a warp to a ray / tiles, on 16-byte boundaries: 512 rays of 64 samples
+// 51 / 77, of 300 304 / 242; 256 of 64 51 / 45; 64 of 2000 1664 / 200; and off them: 1024 of 200 389 / 505,
+// 512 of 300 484 / 314, 4096 of 64 168 / 688.
+constexpr int64_t kWideRays = 1024, kWideShort = 128;
 // Lanes that all rays together can have at once; 4096 rays of 21, forward: 9.1 / 6.0 / 4.3 / 4.0 us.
 constexpr int64_t kQuadsFew = 1 << 17;
 // Warps that a window of rays has to leave.
@@ -40,12 +46,16 @@ RayPlan ray_plan(const svoxb_scan* s) {
     // (their lengths are counted in 32 bits)
     if (mean > kRayLongest || (s->offsets && s->T > 0x7fffffff - 256)) return plan;
     if (s->C > kRayChannels) {
+        // (sizes and types alone choose between these kernels and the tiles, which keep other things
+        // for the backward pass; where the rows lie, only how these read them)
         const int size = s->values_type == SVOXB_TYPE_F32 ? 4 : 2, piece = 16 / size;
-        const bool whole = reinterpret_cast<uintptr_t>(s->values) % 16 == 0 && s->C % piece == 0 &&
+        const bool pieces = s->C % piece == 0;
+        const int64_t rays = mean <= kWideShort ? kWideRays / 2 : kWideRays;
+        if (s->C > 128 && !(pieces && s->C / piece <= 32 && s->B >= rays)) return plan;
+        const bool whole = reinterpret_cast<uintptr_t>(s->values) % 16 == 0 && pieces &&
                            s->values_step % piece == 0 && s->values_row % piece == 0;
         plan.share = whole ? piece : 1;
         const int shares = s->C / plan.share;
-        if (shares > (whole ? 32 : 128)) return RayPlan{};
         plan.width = 1;
         while (plan.width < shares && plan.width < 32) plan.width *= 2;
         plan.lanes = 32;
@@ -132,7 +142,8 @@ void with_rows(const svoxb_scan* s, RayPlan plan, F f) {
         constexpr int piece = 16 / (int)sizeof(typename decltype(t)::V);
         if (plan.share > 1) f(t, Int<piece>{}, Int<1>{});
         else if (s->C <= 32) f(t, Int<1>{}, Int<1>{});
-        else f(t, Int<1>{}, Int<4>{});
+        else if (s->C <= 128 || piece == 4) f(t, Int<1>{}, Int<4>{});
+        else if constexpr (piece == 8) f(t, Int<1>{}, Int<8>{});
     };
     const bool same = s->thickness_type == s->values_type;
     if (s->values_type == SVOXB_TYPE_F32) types(Types<float, float>{});

@@ -818,3 +818,82 @@ def test_abi_refusals():
     s = call()[1]
     assert lib.svoxb_gated_scan_backward(C.byref(s), None, None, None, None, None, None, None,
                                          None) == 1         # no kept states
+
+
+def scan_struct():
+    import ctypes as C
+
+    class Scan(C.Structure):
+        _fields_ = [("values", C.c_void_p), ("thickness", C.c_void_p), ("initial", C.c_void_p),
+                    ("offsets", C.c_void_p), ("B", C.c_int64), ("T", C.c_int64),
+                    ("values_row", C.c_int64), ("values_step", C.c_int64),
+                    ("thickness_row", C.c_int64), ("thickness_step", C.c_int64),
+                    ("initial_row", C.c_int64), ("C", C.c_int32), ("H", C.c_int32),
+                    ("values_type", C.c_int32), ("thickness_type", C.c_int32),
+                    ("reverse", C.c_int32), ("weighted", C.c_int32),
+                    ("last_only", C.c_int32), ("layout", C.c_int32)]
+
+    return Scan
+
+
+@pytest.mark.parametrize("C", [3, 32, 35, 120, 128, 136, 200, 256, 264])
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_what_is_kept_follows_the_layout(C, kind):
+    """What the forward pass keeps goes by sizes, types and `layout`, not by where the arrays lie."""
+    import ctypes as ct
+    lib = csrc.library()
+    lib.svoxb_gated_scan_kept.restype = ct.c_int64
+    B, T, size = 1000, 64, 4 if kind == 0 else 2
+    wide = (C + 5) // 2 * 2 + 1
+    for offsets in (None, 16):
+        kept = {}
+        for address, step in ((1 << 20, C), ((1 << 20) + size, C), (1 << 20, wide)):
+            s = scan_struct()(address, 1 << 20, None, offsets, B, T * B if offsets else T, T * step,
+                              step, T, 1, 0, C, 1, kind, 0, 1, 0, 1, 0)
+            layout = lib.svoxb_gated_scan_layout(ct.byref(s))
+            mine = lib.svoxb_gated_scan_kept(ct.byref(s))
+            s.layout = layout
+            assert lib.svoxb_gated_scan_layout(ct.byref(s)) == layout
+            assert lib.svoxb_gated_scan_kept(ct.byref(s)) == mine
+            assert kept.setdefault(layout, mine) == mine, (layout, kept, mine)
+
+
+def off_boundary(t):
+    """The same values, one element off a 16-byte boundary."""
+    to = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    to[1:] = t.detach().flatten()
+    return to[1:].view(t.shape)
+
+
+def on_columns(t):
+    """The same values in rows of a wider array."""
+    wide = torch.zeros(*t.shape[:-1], t.shape[-1] + 3, dtype=t.dtype, device=t.device)
+    wide[..., 1:-2] = t.detach()
+    return wide[..., 1:-2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+@pytest.mark.parametrize("C", [120, 136, 200, 256, 264])
+@pytest.mark.parametrize("many", [False, True])
+def test_features_saved_elsewhere(cuda_device, C, dtype, many):
+    """Wide features in 16 bits whose saved tensors lie elsewhere than the forward's, either way: on
+    their boundaries, off them, in a wider array, by way of the host."""
+    gen = torch.Generator().manual_seed(C)
+    n = torch.tensor([30, 0, 77, 5, 1, 200] + [0, 1, 0] * (200 if many else 0))
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), n.cumsum(0)]).to(cuda_device)
+    x, g = inputs(gen, (int(n.sum()),), C, 1, dtype, F32, cuda_device)
+    d = torch.randn(n.numel(), C, generator=gen).to(cuda_device)
+    want = reference(x, g, None, offsets, True, False, None, d)
+    places = [lambda t: t.detach().clone(), off_boundary, on_columns]
+    for place in places:
+        def moved(to):
+            return lambda t: to(t) if t.dtype == dtype else t
+        hooks = [torch.autograd.graph.saved_tensors_hooks(lambda t: t, moved(to)) for to in places]
+        for hook in [*hooks, torch.autograd.graph.save_on_cpu()]:
+            leaves = [place(x).requires_grad_(True), g.detach().clone().requires_grad_(True)]
+            with hook:
+                out = svox.composite(*leaves, offsets=offsets)
+            close("last", out, want["last"])
+            for name, got in zip(("d_values", "d_thickness"), torch.autograd.grad(out, leaves, d)):
+                close(name, got, want[name])
