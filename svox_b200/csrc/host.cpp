@@ -649,9 +649,25 @@ Tensor dense_rows(const Tensor& t) {
     return t.size(last) <= 1 || t.stride(last) == 1 ? t : t.contiguous();
 }
 
+// What a tensor has to be when it comes back from where the backward pass found it.
+struct Kind {
+    at::DimVector sizes;
+    at::ScalarType type = at::kFloat;
+    at::Device device = at::kCPU;
+    Kind() = default;
+    explicit Kind(const Tensor& t) {
+        if (t.defined()) sizes = t.sizes(), type = t.scalar_type(), device = t.device();
+    }
+    bool fits(const Tensor& t) const {
+        return !t.defined() ? device == at::kCPU
+                            : t.sizes() == sizes && t.scalar_type() == type && t.device() == device;
+    }
+};
+
 // What a call of the recurrence works on; the tensors lie as the kernels read them.
 struct Scan {
     Tensor values, thickness, initial, offsets;
+    std::array<Kind, 5> saved;      // for the backward pass
     bool reverse = false, weighted = false, states = true;
     int32_t layout = 0;     // of what the forward kept
     svoxb_scan c{};
@@ -774,8 +790,10 @@ class ScanNode : public torch::autograd::Function<ScanNode> {
         ctx->set_materialize_grads(false);
         auto [states, last, kept] = run_scan(*call, true);
         call->layout = lib.gated_scan_layout(&call->c);
-        ctx->save_for_backward(
-            {values, thickness, initial ? *initial : Tensor(), call->offsets, kept});
+        torch::autograd::variable_list saved{values, thickness, initial ? *initial : Tensor(),
+                                             call->offsets, kept};
+        for (size_t i = 0; i < saved.size(); ++i) call->saved[i] = Kind(saved[i]);
+        ctx->save_for_backward(std::move(saved));
         torch::autograd::variable_list out;
         if (states.defined()) out.push_back(states);
         out.push_back(last);
@@ -788,11 +806,17 @@ class ScanNode : public torch::autograd::Function<ScanNode> {
                                                    torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         Scan s = *kept<std::shared_ptr<Scan>>(ctx);
-        s.values = saved[0], s.thickness = saved[1], s.initial = saved[2], s.offsets = saved[3];
-        const Tensor& kept = saved[4];
+        // (a saved-tensor hook may hand back other tensors than it was given, with strides of their
+        // own; what the forward kept is laid out for those that it had)
+        for (size_t i = 0; i < saved.size(); ++i)
+            if (!s.saved[i].fits(saved[i]))
+                fail("a saved tensor of gated_scan came back with another shape, type or device");
+        s.values = dense_rows(saved[0]);
+        s.thickness = saved[1].dim() == saved[0].dim() ? dense_rows(saved[1]) : saved[1];
+        if (saved[2].defined()) s.initial = dense_rows(saved[2]);
+        if (saved[3].defined()) s.offsets = saved[3].contiguous();
+        const Tensor kept = saved[4].contiguous();
         s.bind();
-        // (a saved-tensor hook may hand back other tensors than it was given: what the forward kept
-        // is laid out for those)
         svoxb_scan anew = s.c;
         anew.layout = 0;
         if (s.layout == 1 && lib.gated_scan_layout(&anew) != 1) {

@@ -897,3 +897,41 @@ def test_features_saved_elsewhere(cuda_device, C, dtype, many):
             close("last", out, want["last"])
             for name, got in zip(("d_values", "d_thickness"), torch.autograd.grad(out, leaves, d)):
                 close(name, got, want[name])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,H", [(3, 1), (32, 1), (200, 1), (64, 8), (5, 5)])
+def test_saved_tensors_in_another_order(cuda_device, C, H):
+    """A hook hands back the saved tensors with strides of its own, or something else altogether."""
+    gen = torch.Generator().manual_seed(C)
+    n = torch.tensor([30, 0, 77, 5, 1])
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), n.cumsum(0)]).to(cuda_device)
+    x, g = inputs(gen, (int(n.sum()),), C, H, F32, F32, cuda_device)
+    h0 = torch.randn(5, C, generator=gen).to(cuda_device)
+    d = torch.randn(5, C, generator=gen).to(cuda_device)
+    want = reference(x, g, h0, offsets, True, False, None, d)
+
+    def strided(t):
+        out = torch.empty(*t.shape[:-1], 2 * t.shape[-1], dtype=t.dtype, device=t.device)
+        out[..., ::2] = t
+        return out[..., ::2]
+
+    def transposed(t):
+        return t.transpose(0, -1).clone(memory_format=torch.contiguous_format).transpose(0, -1)
+
+    def grads(unpack):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, g, h0)]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            if H == 1:
+                out = svox.composite(*leaves, offsets)
+            else:
+                out = svox.gated_scan(*leaves, offsets, reverse=True)[1]
+        return torch.autograd.grad(out, leaves, d)
+
+    for to in (strided, transposed):
+        for name, got in zip(("d_values", "d_thickness", "d_initial"), grads(to)):
+            close(name, got, want[name])
+    for to in (lambda t: t.double() if t.dtype == F32 else t, lambda t: t[:-1], lambda t: t.cpu(),
+               lambda t: t[None]):
+        with pytest.raises(RuntimeError, match="saved tensor"):
+            grads(to)
