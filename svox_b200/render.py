@@ -294,7 +294,8 @@ class VolumeRenderer(nn.Module):
         ``depths`` holds the distances of the samples from the rays' origins, in units of ``dirs``
         and from the nearest to the farthest, and ``lengths`` what each stands for (its thickness is
         the density there times its length): both ``(B, T)``, or ``(N,)`` with ``offsets``
-        ``(B + 1,)`` int64 for rays of any number of samples.  The records are looked up in the tree
+        ``(B + 1,)`` int64 for rays of any number of samples (steps that no ray covers may hold
+        anything).  The records are looked up in the tree
         -- differentiable w.r.t. ``tree.data`` and ``lengths`` -- or in ``cache``, a
         :class:`RecordCache` (no gradient w.r.t. records), and composited by :func:`composite`.
         Densities, colours, ``min_comp`` / ``max_comp``, ``density_softplus``, ``rgb_padding`` and the
@@ -307,6 +308,7 @@ class VolumeRenderer(nn.Module):
         if fmt.format not in (DataFormat.RGBA, DataFormat.SH):
             raise RuntimeError("render_samples takes RGBA and SH records")
         B = rays.origins.shape[0]
+        origins, dirs, viewdirs = rays.origins, rays.dirs, rays.viewdirs
         if offsets is None:
             if depths.dim() != 2 or depths.shape[0] != B or lengths.shape != depths.shape:
                 raise RuntimeError("depths and lengths must be (B, T)")
@@ -314,19 +316,22 @@ class VolumeRenderer(nn.Module):
         else:
             if depths.dim() != 1 or lengths.shape != depths.shape or offsets.numel() != B + 1:
                 raise RuntimeError("depths and lengths must be (N,) and offsets (B + 1,)")
-            steps = torch.arange(depths.shape[0], device=depths.device)
-            ray = (torch.searchsorted(offsets, steps, right=True) - 1).clamp(0, max(B - 1, 0))
-            if B == 0:
-                ray = ray[:0]
-        d = depths.detach().reshape(-1)
-        points = torch.addcmul(rays.origins[ray], d[:ray.numel(), None], rays.dirs[ray])
+            # Room that no ray covers may hold anything, and so may a ray without samples: such steps,
+            # ray -1 or B, are those of one more ray, of zeros (a depth that is not a number there is
+            # a place like any other to the lookup).
+            ray = torch.searchsorted(offsets, torch.arange(depths.shape[0], device=depths.device),
+                                     right=True) - 1
+            origins, dirs, viewdirs = (nn.functional.pad(t, (0, 0, 0, 1))
+                                       for t in (origins, dirs, viewdirs))
+            lengths = torch.where((ray >= 0) & (ray < B), lengths, 0.0)
+        points = torch.addcmul(origins[ray], depths.detach().reshape(-1, 1), dirs[ray])
         records = self.tree(points) if cache is None else cache(points)
         sigma = records[:, -1]
         sigma = nn.functional.softplus(sigma - 1.0) if self.density_softplus else sigma.relu()
         rgb = records[:, :-1]
         if fmt.format == DataFormat.SH:
             n = fmt.basis_dim
-            basis = eval_sh_bases(int(round(n ** 0.5)) - 1, rays.viewdirs)
+            basis = eval_sh_bases(int(round(n ** 0.5)) - 1, viewdirs)
             some = slice(opt.min_comp, opt.max_comp + 1)
             rgb = (rgb.reshape(rgb.shape[0], rgb.shape[1] // n, n)[..., some] *
                    basis[ray][:, None, some]).sum(dim=-1)
@@ -336,7 +341,7 @@ class VolumeRenderer(nn.Module):
         if offsets is None:
             shape = (B, depths.shape[1])
             return composite(rgb.reshape(*shape, rgb.shape[-1]), sigma.reshape(shape) * lengths, background)
-        return composite(rgb, sigma * lengths[:ray.numel()], background, offsets)
+        return composite(rgb, sigma * lengths, background, offsets)
 
     def se_grad(self, rays: Rays, colors):
         """Rendered colour, gradient and Gauss-Newton diagonal of the total squared error

@@ -185,3 +185,40 @@ def test_refusals_gpu(cuda_device):
     assert renderer.render_samples(none, d[:0], d[:0]).shape == (0, 3)
     assert renderer.render_samples(none, d[0, :0], d[0, :0], o[:1]).shape == (0, 3)
     assert (renderer.render_samples(rays, d[:, :0], d[:, :0]) == 1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("junk", [float("nan"), float("inf")])
+def test_buffers_that_are_not_full(cuda_device, junk):
+    """Room for more samples than there are, and whatever lies there: the same colours and gradients as
+    where only the samples themselves are given, and no gradient in the room that is left."""
+    tree, rays, gen = scene("SH4", cuda_device)
+    renderer = svox.VolumeRenderer(tree)
+    n = torch.randint(0, 60, (70,), generator=gen)
+    n[0] = n[69] = 0            # (the rays next to the room, and nothing of them is known)
+    for t in rays:
+        t[0] = t[69] = float("nan")
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), n.cumsum(0)])
+    N, lo, hi = int(offsets[-1]), 13, 29
+    some = torch.cat([torch.linspace(1.2, 1.8, int(k)) for k in n]), torch.rand(N, generator=gen) * 0.05
+    d = torch.randn(70, 3, generator=gen).to(cuda_device)
+    got = []
+    for room in (False, True):
+        depths, lengths, o = *some, offsets
+        if room:
+            def wide(t):
+                out = torch.full((lo + N + hi,), junk)
+                out[lo:lo + N] = t
+                return out
+            depths, lengths, o = wide(depths), wide(lengths), offsets + lo
+        lengths = lengths.to(cuda_device).requires_grad_(True)
+        out = renderer.render_samples(rays, depths.to(cuda_device), lengths, o.to(cuda_device))
+        got.append([out, *torch.autograd.grad(out, [tree.data, lengths], d)])
+    assert all(t.isfinite().all() for t in got[1])
+    # (samples at another place of the arrays are summed in another order: either side is off from the
+    # sums by at most the tolerances of test_render_samples, with its scales, so twice those between them)
+    for a, b, scale in ((got[0][0], got[1][0], 1), (got[0][1], got[1][1], 10),
+                        (got[0][2], got[1][2][lo:lo + N], 50 * 3)):
+        assert (a - b).abs().max() <= 2 * tolerance(60) * scale * max(1.0, a.abs().max().item())
+    assert (got[1][2][:lo] == 0).all() and (got[1][2][lo + N:] == 0).all()
+    assert csrc.device_status() == 0
