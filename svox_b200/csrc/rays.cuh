@@ -433,6 +433,7 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
                 T_end = total;
                 behind = past(T_end, bg, 0.f);
             }
+            const float front = T;
             float W[4], c[4], Wc[4], own[4];
             unsigned none = 0;          // samples that have no gradient of their thickness
 #pragma unroll
@@ -446,13 +447,15 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
                 own[i] = p.weighted ? 0.f : T * c[i];
             }
             if (!finite((c[0] + c[1]) + (c[2] + c[3]))) {
-                // What is not finite counts only where it has weight; where there is no thickness it
-                // is no sample, and behind an opaque one neither.
+                // What is not finite counts only where it has weight, and past its sample only what
+                // that lets through; where there is no thickness it is no sample.
+                float past_it = front;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     Wc[i] = times(W[i], c[i]);
-                    if (!finite(c[i]) && !p.weighted && (gv[i] == 0.f || W[i] == 0.f))
-                        none |= 1u << i;
+                    past_it *= gate[i].a;
+                    if (!p.weighted) own[i] = times(past_it, c[i]);
+                    if (!finite(c[i]) && !p.weighted && gate[i].w == 0.f) none |= 1u << i;
                 }
             }
             const float here = th.from((Wc[0] + Wc[1]) + (Wc[2] + Wc[3])) + behind;

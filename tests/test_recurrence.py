@@ -935,3 +935,29 @@ def test_saved_tensors_in_another_order(cuda_device, C, H):
                lambda t: t[None]):
         with pytest.raises(RuntimeError, match="saved tensor"):
             grads(to)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [1, 3, 4, 32, 300])
+@pytest.mark.parametrize("place", [0, 1, 2])
+def test_an_opaque_sample_of_infinite_value(cuda_device, C, place):
+    """Its thickness has no gradient (nothing is behind it, and none of it gets past): wherever the
+    arrays lie."""
+    gen = torch.Generator().manual_seed(C)
+    x, g = inputs(gen, (9, 40), C, 1, F32, F32, cuda_device)
+    at = [0, 1, 2, 3, 13, 17, 22, 31, 39]
+    for row, k in enumerate(at):
+        g[row, k] = float("inf")
+        x[row, k, C // 2] = float("inf")
+    bg = torch.rand(9, C, generator=gen).to(cuda_device)
+    d = torch.rand(9, C, generator=gen).to(cuda_device) + 0.5
+    where = (lambda t: t.detach().clone(), off_boundary, on_columns)[place]
+    leaves = [where(t).requires_grad_(True) for t in (x, g, bg)]
+    out = svox.composite(*leaves)
+    dx, dg, db = torch.autograd.grad(out, leaves, d)
+    want = reference(x, g, bg, None, True, False, None, d)
+    for row, k in enumerate(at):
+        assert out[row, C // 2] == float("inf")
+        assert (dg[row, k:] == 0).all() and (dx[row, k + 1:] == 0).all() and (db[row] == 0).all()
+        part = slice(row, row + 1)
+        close("d_values", dx[part], [v[part] for v in want["d_values"]])
