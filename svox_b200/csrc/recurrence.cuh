@@ -152,11 +152,31 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 __device__ __forceinline__ F2 past2(F2 a, F2 h, F2 b) {
     return {past(a.x, h.x, b.x), past(a.y, h.y, b.y)};
 }
-// The product of a stretch's gates and those of the stretch before it: 0 where its own are, whatever
-// the others.
+// The product of the gates of two neighbouring stretches.  It is 0 where one of them is, whatever the
+// other, and only there: a product of many gates that rounds to 0 is held as the smallest float, so
+// that a stretch of 0 has an opaque step, which nothing gets past, while a state that is not a number
+// gets past any other.  (It need not be a number where a gate is not: what its stretch adds is not
+// either.)
+constexpr float kLeast = 1.4e-45f;
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float r;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ F2 gates2(F2 a, F2 before) {
     const F2 r = mul2(a, before);
-    return {a.x == 0.f ? 0.f : r.x, a.y == 0.f ? 0.f : r.y};
+    return {fmaxf(r.x, min3(a.x, before.x, kLeast)), fmaxf(r.y, min3(a.y, before.y, kLeast))};
+}
+// The same of the product A of a stretch's steps (without a gate for each channel both are the same).
+__device__ __forceinline__ float least8(float a, float b, float c, float d, float e, float f, float g,
+                                        float h) {
+    return min3(min3(a, b, c), min3(d, e, f), min3(g, h, kLeast));
+}
+template <bool PC>
+__device__ __forceinline__ void keep_open(F2& A, const F2 (&a)[8]) {
+    A.x = fmaxf(A.x, least8(a[0].x, a[1].x, a[2].x, a[3].x, a[4].x, a[5].x, a[6].x, a[7].x));
+    A.y = !PC ? A.x : fmaxf(A.y, least8(a[0].y, a[1].y, a[2].y, a[3].y, a[4].y, a[5].y, a[6].y,
+                                        a[7].y));
 }
 __device__ __forceinline__ F2 shfl2(F2 v, int lane) {
     return {__shfl_sync(~0u, v.x, lane), __shfl_sync(~0u, v.y, lane)};
@@ -493,8 +513,8 @@ struct ScanThread {
 
 // Joins the pairs of a warp's groups of lanes.  In: (A, B) of this lane's steps.  Out: what the
 // warp's steps before them (BACK: behind them, from the other end) do to the state, and the pair of
-// all.
-template <bool BACK>
+// all (TA only if ALL).
+template <bool BACK, bool PC, bool ALL = true>
 __device__ __forceinline__ void join_lanes(int lanes, int lane, F2& A, F2& B, F2& TA, F2& TB) {
     if (lanes == 32) {
         TA = A;
@@ -503,19 +523,23 @@ __device__ __forceinline__ void join_lanes(int lanes, int lane, F2& A, F2& B, F2
         B = two(0.f);
         return;
     }
+    // (without a gate for each channel both are the same)
+    auto shfl_a = [&](int from) {
+        return PC ? shfl2(A, from) : two(__shfl_sync(~0u, A.x, from));
+    };
     for (int d = lanes; d < 32; d *= 2) {
         const int from = BACK ? lane + d : lane - d;
-        const F2 a = shfl2(A, from & 31), b = shfl2(B, from & 31);
+        const F2 a = shfl_a(from & 31), b = shfl2(B, from & 31);
         if (from >= 0 && from < 32) {
             B = past2(A, b, B);
             A = gates2(A, a);
         }
     }
     const int edge = BACK ? lane & (lanes - 1) : 32 - lanes + (lane & (lanes - 1));
-    TA = shfl2(A, edge);
+    if (ALL) TA = shfl_a(edge);
     TB = shfl2(B, edge);
     const int by = BACK ? lane + lanes : lane - lanes;
-    A = shfl2(A, by & 31);
+    A = shfl_a(by & 31);
     B = shfl2(B, by & 31);
     if (by < 0 || by >= 32) {
         A = two(1.f);
@@ -581,7 +605,7 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
     };
     for (int i = 0; i < p.stages - 1; ++i) issue();
     F2 carry = MODE == 0 ? th.ranges(p, pairs, th.start(p), false, &s_pair[0][0][0]) : two(0.f);
-    F2 through = two(1.f);              // MODE 1, 2: with carry, the pair so far
+    F2 through = two(1.f);              // MODE 1, 2: with carry, the pair so far (of the first warp)
     VT* out = states == nullptr ? nullptr
         : states + (th.row.first + th.place(p, first * th.chunk + th.step0)) * p.C + th.ch;
     float* keep = kept == nullptr || th.wseg != 0 || th.sub != 0 ? nullptr
@@ -621,6 +645,7 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
         // What is not finite stays so to the end of the stretch; then the steps that do not count
         // are told from those that do, in a loop of its own.
         bool odd = spoilt(A, B) != 0.f;
+        keep_open<PC>(A, a);
         if (odd) {
             A = two(1.f);
             B = two(0.f);
@@ -642,7 +667,7 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
             keep += p.C;
         }
         F2 TA, TB;
-        join_lanes<BACK>(Th::lanes_of(p), th.lane, A, B, TA, TB);
+        join_lanes<BACK, PC>(Th::lanes_of(p), th.lane, A, B, TA, TB);
         F2 h = carry;
         if (Th::warps_of(p) == 1) {
             carry = past2(TA, carry, TB);
@@ -651,7 +676,7 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
             auto& pair = s_pair[i & 1];
             if (th.sub == 0) pair[th.warp][th.cl] = make_float4(TA.x, TA.y, TB.x, TB.y);
             th.unit_sync(p);
-            const F2 before = carry, through_before = through;
+            const F2 before = carry;
             const float4* const all = &pair[th.group * Th::warps_of(p)][th.cl];
 #pragma unroll 8
             for (int j = 0; j < Th::warps_of(p); ++j) {
@@ -659,17 +684,20 @@ scan_kernel(ScanArgs p, const VT* __restrict__ x, float2* __restrict__ pairs,
                 if (w == th.wseg) h = carry;
                 const float4 q = all[w * 32];
                 carry = fma2({q.x, q.y}, carry, {q.z, q.w});
-                if (MODE != 0) through = mul2(through, {q.x, q.y});
             }
+            if (MODE != 0 && th.wseg == 0)
+#pragma unroll 8
+                for (int w = 0; w < Th::warps_of(p); ++w) {
+                    const float2 q = *reinterpret_cast<const float2*>(&all[w * 32]);
+                    through = gates2({q.x, q.y}, through);
+                }
             if (spoilt(carry, carry) != 0.f) {
                 carry = before;
-                through = through_before;
                 for (int j = 0; j < Th::warps_of(p); ++j) {
                     const int w = BACK ? Th::warps_of(p) - 1 - j : j;
                     if (w == th.wseg) h = carry;
                     const float4 q = all[w * 32];
                     carry = past2({q.x, q.y}, carry, {q.z, q.w});
-                    if (MODE != 0) through = gates2({q.x, q.y}, through);
                 }
             }
         }
@@ -815,6 +843,7 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
 #pragma unroll
             for (int l = L - 1; l >= 0; --l) E = mul2(a[l], add2(E, th.at(td, l)));
         bool odd = spoilt(A, B) != 0.f || spoilt(E, E) != 0.f;
+        keep_open<PC>(A, a);
         if (odd) {
             F2 al, ul;
             A = two(1.f);
@@ -832,8 +861,8 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
             }
         }
         F2 EA = A, TA, TB, TE, all_a;
-        join_lanes<false>(Th::lanes_of(p), th.lane, A, B, TA, TB);
-        join_lanes<true>(Th::lanes_of(p), th.lane, EA, E, all_a, TE);
+        join_lanes<false, PC>(Th::lanes_of(p), th.lane, A, B, TA, TB);
+        join_lanes<true, PC, false>(Th::lanes_of(p), th.lane, EA, E, all_a, TE);
         F2 G = R;
         if (Th::warps_of(p) == 1) {
             R = past2(TA, R, TE);

@@ -31,7 +31,9 @@ def gated_scan(values, thickness, initial=None, offsets=None, reverse=False, pre
     ``states`` is shaped and typed like ``values``; ``last``, ``(B, C)``, is float32, as is the state
     that is carried: pass it as ``initial`` to go on, one step at a time if need be.  Steps that no
     row covers have states and gradients of zero.  A step of no thickness adds nothing whatever its
-    value (NaN included), and nothing from before a step of infinite thickness gets past it.
+    value (NaN included), and nothing from before a step of infinite thickness (of more than about 87,
+    whose ``exp(-thickness)`` is 0 in 32 bits) gets past it; a state that is not a number gets past any
+    other.
 
     Differentiable, once, with respect to ``values``, ``thickness`` and ``initial``.  Offsets are
     read on the device: one out of order or range is cut to it and noticed by

@@ -961,3 +961,40 @@ def test_an_opaque_sample_of_infinite_value(cuda_device, C, place):
         assert (dg[row, k:] == 0).all() and (dx[row, k + 1:] == 0).all() and (db[row] == 0).all()
         part = slice(row, row + 1)
         close("d_values", dx[part], [v[part] for v in want["d_values"]])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,C,H", [(1, 6000, 64, 64), (1, 6000, 64, 2), (2, 700, 70, 70), (3, 90, 6, 1),
+                                     (3, 90, 6, 3), (1, 6000, 5, 1), (400, 40, 8, 8), (40, 300, 130, 1)])
+@pytest.mark.parametrize("thick", [0.4, 20.0])
+def test_not_a_number_stays(cuda_device, B, T, C, H, thick):
+    """Only a step that is opaque by itself ends it, not many that together leave nothing of a finite
+    amount, however the steps are shared out: forwards for the states, backwards for the gradients."""
+    gen = torch.Generator().manual_seed(T + C)
+    for bad in (float("nan"), float("inf")):
+        x, g = inputs(gen, (B, T), C, H, F32, F32, cuda_device)
+        g = torch.rand(g.shape, generator=gen).to(cuda_device) * thick + thick / 2
+        x[:, 0] = bad
+        h0 = torch.rand(B, C, generator=gen).to(cuda_device)
+        d_states = torch.rand(B, T, C, generator=gen).to(cuda_device)
+        leaves = [t.clone().requires_grad_(True) for t in (x, g, h0)]
+        states, last = svox.gated_scan(*leaves)
+        assert not states.isfinite().any() and not last.isfinite().any()
+        if bad == float("inf"):
+            assert (last == bad).all() and (states == bad).all()
+        x[:, 0] = 1.0
+        leaves = [t.clone().requires_grad_(True) for t in (x, g, h0)]
+        states, last = svox.gated_scan(*leaves)
+        d_states[:, -1] = bad
+        grads = torch.autograd.grad((states, last), leaves, (d_states, torch.rand_like(last)))
+        for t in grads[:1] + grads[2:]:
+            assert not t.isfinite().any()
+            if bad == float("inf"):
+                assert (t == bad).all()
+        # an opaque step ends it
+        k = T * 2 // 3
+        g[:, k] = float("inf")
+        x[:, 0] = bad
+        states, last = svox.gated_scan(x, g, h0)
+        assert not states[:, :k].isfinite().any()
+        assert states[:, k:].isfinite().all() and last.isfinite().all()
