@@ -43,34 +43,45 @@ __device__ __forceinline__ Gate gate_of(float g) {
 }
 
 // What reaches beyond each lane's N samples, and `reach` what reaches the group.  Behind an opaque
-// sample nothing counts, a thickness that is not a number either: where one spoils a product, the
-// gates behind a 0 are closed first.
+// sample nothing counts, a thickness that is not a number neither, and behind such a thickness nothing
+// is known up to the next opaque sample.  `careful`: some product here is not a number, so that the
+// lanes tell what is in front of what (and the gates of samples that nothing reaches are closed).
 template <int G, int N>
-__device__ __forceinline__ float reach_beyond(int lane, float reach, Gate (&gate)[N]) {
-    auto scan = [&](bool careful) {
-        float v = gate[0].a;
-        if (N == 4 && !careful) v = (gate[0].a * gate[1 % N].a) * (gate[2 % N].a * gate[3 % N].a);
-        if (careful)
+__device__ __forceinline__ float reach_beyond(int lane, float reach, Gate (&gate)[N], bool& careful) {
+    float v = gate[0].a;
+    if (N == 4) v = (gate[0].a * gate[1 % N].a) * (gate[2 % N].a * gate[3 % N].a);
 #pragma unroll
-            for (int i = 1; i < N; ++i) v = v == 0.f ? 0.f : v * gate[i].a;
+    for (int d = 1; d < G; d *= 2) {
+        const float o = __shfl_up_sync(~0u, v, d, G);
+        if (lane >= d) v *= o;
+    }
+    v *= reach;
+    careful = __any_sync(~0u, v != v);
+    if (careful) {
+        // of the lane's samples, then of all up to them: what is left of 1, and whether one is opaque
+        float left = 1.f;
+        bool opaque = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            opaque |= gate[i].a == 0.f;
+            left = left == 0.f || gate[i].a == 0.f ? 0.f : left * gate[i].a;
+        }
 #pragma unroll
         for (int d = 1; d < G; d *= 2) {
-            const float o = __shfl_up_sync(~0u, v, d, G);
-            if (lane >= d) v = careful && o == 0.f ? 0.f : v * o;
+            const float o = __shfl_up_sync(~0u, left, d, G);
+            const bool shut = __shfl_up_sync(~0u, opaque, d, G);
+            if (lane < d) continue;
+            left = o == 0.f || (o != o && opaque) ? 0.f : o * left;
+            opaque |= shut;
         }
-        return v;
-    };
-    float v = reach * scan(false);
-    if (__any_sync(~0u, v != v)) {
-        const float all = scan(true);
-        float front = __shfl_up_sync(~0u, all, 1, G);
-        front = reach == 0.f ? 0.f : lane > 0 ? reach * front : reach;
+        if (v != v) v = reach == 0.f || (reach != reach && opaque) ? 0.f : reach * left;
+        float front = __shfl_up_sync(~0u, v, 1, G);
+        if (lane == 0) front = reach;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (front == 0.f) gate[i] = Gate{0.f, 0.f};
-            else front *= gate[i].a;
+            front = gate[i].a == 0.f ? 0.f : front * gate[i].a;
         }
-        v = reach * scan(false);
     }
     return v;
 }
@@ -134,7 +145,8 @@ ray_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
         th.g += dg;
         if (keep != nullptr && in) *keep++ = reach;
         Gate gates[1] = {gate_of(gi)};
-        const float v = reach_beyond<G>(th.lane, reach, gates);
+        bool careful;
+        const float v = reach_beyond<G>(th.lane, reach, gates, careful);
         const Gate gate = gates[0];
         float T = __shfl_up_sync(~0u, v, 1, G);
         if (th.lane == 0) T = reach;
@@ -204,7 +216,8 @@ ray_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restr
         th.x -= step_x;
         th.g -= step_g;
         Gate gates[1] = {gate_of(gi)};
-        const float v = reach_beyond<G>(th.lane, reach, gates);
+        bool careful;
+        const float v = reach_beyond<G>(th.lane, reach, gates, careful);
         const Gate gate = gates[0];
         float T = __shfl_up_sync(~0u, v, 1, G);
         if (th.lane == 0) T = reach;
@@ -360,7 +373,8 @@ quad_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
                 gv[i] = th.in(at + i) ? gv[i] : 0.f;
                 gate[i] = gate_of(gv[i]);
             }
-            const float v = reach_beyond<G>(th.lane, reach, gate);
+            bool careful;
+            const float v = reach_beyond<G>(th.lane, reach, gate, careful);
             float T = __shfl_up_sync(~0u, v, 1, G);
             if (th.lane == 0) T = reach;
             reach = __shfl_sync(~0u, v, G - 1, G);
@@ -371,6 +385,7 @@ quad_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
 #pragma unroll
                     for (int c = 0; c < C; ++c) acc[c] = fmaf(W, xv[i * C + c], acc[c]);
                 T *= gate[i].a;
+                if (careful && gate[i].a == 0.f) T = 0.f;
             }
         }
 #pragma unroll
@@ -425,7 +440,8 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
                 gv[i] = th.in(at + i) ? gv[i] : 0.f;
                 gate[i] = gate_of(gv[i]);
             }
-            const float v = reach_beyond<G>(th.lane, reach, gate);
+            bool careful;
+            const float v = reach_beyond<G>(th.lane, reach, gate, careful);
             float T = __shfl_up_sync(~0u, v, 1, G);
             if (th.lane == 0) T = reach;
             const float total = __shfl_sync(~0u, v, G - 1, G);
@@ -444,6 +460,7 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
                 W[i] = T * (p.weighted ? (th.in(at + i) ? 1.f : 0.f) : gate[i].w);
                 Wc[i] = W[i] * c[i];
                 T *= gate[i].a;
+                if (careful && gate[i].a == 0.f) T = 0.f;
                 own[i] = p.weighted ? 0.f : T * c[i];
             }
             if (!finite((c[0] + c[1]) + (c[2] + c[3]))) {
@@ -453,7 +470,7 @@ quad_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __rest
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     Wc[i] = times(W[i], c[i]);
-                    past_it *= gate[i].a;
+                    past_it = gate[i].a == 0.f ? 0.f : past_it * gate[i].a;
                     if (!p.weighted) own[i] = times(past_it, c[i]);
                     if (!finite(c[i]) && !p.weighted && gate[i].w == 0.f) none |= 1u << i;
                 }
@@ -556,7 +573,8 @@ row_kernel(ScanArgs p, float* __restrict__ last, float* __restrict__ kept) {
         g_next = th.lane + 32 < left ? to_float(*th.g) : 0.f;
         if (keep != nullptr) keep[k] = reach;
         Gate gates[1] = {gate_of(gi)};
-        const float v = reach_beyond<32>(th.lane, reach, gates);
+        bool careful;
+        const float v = reach_beyond<32>(th.lane, reach, gates, careful);
         const Gate gate = gates[0];
         float T = __shfl_up_sync(~0u, v, 1);
         if (th.lane == 0) T = reach;
@@ -651,7 +669,8 @@ row_back_kernel(ScanArgs p, const float* __restrict__ kept, const float* __restr
             if (th.lane / rows.per == j) c = part;
         }
         Gate gates[1] = {gate_of(gi)};
-        const float v = reach_beyond<32>(th.lane, reach, gates);
+        bool careful;
+        const float v = reach_beyond<32>(th.lane, reach, gates, careful);
         const Gate gate = gates[0];
         float T = __shfl_up_sync(~0u, v, 1);
         if (th.lane == 0) T = reach;

@@ -50,7 +50,9 @@ def composite(values, thickness, background=None, offsets=None, premultiplied=Fa
 
     The last state alone of :func:`gated_scan` run from the far end of each ray, where it starts as
     ``background`` (``(B, C)`` or what broadcasts to it; nothing by default).  Arguments and
-    gradients as there; a ray without samples shows its background.
+    gradients as there; a ray without samples shows its background.  Behind samples that together
+    leave nothing of the light in 32 bits (thicknesses of 87 and more), a value that is not finite may
+    count or not, none of them being opaque by itself.
     """
     if _fwd._current_level >= 0:
         _C.refuse_tangents(values, thickness, background)

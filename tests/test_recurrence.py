@@ -998,3 +998,34 @@ def test_not_a_number_stays(cuda_device, B, T, C, H, thick):
         states, last = svox.gated_scan(x, g, h0)
         assert not states[:, :k].isfinite().any()
         assert states[:, k:].isfinite().all() and last.isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [1, 3, 32, 64, 300])
+@pytest.mark.parametrize("premultiplied", [False, True])
+def test_not_a_number_in_front_of_an_opaque_sample(cuda_device, C, premultiplied):
+    """The colour is not a number then, but what the opaque sample hides has no part in it: no
+    gradient, in `composite` as in `gated_scan`, whatever the sums of thickness in between."""
+    gen = torch.Generator().manual_seed(C)
+    x, g = inputs(gen, (8, 300), C, 1, F32, F32, cuda_device)
+    g = g.clamp(min=0.01)
+    at = [(0, 1), (0, 2), (5, 7), (3, 130), (17, 40), (60, 299), (128, 129), (100, 255)]
+    for row, (k, opaque) in enumerate(at):
+        g[row, k] = float("nan")
+        g[row, opaque] = float("inf")
+    g[3, 40:130] = 30.0                 # (together far more than leaves nothing of a finite amount)
+    bg = torch.rand(8, C, generator=gen).to(cuda_device)
+    d = torch.randn(8, C, generator=gen).to(cuda_device)
+    for place in (lambda t: t.detach().clone(), off_boundary, on_columns):
+        leaves = [place(t).requires_grad_(True) for t in (x, g, bg)]
+        for call in (lambda *v: svox.composite(*v, premultiplied=premultiplied),
+                     lambda *v: svox.gated_scan(*v, reverse=True, premultiplied=premultiplied)[1]):
+            out = call(*leaves)
+            dx, dg, db = torch.autograd.grad(out, leaves, d)
+            for row, (k, opaque) in enumerate(at):
+                assert (dx[row, opaque + 1:] == 0).all() and (dg[row, opaque + 1:] == 0).all()
+                assert (db[row] == 0).all() and dx[row, :k].isfinite().all()
+                # what is in front of it is not hidden, where anything of the light gets there (a
+                # composite counts nothing where 32 bits hold nothing of it)
+                if torch.exp(-g[row, :k].double().sum()) > 2.0 ** -126:
+                    assert out[row].isnan().all() and dx[row, k + 1:opaque + 1].isnan().all()
