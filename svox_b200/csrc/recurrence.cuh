@@ -962,7 +962,8 @@ scan_back_kernel(ScanArgs p, const VT* __restrict__ x, const float2* __restrict_
                 if (wl.y == 0.f && !finite(v.y)) v.y = hb.y;
                 q.x = al.x == 0.f ? 0.f : al.x * (p.weighted ? -hb.x : v.x - hb.x);
                 q.y = al.y == 0.f ? 0.f : al.y * (p.weighted ? -hb.y : v.y - hb.y);
-                give(l, l < mine, mul2(wl, G), mul2(q, G));
+                // (nor has anything a gradient whose state has none)
+                give(l, l < mine, mul2(wl, G), {times(G.x, q.x), times(G.y, q.y)});
                 G = past2(al, G, two(0.f));
             }
         } else if (p.weighted) {

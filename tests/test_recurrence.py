@@ -1029,3 +1029,29 @@ def test_not_a_number_in_front_of_an_opaque_sample(cuda_device, C, premultiplied
                 # composite counts nothing where 32 bits hold nothing of it)
                 if torch.exp(-g[row, :k].double().sum()) > 2.0 ** -126:
                     assert out[row].isnan().all() and dx[row, k + 1:opaque + 1].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,H", [(3, 1), (32, 1), (300, 1), (64, 4), (70, 70)])
+@pytest.mark.parametrize("premultiplied", [False, True])
+def test_hidden_samples_have_no_gradient(cuda_device, C, H, premultiplied):
+    """Behind an opaque sample neither a value nor a thickness has one, whatever the values are."""
+    gen = torch.Generator().manual_seed(C)
+    x, g = inputs(gen, (4, 120), C, H, F32, F32, cuda_device)
+    at = [0, 9, 50, 118]
+    for row, k in enumerate(at):
+        g[row, k] = float("inf")
+        x[row, k + 1::2] = float("nan")
+        x[row, k + 3::4] = float("inf")
+    bg = torch.full((4, C), float("nan"), device=cuda_device)
+    d = torch.randn(4, C, generator=gen).to(cuda_device)
+    leaves = [t.requires_grad_(True) for t in (x, g, bg)]
+    out = svox.composite(*leaves, premultiplied=premultiplied)
+    dx, dg, db = torch.autograd.grad(out, leaves, d)
+    assert (db == 0).all()
+    for row, k in enumerate(at):
+        assert (dx[row, k + 1:] == 0).all() and (dg[row, k + 1:] == 0).all()
+        part = slice(row, row + 1), slice(0, k + 1)
+        want = reference(x[part], g[part], None, None, True, premultiplied, None, d[part[0]])
+        close("d_values", dx[part], want["d_values"])
+        close("d_thickness", dg[part], want["d_thickness"])
