@@ -27,21 +27,6 @@ namespace svoxb {
 constexpr int kRayBlock = 64;       // (rays differ in length: blocks of few wait for few)
 constexpr int kRayChannels = 4;     // of those whose channels are summed in every lane
 
-// a = exp(-g) and w = 1 - a for products of many a.  The hardware's power of two is off to one side
-// near 1, by about 1e-8, and so is the nearest float to log2(e): over 200 samples that made 2e-6 of
-// what reaches the background.  Near 1, a comes from the series of w, rounded to nearest, and log2(e)
-// in two parts.
-struct Gate { float a, w; };
-__device__ __forceinline__ Gate gate_of(float g) {
-    const float s = g * fmaf(g, fmaf(g, fmaf(g, fmaf(g, fmaf(g, -1.f / 720, 1.f / 120), -1.f / 24),
-                                            1.f / 6), -0.5f), 1.f);
-    constexpr double log2e = 1.4426950408889634;
-    constexpr float most = (float)log2e, rest = (float)(log2e - most);
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(g, -most, g * -rest)));
-    return fabsf(g) < 0.25f ? Gate{1.f - s, s} : Gate{e, 1.f - e};
-}
-
 // What reaches beyond each lane's N samples, and `reach` what reaches the group.  Behind an opaque
 // sample nothing counts, a thickness that is not a number neither, and behind such a thickness nothing
 // is known up to the next opaque sample.  `careful`: some product here is not a number, so that the

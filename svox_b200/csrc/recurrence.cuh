@@ -104,19 +104,24 @@ __device__ __forceinline__ void store_some(T* to, const float (&from)[V]) {
     *reinterpret_cast<Some<T, V>*>(to) = s;
 }
 
-// a = exp(-g) by the hardware's power of two: 2 ulp of its own and g * 2^-24 from the product, an
-// error that a itself outweighs (g exp(-g) < 0.4).
-__device__ __forceinline__ float decay_of(float g) {
-    float a;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(g * -1.4426950408889634f));
-    return a;
-}
-// w = 1 - exp(-g): near 0, where the difference would cancel, by its Taylor series (the first term
-// left out is below 2^-24 of the sum).
-__device__ __forceinline__ float weight_of(float g, float a) {
-    const float s = g * fmaf(g, fmaf(g, fmaf(g, fmaf(g, fmaf(g, -1.f / 720, 1.f / 120), -1.f / 24),
-                                            1.f / 6), -0.5f), 1.f);
-    return fabsf(g) < 0.25f ? s : 1.f - a;
+// a = exp(-g) and w = 1 - a.  Up to kThin, where the difference would cancel, w comes from a
+// polynomial g (1 + c1 g + ... + c4 g^4), the best of its degree there (off by 2.7e-9 of w, and by
+// 1.6 u with its rounding, u = 2^-24), and a from w, rounded to nearest: the hardware's power of two is
+// off to one side near 1, by about 1e-8, and so is the nearest float to log2(e).  That made 2e-6 of what
+// reaches a background behind 200 samples, and 4e-4 of a state behind 2^17 thin steps, now 2e-5.
+// Beyond, where few steps leave nothing, a is off by 2 ulp of the power of two and g u from its
+// argument, an error that a itself outweighs (g exp(-g) < 0.4).
+constexpr float kThin = 0.25f;
+constexpr float kThin1 = -0.49999964f, kThin2 = 0.16665322f, kThin3 = -0.041502316f,
+                kThin4 = 0.0075347046f;
+struct Gate { float a, w; };
+__device__ __forceinline__ Gate gate_of(float g) {
+    const float s = g * fmaf(g, fmaf(g, fmaf(g, fmaf(g, kThin4, kThin3), kThin2), kThin1), 1.f);
+    constexpr double log2e = 1.4426950408889634;
+    constexpr float most = (float)log2e, rest = (float)(log2e - most);
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(g, -most, g * -rest)));
+    return fabsf(g) < kThin ? Gate{1.f - s, s} : Gate{e, 1.f - e};
 }
 __device__ __forceinline__ float times(float w, float x) { return w == 0.f ? 0.f : w * x; }
 // a h + b, with nothing of h where a is 0
@@ -186,21 +191,20 @@ __device__ __forceinline__ float spoilt(F2 a, F2 b) {
     const F2 r = fma2(a, two(0.f), mul2(b, two(0.f)));
     return r.x + r.y;
 }
-__device__ __forceinline__ F2 decay2(F2 g) {
+// gate_of of two channels (with log2(e) in one part: an argument's own rounding is as large).
+__device__ __forceinline__ void gates_of(F2 g, F2& a, F2& w) {
     const F2 t = mul2(g, two(-1.4426950408889634f));
-    F2 a;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a.x) : "f"(t.x));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a.y) : "f"(t.y));
-    return a;
-}
-__device__ __forceinline__ F2 weight2(F2 g, F2 a) {
-    F2 s = fma2(g, two(-1.f / 720), two(1.f / 120));
-    s = fma2(g, s, two(-1.f / 24));
-    s = fma2(g, s, two(1.f / 6));
-    s = fma2(g, s, two(-0.5f));
+    F2 e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    F2 s = fma2(g, two(kThin4), two(kThin3));
+    s = fma2(g, s, two(kThin2));
+    s = fma2(g, s, two(kThin1));
     s = mul2(g, fma2(g, s, two(1.f)));
-    const F2 d = fma2(a, two(-1.f), two(1.f));
-    return {fabsf(g.x) < 0.25f ? s.x : d.x, fabsf(g.y) < 0.25f ? s.y : d.y};
+    const F2 c = fma2(s, two(-1.f), two(1.f)), d = fma2(e, two(-1.f), two(1.f));
+    const bool x = fabsf(g.x) < kThin, y = fabsf(g.y) < kThin;
+    a = {x ? c.x : e.x, y ? c.y : e.y};
+    w = {x ? s.x : d.x, y ? s.y : d.y};
 }
 
 // Steps of a packed call that no row covers, before the first row and behind the last (a buffer that
@@ -429,14 +433,13 @@ struct ScanThread {
                 v[0] = to_float(g[l * 64 + gate]);
                 v[1] = to_float(g[l * 64 + gate2]);
             }
-            const F2 t{v[0], v[1]};
-            a = decay2(t);
-            w = WEIGHTED ? two(1.f) : weight2(t, a);
+            gates_of({v[0], v[1]}, a, w);
         } else {
-            const float t = to_float(g[l * 32 + gate]);
-            a = two(decay_of(t));
-            w = two(WEIGHTED ? 1.f : weight_of(t, a.x));
+            const Gate t = gate_of(to_float(g[l * 32 + gate]));
+            a = two(t.a);
+            w = two(t.w);
         }
+        if (WEIGHTED) w = two(1.f);
     }
     __device__ __forceinline__ F2 at(const VT* tile_x, int l) const {
         float v[2];
@@ -1038,9 +1041,8 @@ scan_few_kernel(ScanArgs p, VT* __restrict__ states, float* __restrict__ last,
         load_some<W>(x + at * p.xs, xv);
 #pragma unroll
         for (int v = 0; v < W; ++v) {
-            const float gv = to_float(g[at * p.gs + (c + v) / p.D]);
-            const float a = decay_of(gv);
-            h[v] = past(a, h[v], times(p.weighted ? 1.f : weight_of(gv, a), xv[v]));
+            const Gate gate = gate_of(to_float(g[at * p.gs + (c + v) / p.D]));
+            h[v] = past(gate.a, h[v], times(p.weighted ? 1.f : gate.w, xv[v]));
         }
         if (states != nullptr) store_some<W>(states + (b * p.T + at) * p.C + c, h);
     }

@@ -1055,3 +1055,44 @@ def test_hidden_samples_have_no_gradient(cuda_device, C, H, premultiplied):
         want = reference(x[part], g[part], None, None, True, premultiplied, None, d[part[0]])
         close("d_values", dx[part], want["d_values"])
         close("d_thickness", dg[part], want["d_thickness"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,H", [(64, 64), (64, 8), (3, 1)])
+@pytest.mark.parametrize("premultiplied", [False, True])
+def test_thin_gates_over_a_long_sequence(cuda_device, C, H, premultiplied):
+    """2^17 steps of a thickness around 1e-5: errors of single steps that lie to one side would add up
+    to T of them.  Rounded to nearest, a = exp(-g) and the sum of a step are off by at most u / 2 each
+    of a state that stays within 1 (weighted beforehand: of the sum of its terms), to either side
+    as g varies: a random walk of 2 T such steps, each of variance u^2 / 12, that leaves
+    6 sqrt(T / 6) u with a probability of 2e-9; the weights' own error, 3 u of each, adds 3 u.  A product
+    of numbers 1 - p, 1 - q just below 1 rounds up or down to 1 - p - q wherever p q is below u / 2: each
+    stretch of 8 steps loses its 28 pairs, 28 g^2, and the first few of the folds of a range of steps
+    half a u each, of up to 256 ranges below 1.5 g^2 for every step of all: 5 T g^2 together."""
+    gen = torch.Generator().manual_seed(C + H)
+    T = 1 << 17
+    g = (torch.rand(1, T, H, generator=gen) * 1.9 + 0.1) * 1e-5
+    x = torch.full((1, T, C), 0.75)
+    if premultiplied:
+        x *= 1e-5
+    h0 = torch.full((1, C), 0.5)
+    args = [t.to(cuda_device).requires_grad_(True) for t in (x, g, h0)]
+    states, last = svox.gated_scan(*args, premultiplied=premultiplied)
+    d = torch.ones(1, C, device=cuda_device)
+    grads = torch.autograd.grad(last, args, d)
+    gates = g[0].double().repeat_interleave(C // H, 1)
+    upto = gates.cumsum(0)
+    if premultiplied:       # (a sum of positive terms by the share that remains of each)
+        want = torch.exp(-upto[-1]) * 0.5 + \
+            (torch.exp(upto - upto[-1]) * x[0].double()).sum(0)
+        mid = torch.exp(-upto[T // 2]) * 0.5 + \
+            (torch.exp(upto[:T // 2 + 1] - upto[T // 2]) * x[0, :T // 2 + 1].double()).sum(0)
+    else:                   # (a constant value: what is not the first state is that)
+        want, mid = (0.75 - 0.25 * torch.exp(-upto[k]) for k in (-1, T // 2))
+    tol = ((6 * (T / 6) ** 0.5 + 3) * U + 5 * T * 1.05e-5 ** 2) * max(1.0, float(want.max()))
+    assert (last[0].cpu().double() - want).abs().max() <= tol
+    assert (states[0, T // 2].cpu().double() - mid).abs().max() <= tol
+    assert (grads[2][0].cpu().double() - torch.exp(-upto[-1])).abs().max() <= tol
+    through = torch.exp(upto - upto[-1])
+    dx = through if premultiplied else through * -torch.expm1(-gates)
+    assert ((grads[0][0].cpu().double() - dx).abs() <= tol * dx / through).all()
