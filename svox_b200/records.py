@@ -69,7 +69,8 @@ class RecordCache(nn.Module):
         return (f"records={len(self)}, data_dim={self.data_dim}, dtype={self.dtype}, "
                 f"group={self.group}")
 
-    # What the bytes mean goes with them: a state of another kind of cache is refused.
+    # What the bytes mean goes with them: a state of another kind of cache is refused, and a state is
+    # taken whole or not at all.
     def get_extra_state(self):
         return {"data_dim": self.data_dim, "group": self.group, "dtype": str(self.dtype)}
 
@@ -77,6 +78,32 @@ class RecordCache(nn.Module):
         mine = self.get_extra_state()
         if state != mine:
             raise RuntimeError(f"the state is that of a record cache with {state}, this one has {mine}")
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys,
+                              unexpected_keys, error_msgs):
+        # (buffers are copied before set_extra_state is called)
+        try:
+            self._check_state({k[len(prefix):]: v for k, v in state_dict.items()
+                               if k.startswith(prefix)})
+        except RuntimeError as error:
+            error_msgs.append(str(error))
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys,
+                                      unexpected_keys, error_msgs)
+
+    def _check_state(self, state):
+        names = ["child", "offset", "invradius", "records"]
+        given = [name for name in (*names, "_extra_state") if name in state]
+        if not given:
+            return              # (the state of something else: for `strict` to judge)
+        if len(given) <= len(names):
+            raise RuntimeError(f"the state of a record cache has only {', '.join(given)}")
+        self.set_extra_state(state["_extra_state"])
+        for name in names:
+            new, old = state[name], self._buffers[name]
+            if new.shape != old.shape or new.dtype != old.dtype:
+                raise RuntimeError(f"{name} of the state of a record cache is {tuple(new.shape)} "
+                                   f"{new.dtype}, here {tuple(old.shape)} {old.dtype}")
 
     def _write(self, where, points, values, offset, scaling):
         b = self._buffers

@@ -366,3 +366,33 @@ def test_abi_refusals():
     r.owner = 16
     assert lib.svoxb_records_write(C.byref(r), None, C.c_void_p(16), C.c_int64(4), C.c_void_p(16),
                                    C.c_int32(0), None, None) == 1               # no workspace
+
+
+@pytest.mark.gpu
+def test_a_refused_state_changes_nothing(cuda_device):
+    """A cache's state is taken whole or not at all, on its own and as a part of another module."""
+    kind = svox.RecordCache(make_tree("SH4", cuda_device, refine=2), dtype=E4M3)
+    kind.invradius *= 0.5
+    other = svox.RecordCache(make_tree("SH4", cuda_device, refine=2))
+    larger = svox.RecordCache(make_tree("SH4", cuda_device, refine=3), dtype=E4M3)
+    state = other.state_dict()
+    unsaid = {k: v for k, v in kind.state_dict().items() if k != "_extra_state"}
+    part = {k: v for k, v in kind.state_dict().items() if k != "child"}
+    before = {k: v.clone() for k, v in kind.state_dict().items() if k != "_extra_state"}
+    for bad in (state, larger.state_dict(), unsaid, part):
+        bad = {k: torch.zeros_like(v) + 1 if k == "records" else v for k, v in bad.items()}
+        for strict in (True, False):
+            with pytest.raises(RuntimeError):
+                kind.load_state_dict(bad, strict=strict)
+            holder = torch.nn.ModuleDict({"cache": kind})
+            with pytest.raises(RuntimeError):
+                holder.load_state_dict({"cache." + k: v for k, v in bad.items()}, strict=strict)
+            for k, v in before.items():
+                assert torch.equal(kind.state_dict()[k], v), k
+    # a state of something else without a word of the cache, and its own
+    torch.nn.ModuleDict({"cache": kind}).load_state_dict({}, strict=False)
+    twin = svox.RecordCache(make_tree("SH4", cuda_device, refine=2), dtype=E4M3)
+    twin.write(torch.arange(50, device=cuda_device), torch.ones(50, 13, device=cuda_device))
+    torch.nn.ModuleDict({"cache": twin}).load_state_dict(
+        torch.nn.ModuleDict({"cache": kind}).state_dict())
+    assert torch.equal(twin.read(), kind.read()) and torch.equal(twin.invradius, kind.invradius)
