@@ -403,9 +403,10 @@ enum { SVOXB_TYPE_F32 = 0, SVOXB_TYPE_BF16 = 1, SVOXB_TYPE_F16 = 2 };
  *   offsets == null: every row has T steps, step t of row b lies at
  *     b * values_row + t * values_step (elements; the channels are neighbours).
  *   else rows are packed: row b has the steps [offsets[b], offsets[b+1]) of T
- *     (device memory, B + 1 ascending numbers; an offset out of order or
- *     range is cut to it and recorded as SVOXB_ERR_INDEX in the device
- *     status).  *_row is not used.
+ *     (device memory, B + 1 ascending numbers).  *_row is not used.  An offset
+ *     out of order or range is recorded as SVOXB_ERR_INDEX in the device
+ *     status: no access leaves the arrays then, but the outputs are undefined,
+ *     as rows may overlap.
  * `reverse`: from the last step of a row to its first.  `thickness` has the
  * type of `values` or is float. */
 typedef struct {

@@ -36,8 +36,8 @@ def gated_scan(values, thickness, initial=None, offsets=None, reverse=False, pre
     other.
 
     Differentiable, once, with respect to ``values``, ``thickness`` and ``initial``.  Offsets are
-    read on the device: one out of order or range is cut to it and noticed by
-    ``csrc.check_device_status()``.
+    read on the device: one out of order or range is noticed by ``csrc.check_device_status()``, and
+    the outputs are undefined then (all accesses stay within the arrays).
     """
     if _fwd._current_level >= 0:
         _C.refuse_tangents(values, thickness, initial)
