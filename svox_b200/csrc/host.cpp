@@ -724,6 +724,8 @@ Scan read_scan(const Tensor& values, const Tensor& thickness, const optional<Ten
     if (values.dim() != lead + 1)
         fail(packed ? "values must be (N, C) where offsets are given" : "values must be (B, T, C)");
     if (values.size(lead) < 1) fail("values must have a channel");
+    // (refused here: the library gets them in 32 bits)
+    if (values.size(lead) > 1 << 24) fail("values must have at most 2^24 channels");
     if (thickness.device() != values.device())
         fail("thickness must be on the same device as values");
     if (thickness.scalar_type() != at::kFloat && thickness.scalar_type() != values.scalar_type())

@@ -1096,3 +1096,13 @@ def test_thin_gates_over_a_long_sequence(cuda_device, C, H, premultiplied):
     through = torch.exp(upto - upto[-1])
     dx = through if premultiplied else through * -torch.expm1(-gates)
     assert ((grads[0][0].cpu().double() - dx).abs() <= tol * dx / through).all()
+
+
+def test_sizes_beyond_the_maximum_are_refused():
+    """More channels than the kernels count, beyond 32 bits too."""
+    for C in ((1 << 24) + 1, 1 << 31, (1 << 32) + 64):
+        x = torch.zeros(1).expand(1, 1, C)
+        with pytest.raises(RuntimeError, match="channels"):
+            svox.gated_scan(x, torch.zeros(1, 1))
+        with pytest.raises(RuntimeError, match="channels"):
+            svox.composite(x, torch.zeros(1, 1, 1).expand(1, 1, C))
