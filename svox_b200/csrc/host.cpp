@@ -643,11 +643,14 @@ int32_t element_type(at::ScalarType t) {
     }
 }
 
-// `t` with its last dimension dense (a copy if it is not).
-Tensor dense_rows(const Tensor& t) {
+// `t` with its last dimension dense (a copy if it is not), and its memory holding its values (a view
+// such as z.conj().imag stands for their negatives).
+Tensor dense_rows(const Tensor& view) {
+    const Tensor t = view.resolve_neg();
     const int64_t last = t.dim() - 1;
     return t.size(last) <= 1 || t.stride(last) == 1 ? t : t.contiguous();
 }
+Tensor dense(const Tensor& t) { return t.resolve_neg().contiguous(); }
 
 // What a tensor has to be when it comes back from where the backward pass found it.
 struct Kind {
@@ -757,7 +760,7 @@ Scan read_scan(const Tensor& values, const Tensor& thickness, const optional<Ten
     if (!values.is_cuda()) fail("values must be a CUDA tensor");
     Scan s;
     s.values = dense_rows(values);
-    s.thickness = thickness.dim() == lead + 1 ? dense_rows(thickness) : thickness;
+    s.thickness = thickness.dim() == lead + 1 ? dense_rows(thickness) : thickness.resolve_neg();
     if (packed) s.offsets = offsets->contiguous();
     if (initial) {
         const bool plain = initial->scalar_type() == at::kFloat && initial->dim() == 2 &&
@@ -814,10 +817,10 @@ class ScanNode : public torch::autograd::Function<ScanNode> {
             if (!s.saved[i].fits(saved[i]))
                 fail("a saved tensor of gated_scan came back with another shape, type or device");
         s.values = dense_rows(saved[0]);
-        s.thickness = saved[1].dim() == saved[0].dim() ? dense_rows(saved[1]) : saved[1];
+        s.thickness = saved[1].dim() == saved[0].dim() ? dense_rows(saved[1]) : saved[1].resolve_neg();
         if (saved[2].defined()) s.initial = dense_rows(saved[2]);
         if (saved[3].defined()) s.offsets = saved[3].contiguous();
-        const Tensor kept = saved[4].contiguous();
+        const Tensor kept = dense(saved[4]);
         s.bind();
         svoxb_scan anew = s.c;
         anew.layout = 0;
@@ -828,8 +831,8 @@ class ScanNode : public torch::autograd::Function<ScanNode> {
         }
         const c10::cuda::CUDAGuard guard(s.values.device());
         Tensor d_states, d_last;
-        if (s.states && grads[0].defined()) d_states = grads[0].contiguous();
-        if (grads.back().defined()) d_last = grads.back().contiguous();
+        if (s.states && grads[0].defined()) d_states = dense(grads[0]);
+        if (grads.back().defined()) d_last = dense(grads.back());
         Tensor dx, dg, d0;
         if (ctx->needs_input_grad(0)) dx = at::empty(s.values.sizes(), s.values.options());
         if (ctx->needs_input_grad(1)) dg = at::empty(s.thickness.sizes(), s.thickness.options());

@@ -396,3 +396,18 @@ def test_a_refused_state_changes_nothing(cuda_device):
     torch.nn.ModuleDict({"cache": twin}).load_state_dict(
         torch.nn.ModuleDict({"cache": kind}).state_dict())
     assert torch.equal(twin.read(), kind.read()) and torch.equal(twin.invradius, kind.invradius)
+
+
+@pytest.mark.gpu
+def test_views_of_negatives(cuda_device):
+    """Points and values whose memory holds their negatives."""
+    cache = svox.RecordCache(make_tree("SH4", cuda_device, refine=2))
+    points = torch.rand(200, 3, device=cuda_device)
+    rows = torch.randn(200, 13, device=cuda_device)
+    cache.set(points, rows)
+    want = cache(points)
+    cache.set(points, rows + 1)
+    view = torch._neg_view
+    assert view(-points).is_neg()
+    cache.set(view(-points), view(-rows))
+    assert torch.equal(cache(points), want) and torch.equal(cache(view(-points)), want)

@@ -1106,3 +1106,32 @@ def test_sizes_beyond_the_maximum_are_refused():
             svox.gated_scan(x, torch.zeros(1, 1))
         with pytest.raises(RuntimeError, match="channels"):
             svox.composite(x, torch.zeros(1, 1, 1).expand(1, 1, C))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,H", [(3, 1), (64, 64)])
+def test_views_of_negatives(cuda_device, C, H):
+    """Imaginary parts of a conjugate, whose memory holds their negatives: inputs and gradients."""
+    gen = torch.Generator().manual_seed(C)
+    x, g = inputs(gen, (2, 40), C, H, F32, F32, cuda_device)
+    h0 = torch.randn(2, C, generator=gen).to(cuda_device)
+    d = torch.randn(2, C, generator=gen).to(cuda_device)
+
+    def view(t):
+        t = torch.complex(t, -t).conj().imag
+        assert t.is_neg()
+        return t
+
+    for to in (view, lambda t: torch._neg_view(-t)):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, g, h0)]
+        plain = svox.gated_scan(*leaves)
+        want = torch.autograd.grad(plain[1], leaves, d)
+        states, last = svox.gated_scan(*[to(t.detach()) for t in leaves])
+        assert torch.equal(states, plain[0]) and torch.equal(last, plain[1])
+        for a, b in zip(torch.autograd.grad(svox.gated_scan(*leaves)[1], leaves, to(d)), want):
+            assert torch.equal(a, b)
+        with torch.autograd.graph.saved_tensors_hooks(
+                lambda t: t, lambda t: to(t) if t.dtype == F32 else t):
+            last = svox.gated_scan(*leaves)[1]
+        for a, b in zip(torch.autograd.grad(last, leaves, d), want):
+            assert torch.equal(a, b)
