@@ -643,14 +643,14 @@ int32_t element_type(at::ScalarType t) {
     }
 }
 
-// `t` with its last dimension dense (a copy if it is not), and its memory holding its values (a view
-// such as z.conj().imag stands for their negatives).
-Tensor dense_rows(const Tensor& view) {
-    const Tensor t = view.resolve_neg();
+// `t` with its memory holding its values (a view such as z.conj().imag stands for their negatives).
+Tensor resolved(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor dense(const Tensor& t) { return resolved(t).contiguous(); }
+// And with its last dimension dense (a copy if it is not).
+Tensor dense_rows(const Tensor& t) {
     const int64_t last = t.dim() - 1;
-    return t.size(last) <= 1 || t.stride(last) == 1 ? t : t.contiguous();
+    return t.size(last) <= 1 || t.stride(last) == 1 ? resolved(t) : dense(t);
 }
-Tensor dense(const Tensor& t) { return t.resolve_neg().contiguous(); }
 
 // What a tensor has to be when it comes back from where the backward pass found it.
 struct Kind {
@@ -760,7 +760,7 @@ Scan read_scan(const Tensor& values, const Tensor& thickness, const optional<Ten
     if (!values.is_cuda()) fail("values must be a CUDA tensor");
     Scan s;
     s.values = dense_rows(values);
-    s.thickness = thickness.dim() == lead + 1 ? dense_rows(thickness) : thickness.resolve_neg();
+    s.thickness = thickness.dim() == lead + 1 ? dense_rows(thickness) : resolved(thickness);
     if (packed) s.offsets = offsets->contiguous();
     if (initial) {
         const bool plain = initial->scalar_type() == at::kFloat && initial->dim() == 2 &&
@@ -817,7 +817,7 @@ class ScanNode : public torch::autograd::Function<ScanNode> {
             if (!s.saved[i].fits(saved[i]))
                 fail("a saved tensor of gated_scan came back with another shape, type or device");
         s.values = dense_rows(saved[0]);
-        s.thickness = saved[1].dim() == saved[0].dim() ? dense_rows(saved[1]) : saved[1].resolve_neg();
+        s.thickness = saved[1].dim() == saved[0].dim() ? dense_rows(saved[1]) : resolved(saved[1]);
         if (saved[2].defined()) s.initial = dense_rows(saved[2]);
         if (saved[3].defined()) s.offsets = saved[3].contiguous();
         const Tensor kept = dense(saved[4]);
@@ -1077,7 +1077,8 @@ PYBIND11_MODULE(_host, m) {
 
     m.def("records_read", [](const Tensor& records, const Tensor& child, const Tensor& offset,
                              const Tensor& scaling, int64_t K, int64_t group, int64_t code,
-                             const optional<Tensor>& where, bool points, at::ScalarType type) {
+                             const optional<Tensor>& given, bool points, at::ScalarType type) {
+        const optional<Tensor> where = given ? optional<Tensor>(resolved(*given)) : std::nullopt;
         const svoxb_records r =
             read_records(records, {}, child, offset, scaling, K, group, code);
         const Places at = read_places(where, points, records);
@@ -1093,8 +1094,10 @@ PYBIND11_MODULE(_host, m) {
     });
     m.def("records_write", [](const Tensor& records, const Tensor& owner, const Tensor& child,
                               const Tensor& offset, const Tensor& scaling, int64_t K, int64_t group,
-                              int64_t code, const optional<Tensor>& where, bool points,
-                              const Tensor& values) {
+                              int64_t code, const optional<Tensor>& given, bool points,
+                              const Tensor& rows) {
+        const optional<Tensor> where = given ? optional<Tensor>(resolved(*given)) : std::nullopt;
+        const Tensor values = resolved(rows);
         const svoxb_records r =
             read_records(records, owner, child, offset, scaling, K, group, code);
         const Places at = read_places(where, points, records);

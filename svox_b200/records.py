@@ -115,7 +115,7 @@ class RecordCache(nn.Module):
             values = values.float()
         _C.host().records_write(b["records"], b["_owner"], b["child"], offset, scaling,
                                 self.data_dim, self.group, _CODES[self.dtype], where, points,
-                                values.resolve_neg().contiguous())
+                                values.contiguous())
 
     def _read(self, where, points, dtype, offset, scaling):
         b = self._buffers
@@ -155,4 +155,4 @@ class RecordCache(nn.Module):
         assert points.dim() == 2
         if points.dtype != torch.float32:
             points = points.to(torch.float32)
-        return points.resolve_neg().contiguous()
+        return points.contiguous()
