@@ -84,7 +84,7 @@ RayPlan ray_plan(const svoxb_scan* s) {
     return plan;
 }
 
-// Floats that the forward keeps: the thickness in front of every chunk.  The chunks of quads begin
+// Floats that the forward keeps: what reaches every chunk.  The chunks of quads begin
 // with the ray's first quad, up to three samples in front of it, so that a ray may have one more:
 // two rays never share an entry where ray b begins at first / chunk + 2 b.
 int64_t ray_kept(const svoxb_scan* s, RayPlan plan) {
